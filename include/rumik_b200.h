@@ -477,6 +477,139 @@ typedef struct rb_decode_step {
 int64_t rb_decode_layers_workspace(const rb_decode_step* st);
 int rb_decode_layers(const rb_decode_step* st, int dtype, int flags, void* stream);
 
+/* ---- Several continuations of one prompt: a batch of sequences, their caches, and one step of a beam search ---- */
+
+/* How a cache holds its rows. A row is the head_dim values of one (sequence, slot, key-value head) in `dtype`:
+ *   RB_KV_PLAIN  the values themselves
+ *   RB_KV_INT8   codes + 128 (uint8, the storage of the int8 head) and s = bf16(max|x| / 127), value = code * s,
+ *                code = clamp(rint(x / s), -127, 127)
+ *   RB_KV_INT4   codes packed two a byte, low nibble = even column, and the pair s = bf16((max x - m) / 15), m = min x
+ *                in `dtype`; value = code * s + m, code = clamp(rint((x - m) / s), 0, 15)
+ * s == 0 gives codes of zero. A row that holds a NaN or an infinity (or whose range overflows fp32) has s = NaN and
+ * codes of zero, so that all of it reads as NaN. */
+enum rb_kv_format { RB_KV_PLAIN = 0, RB_KV_INT8 = 1, RB_KV_INT4 = 2 };
+
+/* The caches of one layer, contiguous: k, v [n_seqs, n_kv_heads, cache_len, row] with row = head_dim elements of dtype
+ * (PLAIN), head_dim bytes (INT8) or head_dim / 2 bytes (INT4), 16-byte aligned; k_par, v_par
+ * [n_seqs, n_kv_heads, cache_len]: the bf16 scales (INT8) or 32-bit words with s in the low and m in the high half
+ * (INT4), aligned to their size; NULL for PLAIN. head_dim 64 or 128. */
+typedef struct rb_kv_cache {
+  void* k;
+  void* v;
+  void* k_par;
+  void* v_par;
+  int fmt;              /* rb_kv_format */
+  int dtype;            /* RB_F16 or RB_BF16: what rows are written from and read back as */
+  int64_t n_seqs;
+  int n_kv_heads;       /* 1 .. 256 */
+  int head_dim;         /* 64 or 128 */
+  int64_t cache_len;    /* slots a sequence */
+} rb_kv_cache;
+
+/*
+ * Write rows into the caches, quantised on the way (one launch for keys and values). k and v hold
+ * [n_seqs, n_tokens, n_kv_heads, head_dim] elements of the cache's dtype; *_stride: the element strides of the
+ * sequence, token and head axes (multiples of 8; the last axis has stride 1), bases 16-byte aligned. Token t of
+ * sequence b goes to slot pos[b] + t (pos: int64 [n_seqs] on the device). A token whose slot is outside
+ * [0, cache_len) is not stored and sets RB_DEVERR_ARG.
+ */
+int rb_kv_write(const rb_kv_cache* cache, const void* k, const void* v, const int64_t* k_stride,
+                const int64_t* v_stride, int64_t n_tokens, const int64_t* pos, int flags, void* stream);
+
+/* Read the slots [start, start + count) of every sequence and head back as values of the cache's dtype (fp32
+ * arithmetic, rounded once, clamped to the dtype's finite range): k_out, v_out [n_seqs, n_kv_heads, count, head_dim],
+ * contiguous, 16-byte aligned. */
+int rb_kv_read(const rb_kv_cache* cache, void* k_out, void* v_out, int64_t start, int64_t count, int flags,
+               void* stream);
+
+/*
+ * Decode attention of a batch of sequences over a prefix that they share and over rows of their own, grouped-query
+ * heads:  out[b, h] = softmax(scale q[b, h] . k_j) v_j over the slots j < *prefix_len of `prefix` (n_seqs 1) and the
+ * slots j < own_len[b] of sequence b in `own` (n_seqs as the call's). The prefix is read once for the whole batch, not
+ * once a sequence. A sequence without any slot gets zeros. Either cache may be NULL; both have one format, dtype, head
+ * count and head_dim. 1 <= n_q_heads / n_kv_heads <= 16. Lengths are int64 on the device; a *prefix_len or own_len[b]
+ * outside its cache stores nothing for the sequences it concerns and sets RB_DEVERR_ARG. Rows at or beyond a length are
+ * not looked at. Scores, softmax and sums are fp32; a quantised row enters the products as its codes.
+ * ws: rb_prefix_attn_workspace(...) bytes, 16-byte aligned, zero before the first call; every call leaves its counters
+ * zero. Calls that share a workspace must not overlap in time.
+ */
+typedef struct rb_prefix_attn_args {
+  const void* q;              /* [n_seqs, n_q_heads, head_dim], sequence stride ldq elements (multiple of 8) */
+  int64_t ldq;
+  void* out;                  /* as q, sequence stride ldo */
+  int64_t ldo;
+  int64_t n_seqs;             /* 0 .. 1024 */
+  int n_q_heads;
+  const rb_kv_cache* prefix;
+  const int64_t* prefix_len;  /* [1] */
+  const rb_kv_cache* own;
+  const int64_t* own_len;     /* [n_seqs] */
+  float scale;
+  void* ws;
+  int64_t ws_bytes;
+} rb_prefix_attn_args;
+
+int64_t rb_prefix_attn_workspace(const rb_prefix_attn_args* a);  /* q, out, lengths and ws are not looked at; < 0: -status */
+int rb_prefix_attn(const rb_prefix_attn_args* a, int flags, void* stream);
+
+/*
+ * One selection of a beam search, for `requests` requests of n_beams beams each, in one launch:
+ *   candidates of a live beam b:     (logits[b, v] - log sum_v exp(logits[b, v])) + scores[b]  for every row v
+ *   candidates of a finished beam:   scores[b] for the row end_idx
+ * and the n_beams best of each request, best first: out_scores, out_parents (the beam's index in its request),
+ * out_tokens (the row, or ids[row]) and out_done (the parent was finished, or the row is end_idx). Of two candidates
+ * of one beam the larger logit is first, of equal ones the lower (beam, row). Rows that are masked (a logit of -inf;
+ * end_idx while *step < min_new) and those of a beam whose score is not finite count as -inf and fill up what is left
+ * in (beam, row) order. A live row with a NaN or +inf has no distribution: its rows count as -inf, RB_DEVERR_ARG is set.
+ * logits [requests * n_beams, n_vocab], row stride ld elements (RB_F16 / RB_BF16 / RB_F32); scores fp32, done bytes,
+ * both [requests, n_beams]; outputs [requests, n_beams], none of them an input. ids int64 [n_vocab] or NULL;
+ * step int64 [1] or NULL. 1 <= n_beams <= 32, 1 <= n_vocab <= 2^20.
+ * ws: rb_beam_select_workspace(...) bytes, 16-byte aligned, zero before the first call (a call leaves its counters
+ * zero); calls that share it must not overlap in time.
+ */
+typedef struct rb_beam_select_args {
+  const void* logits;
+  int logits_dtype;
+  int64_t ld;
+  int64_t requests;
+  int n_beams;
+  int64_t n_vocab;
+  int64_t end_idx;
+  const float* scores;
+  const uint8_t* done;
+  const int64_t* ids;
+  const int64_t* step;
+  int64_t min_new;
+  float* out_scores;
+  int64_t* out_parents;
+  int64_t* out_tokens;
+  uint8_t* out_done;
+  void* ws;
+  int64_t ws_bytes;
+} rb_beam_select_args;
+
+int64_t rb_beam_select_workspace(int64_t requests, int n_beams, int64_t n_vocab);
+int rb_beam_select(const rb_beam_select_args* a, int flags, void* stream);
+
+/* One tensor of the beams' state: [requests * n_beams, n_heads, cache_len, row_bytes] bytes, contiguous (a cache's k or
+ * v, or its row parameters). row_bytes even, p aligned to 2 bytes; 16-byte accesses where p, row_bytes and
+ * cache_len * row_bytes are multiples of 16. */
+typedef struct rb_beam_tensor {
+  void* p;
+  int n_heads;
+  int row_bytes;
+} rb_beam_tensor;
+
+/*
+ * Reorder the beams' rows in place: beam c of a request takes over the slots [0, slots[parents[c]]) of its parent, for
+ * every tensor of the list (launches of up to 100 tensors). parents and slots: int64 [requests, n_beams] on the device
+ * (the beams' lengths BEFORE the reordering). Beams that are their own parent are neither read nor written unless
+ * another beam takes them over. A parent outside [0, n_beams) or a length outside [0, cache_len] leaves the request's
+ * rows as they are and sets RB_DEVERR_ARG. 1 <= n_beams <= 32. `tensors` is a host array read during the call.
+ */
+int rb_beam_reorder(const rb_beam_tensor* tensors, int count, int64_t requests, int n_beams, int64_t cache_len,
+                    const int64_t* parents, const int64_t* slots, int flags, void* stream);
+
 /* Human-readable text for a status code (static storage). */
 const char* rb_status_string(int status);
 

@@ -6,6 +6,8 @@ Drop-in modules with the reference's signatures:
     rumik_fast_b200.int4_gemv  quantize, gemv_int4, G
 Beyond them: Int4GemvSet (a list of GEMVs in one launch), fused (the decode-layer glue in the GEMV launches),
 attention (decode attention), sample (the sampling tail), scales8 (8-bit double-quantised scales).
+For several continuations of one prompt: kv_cache (caches quantised as they are written), prefix_attention (a batch's
+attention over a shared prefix and rows of its own), beams (beam selection, reordering of the beams' caches).
 All compute runs in librumik_b200.so (hand-written CUDA for sm_100a behind the C ABI in
 include/rumik_b200.h), loaded with ctypes from this directory.
 """

@@ -68,6 +68,35 @@ class Sampler(ctypes.Structure):
                 ("out", _vp), ("out_len", _i64), ("ws", _vp)]
 
 
+class KvCache(ctypes.Structure):
+    """struct rb_kv_cache (include/rumik_b200.h)."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_par", _vp), ("v_par", _vp), ("fmt", _int), ("dtype", _int), ("n_seqs", _i64),
+                ("n_kv_heads", _int), ("head_dim", _int), ("cache_len", _i64)]
+
+
+KV_PLAIN, KV_INT8, KV_INT4 = 0, 1, 2
+
+
+class PrefixAttnArgs(ctypes.Structure):
+    """struct rb_prefix_attn_args (include/rumik_b200.h)."""
+    _fields_ = [("q", _vp), ("ldq", _i64), ("out", _vp), ("ldo", _i64), ("n_seqs", _i64), ("n_q_heads", _int),
+                ("prefix", _c.POINTER(KvCache)), ("prefix_len", _vp), ("own", _c.POINTER(KvCache)), ("own_len", _vp),
+                ("scale", _c.c_float), ("ws", _vp), ("ws_bytes", _i64)]
+
+
+class BeamSelectArgs(ctypes.Structure):
+    """struct rb_beam_select_args (include/rumik_b200.h)."""
+    _fields_ = [("logits", _vp), ("logits_dtype", _int), ("ld", _i64), ("requests", _i64), ("n_beams", _int),
+                ("n_vocab", _i64), ("end_idx", _i64), ("scores", _vp), ("done", _vp), ("ids", _vp), ("step", _vp),
+                ("min_new", _i64), ("out_scores", _vp), ("out_parents", _vp), ("out_tokens", _vp), ("out_done", _vp),
+                ("ws", _vp), ("ws_bytes", _i64)]
+
+
+class BeamTensor(ctypes.Structure):
+    """struct rb_beam_tensor (include/rumik_b200.h)."""
+    _fields_ = [("p", _vp), ("n_heads", _int), ("row_bytes", _int)]
+
+
 EPI_STORE, EPI_ROPE_KV, EPI_SWIGLU = 0, 1, 2
 # device error word bits (rb_get_device_error): a wait that ran out, or an out-of-range device-side argument
 DEVERR_TC_WAIT, DEVERR_TP_WAIT, DEVERR_ARG, DEVERR_ATT_WAIT, DEVERR_STEP_WAIT = 1 << 7, 1 << 8, 1 << 9, 1 << 10, 1 << 11
@@ -97,6 +126,13 @@ SIGNATURES = {
     "rb_set_wait_limit": (_int, [_c.c_uint64, _vp]),
     "rb_decode_layers_workspace": (_i64, [_vp]),
     "rb_decode_layers": (_int, [_vp, _int, _int, _vp]),
+    "rb_kv_write": (_int, [_c.POINTER(KvCache), _vp, _vp, _c.POINTER(_i64), _c.POINTER(_i64), _i64, _vp, _int, _vp]),
+    "rb_kv_read": (_int, [_c.POINTER(KvCache), _vp, _vp, _i64, _i64, _int, _vp]),
+    "rb_prefix_attn_workspace": (_i64, [_c.POINTER(PrefixAttnArgs)]),
+    "rb_prefix_attn": (_int, [_c.POINTER(PrefixAttnArgs), _int, _vp]),
+    "rb_beam_select_workspace": (_i64, [_i64, _int, _i64]),
+    "rb_beam_select": (_int, [_c.POINTER(BeamSelectArgs), _int, _vp]),
+    "rb_beam_reorder": (_int, [_c.POINTER(BeamTensor), _int, _i64, _int, _i64, _vp, _vp, _int, _vp]),
     "rb_ipc_alloc": (_int, [_c.c_uint64, _c.POINTER(_vp), _vp]),
     "rb_ipc_free": (_int, [_vp]),
     "rb_ipc_open": (_int, [_vp, _c.c_uint64, _c.POINTER(_vp), _c.POINTER(_vp)]),

@@ -1,0 +1,430 @@
+// beams.cu - one step of a beam search on the device: the selection of the best beams over every beam's vocabulary
+// (rb_beam_select) and the reordering of the beams' cache rows by their parents, in place (rb_beam_reorder).
+//
+// Selection, per request of nb beams:
+//   cand[b, v] = (x[b, v] - lse_b) + score_b,  lse_b = log sum_v exp(x[b, v])        (a live beam)
+//   cand[b, end] = score_b and nothing else                                           (a finished beam)
+// and the nb best of the nb V candidates. Within a beam the order of the candidates is the order of the logits, so no
+// normaliser is needed to find a beam's nb best rows: one pass over the logits yields each 4096-row chunk's maximum,
+// sum of exponentials and nb best (value, row) keys. The last chunk of a beam to finish merges them, and the last beam
+// of a request picks the winners: one launch, every logit read once.
+// A key is the logit's order-preserving 32 bits above the row's complement, so the largest key is the largest logit,
+// the lower row among equals, and no two keys are equal: the result does not depend on the order of arrival.
+#include "common.cuh"
+#include "kernels.h"
+
+namespace rb {
+
+namespace bm {
+
+using Key = unsigned long long;
+constexpr int kThreads = 128;
+constexpr int kPer = 32;                       // logits of a thread, held in registers
+constexpr int kChunk = kThreads * kPer;        // 4096 rows a CTA
+constexpr int kMaxBeams = 32;
+constexpr int kMaxChunks = 256;                // V <= 2^20
+constexpr int kCap = kMaxBeams * (kMaxChunks * kMaxBeams / kThreads);  // keys that may pass a threshold (2048)
+static_assert(kCap >= kMaxBeams * kPer, "a chunk's own candidates fit as well");
+
+struct SelectParams {
+  const void* logits;
+  int64_t ld;
+  const float* scores;
+  const uint8_t* done;
+  const int64_t* ids;
+  const int64_t* step;
+  float* out_scores;
+  int64_t* out_parents;
+  int64_t* out_tokens;
+  uint8_t* out_done;
+  unsigned int* tickets;   // [R nb] chunks done, then [R] beams done: zero between launches
+  float2* part;            // [R nb][chunks] (maximum, sum of exponentials)
+  Key* keys;               // [R nb][chunks][nb]
+  float* row_cand;         // [R nb][nb] a beam's best candidates, best first
+  int* row_idx;            // [R nb][nb] their rows (-1: none)
+  int64_t end_idx, min_new;
+  int nb, V, chunks, dtype;
+};
+
+__device__ __forceinline__ Key make_key(float x, uint32_t row) {
+  const uint32_t b = __float_as_uint(x);
+  const uint32_t k = (b & 0x80000000u) ? ~b : b | 0x80000000u;
+  return (static_cast<Key>(k) << 32) | (0xffffffffu - row);
+}
+__device__ __forceinline__ float key_value(Key key) {
+  const uint32_t k = static_cast<uint32_t>(key >> 32);
+  return __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
+}
+__device__ __forceinline__ uint32_t key_row(Key key) { return 0xffffffffu - static_cast<uint32_t>(key); }
+
+struct Shared {
+  Key top[kThreads];
+  Key cand[kCap];
+  Key threshold;
+  float2 red[kThreads / 32];
+  int n;
+  int last;
+};
+
+// The k largest of the CTA's keys, best first, through `out(rank, key)`. get(i) is this thread's i-th key (0: none),
+// i < count. The k-th largest of the threads' own maxima bounds the k-th largest key from below, and at most k
+// threads hold a key at or above it, so at most k count keys are ranked against one another.
+template <int kCount, typename Get, typename Out>
+__device__ __forceinline__ void cta_top(Shared& sh, int k, int count, Get get, Out out) {
+  const int tid = threadIdx.x;
+  Key best = 0;
+#pragma unroll
+  for (int i = 0; i < kCount; ++i)
+    if (i < count) {
+      const Key v = get(i);
+      best = v > best ? v : best;
+    }
+  sh.top[tid] = best;
+  if (tid == 0) {
+    sh.threshold = 1;
+    sh.n = 0;
+  }
+  __syncthreads();
+  int rank = 0;
+#pragma unroll 8
+  for (int j = 0; j < kThreads; ++j) rank += sh.top[j] > best;
+  if (rank == k - 1 && best != 0) sh.threshold = best;  // keys differ: one thread has this rank
+  __syncthreads();
+  const Key lim = sh.threshold;
+  if (best >= lim) {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i)
+      if (i < count) {
+        const Key v = get(i);
+        if (v >= lim) sh.cand[atomicAdd(&sh.n, 1)] = v;
+      }
+  }
+  __syncthreads();
+  const int n = sh.n;
+  for (int c = tid; c < n; c += kThreads) {
+    const Key v = sh.cand[c];
+    int r = 0;
+    for (int j = 0; j < n; ++j) r += sh.cand[j] > v;
+    if (r < k) out(r, v);
+  }
+  for (int r = n + tid; r < k; r += kThreads) out(r, Key(0));
+  __syncthreads();
+}
+
+// Whether this CTA is the last of `of` to arrive at the ticket, which is then zero again. What the others wrote
+// before they arrived is visible to the last one's loads through L2.
+__device__ __forceinline__ bool last_to_arrive(Shared& sh, unsigned int* ticket, int of) {
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const bool last = atomicAdd(ticket, 1u) + 1u == static_cast<unsigned>(of);
+    if (last) *ticket = 0u;
+    sh.last = last;
+    __threadfence();
+  }
+  __syncthreads();
+  return sh.last != 0;
+}
+
+__device__ __forceinline__ float2 merge_sums(float2 a, float2 b) {
+  const float m = fmaxf(a.x, b.x);
+  if (m == -INFINITY) return make_float2(m, 0.f);
+  return make_float2(m, a.y * expf(a.x - m) + b.y * expf(b.x - m));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) beam_select_kernel(const __grid_constant__ SelectParams p) {
+  __shared__ Shared sh;
+  griddep_wait();
+  griddep_launch_dependents();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int row = blockIdx.y, chunk = blockIdx.x, nb = p.nb;
+  const int req = row / nb;
+  const bool early = p.step && *p.step < p.min_new;
+  const float score = p.scores[row];
+  const bool done = p.done[row] != 0;
+  const bool dead = !(score > -INFINITY && score < INFINITY);  // no candidate of this beam counts
+  if (!done && !dead) {
+    const T* x = reinterpret_cast<const T*>(p.logits) + row * p.ld;
+    const int first = chunk * kChunk + tid;
+    float v[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int at = first + i * kThreads;
+      v[i] = at < p.V ? static_cast<float>(x[at]) : -INFINITY;
+    }
+    float top = -INFINITY;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (early && first + i * kThreads == p.end_idx) v[i] = -INFINITY;
+      odd |= !(v[i] < INFINITY);  // NaN or +inf: the row has no distribution
+      top = fmaxf(top, v[i]);
+    }
+    float sum = 0.f;
+    if (top > -INFINITY) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) sum += expf(v[i] - top);
+    }
+    float2 ms = odd ? make_float2(INFINITY, 0.f) : make_float2(top, sum);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float2 b = make_float2(__shfl_xor_sync(0xffffffffu, ms.x, o), __shfl_xor_sync(0xffffffffu, ms.y, o));
+      ms = ms.x == INFINITY || b.x == INFINITY ? make_float2(INFINITY, 0.f) : merge_sums(ms, b);
+    }
+    if (lane == 0) sh.red[warp] = ms;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 1; w < kThreads / 32; ++w)
+        ms = ms.x == INFINITY || sh.red[w].x == INFINITY ? make_float2(INFINITY, 0.f) : merge_sums(ms, sh.red[w]);
+      p.part[static_cast<int64_t>(row) * p.chunks + chunk] = ms;
+    }
+    Key* dst = p.keys + (static_cast<int64_t>(row) * p.chunks + chunk) * nb;
+    cta_top<kPer>(sh, nb, kPer,
+                  [&](int i) { const int at = first + i * kThreads; return at < p.V ? make_key(v[i], at) : Key(0); },
+                  [&](int r, Key key) { dst[r] = key; });
+  }
+  if (!last_to_arrive(sh, p.tickets + row, p.chunks)) return;
+
+  // ---- the beam's nb best candidates ----
+  float* cand = p.row_cand + static_cast<int64_t>(row) * nb;
+  int* idx = p.row_idx + static_cast<int64_t>(row) * nb;
+  float2 ms = make_float2(-INFINITY, 0.f);
+  bool odd = false;
+  if (!done && !dead) {
+    for (int c = 0; c < p.chunks; ++c) {  // in chunk order, by every thread: the same sum everywhere
+      const float2 b = __ldcg(p.part + static_cast<int64_t>(row) * p.chunks + c);
+      odd |= b.x == INFINITY;
+      if (!odd) ms = merge_sums(ms, b);
+    }
+    if (odd && tid == 0) atomicOr(&g_device_error, static_cast<unsigned>(ERR_ARG));
+  }
+  if (!done && !dead && !odd && ms.x > -INFINITY) {
+    const float lse = ms.x + logf(ms.y);
+    const Key* src = p.keys + static_cast<int64_t>(row) * p.chunks * nb;
+    const int n = p.chunks * nb, count = (n + kThreads - 1) / kThreads;
+    cta_top<kMaxChunks * kMaxBeams / kThreads>(
+        sh, nb, count,
+        [&](int i) { const int at = i * kThreads + tid; return at < n ? __ldcg(src + at) : Key(0); },
+        [&](int r, Key key) {
+          cand[r] = key ? (key_value(key) - lse) + score : -INFINITY;
+          idx[r] = key ? static_cast<int>(key_row(key)) : -1;
+        });
+  } else {
+    // a finished beam: its end row with the score it has; then, and for a beam without any candidate, rows of -inf
+    const int end = static_cast<int>(p.end_idx);
+    for (int r = tid; r < nb; r += kThreads) {
+      const int rest = done ? (r - 1 >= end ? r : r - 1) : r;
+      const int at = done && r == 0 ? end : rest;
+      cand[r] = done && r == 0 && !dead ? score : -INFINITY;
+      idx[r] = at < p.V ? at : -1;
+    }
+  }
+  if (!last_to_arrive(sh, p.tickets + gridDim.y + req, nb)) return;
+
+  // ---- the request's nb best: keys of (candidate, place in the order beam, rank within the beam) ----
+  const int n = nb * nb, count = (n + kThreads - 1) / kThreads;
+  const int64_t base = static_cast<int64_t>(req) * nb * nb;
+  cta_top<kMaxBeams * kMaxBeams / kThreads>(
+      sh, nb, count,
+      [&](int i) {
+        const int at = i * kThreads + tid;
+        return at < n && __ldcg(p.row_idx + base + at) >= 0 ? make_key(__ldcg(p.row_cand + base + at), at) : Key(0);
+      },
+      [&](int r, Key key) {
+        if (key == 0) return;  // not reached: every beam gives min(nb, V) rows
+        const int at = static_cast<int>(key_row(key)), parent = at / nb;
+        const int tok = __ldcg(p.row_idx + base + at);
+        const int64_t o = static_cast<int64_t>(req) * nb + r;
+        p.out_scores[o] = key_value(key);
+        p.out_parents[o] = parent;
+        p.out_tokens[o] = p.ids ? p.ids[tok] : tok;
+        p.out_done[o] = p.done[req * nb + parent] != 0 || tok == p.end_idx;
+      });
+}
+
+// ---- reordering ----
+
+struct Tensor {
+  uint8_t* p;
+  int64_t line;   // bytes of one (beam, head): cache_len rows
+  int heads, row_bytes, unit, line0;  // unit: bytes of one access; line0: the tensor's first line in the launch
+};
+constexpr int kMaxTensors = 100;
+struct ReorderParams {
+  Tensor t[kMaxTensors];
+  const int64_t* parents;
+  const int64_t* slots;
+  int count, nb;
+  int64_t cache_len;
+};
+static_assert(sizeof(ReorderParams) < 4096, "kernel parameters");
+
+template <typename U, int kBeams>
+__device__ __forceinline__ void reorder_line(uint8_t* base, int64_t beam_bytes, const int* parent, const int64_t* bytes,
+                                             uint32_t needed, int nb, int64_t most, int piece, int pieces) {
+  for (int64_t at = (static_cast<int64_t>(piece) * kThreads + threadIdx.x) * sizeof(U); at < most;
+       at += static_cast<int64_t>(pieces) * kThreads * sizeof(U)) {
+    // one column of every beam that another one takes over, all read before any is written: the columns of a line
+    // are independent, so the beams change places in place
+    U v[kBeams];
+#pragma unroll
+    for (int b = 0; b < kBeams; ++b)
+      if ((needed >> b) & 1u) v[b] = *reinterpret_cast<const U*>(base + b * beam_bytes + at);
+#pragma unroll
+    for (int b = 0; b < kBeams; ++b) {
+      if (!((needed >> b) & 1u) || at >= bytes[b]) continue;
+      for (int c = 0; c < nb; ++c)
+        if (parent[c] == b && c != b) *reinterpret_cast<U*>(base + c * beam_bytes + at) = v[b];
+    }
+  }
+}
+
+template <int kBeams>
+__global__ void __launch_bounds__(kThreads) beam_reorder_kernel(const __grid_constant__ ReorderParams p) {
+  __shared__ int parent[kMaxBeams];
+  __shared__ int64_t bytes[kMaxBeams];
+  griddep_wait();
+  griddep_launch_dependents();
+  const int nb = p.nb, req = blockIdx.z;
+  int t = 0;
+  while (t + 1 < p.count && static_cast<int>(blockIdx.x) >= p.t[t + 1].line0) ++t;
+  const Tensor& T = p.t[t];
+  const int head = blockIdx.x - T.line0;
+  bool ok = true;
+  if (threadIdx.x < nb) {
+    const int64_t q = p.parents[req * nb + threadIdx.x], n = p.slots[req * nb + threadIdx.x];
+    ok = q >= 0 && q < nb && n >= 0 && n <= p.cache_len;
+    parent[threadIdx.x] = ok ? static_cast<int>(q) : 0;
+    bytes[threadIdx.x] = ok ? n * T.row_bytes : 0;
+  }
+  if (__syncthreads_or(!ok)) {  // an index that is none: the request's rows stay as they are
+    if (threadIdx.x == 0) atomicOr(&g_device_error, static_cast<unsigned>(ERR_ARG));
+    return;
+  }
+  uint32_t needed = 0;
+  int64_t most = 0;
+  for (int c = 0; c < nb; ++c) {
+    const int b = parent[c];
+    if (b == c) continue;
+    needed |= 1u << b;
+    most = bytes[b] > most ? bytes[b] : most;
+  }
+  if (!needed) return;
+  const int64_t beam_bytes = T.line * T.heads;
+  uint8_t* base = T.p + static_cast<int64_t>(req) * nb * beam_bytes + head * T.line;
+  switch (T.unit) {
+    case 16: reorder_line<uint4, kBeams>(base, beam_bytes, parent, bytes, needed, nb, most, blockIdx.y, gridDim.y); break;
+    case 8: reorder_line<uint2, kBeams>(base, beam_bytes, parent, bytes, needed, nb, most, blockIdx.y, gridDim.y); break;
+    case 4: reorder_line<uint32_t, kBeams>(base, beam_bytes, parent, bytes, needed, nb, most, blockIdx.y, gridDim.y); break;
+    default: reorder_line<uint16_t, kBeams>(base, beam_bytes, parent, bytes, needed, nb, most, blockIdx.y, gridDim.y); break;
+  }
+}
+
+}  // namespace bm
+
+namespace {
+int64_t align16(int64_t n) { return (n + 15) / 16 * 16; }
+int64_t select_chunks(int64_t V) { return (V + bm::kChunk - 1) / bm::kChunk; }
+}  // namespace
+
+int64_t beam_select_tickets(int64_t requests, int nb) { return align16((requests * nb + requests) * 4); }
+
+int64_t beam_select_workspace(int64_t requests, int nb, int64_t V) {
+  const int64_t rows = requests * nb, ch = select_chunks(V);
+  return beam_select_tickets(requests, nb) + align16(rows * ch * 8) + align16(rows * ch * nb * 8) + 2 * align16(rows * nb * 4);
+}
+
+int launch_beam_select(const rb_beam_select_args* a, int flags, cudaStream_t stream) {
+  using namespace bm;
+  const int64_t rows = a->requests * a->n_beams;
+  SelectParams p = {};
+  p.logits = a->logits;
+  p.ld = a->ld;
+  p.scores = a->scores;
+  p.done = a->done;
+  p.ids = a->ids;
+  p.step = a->step;
+  p.out_scores = a->out_scores;
+  p.out_parents = a->out_parents;
+  p.out_tokens = a->out_tokens;
+  p.out_done = a->out_done;
+  p.end_idx = a->end_idx;
+  p.min_new = a->min_new;
+  p.nb = a->n_beams;
+  p.V = static_cast<int>(a->n_vocab);
+  p.chunks = static_cast<int>(select_chunks(a->n_vocab));
+  p.dtype = a->logits_dtype;
+  uint8_t* w = static_cast<uint8_t*>(a->ws);
+  p.tickets = reinterpret_cast<unsigned int*>(w);
+  w += beam_select_tickets(a->requests, a->n_beams);
+  p.part = reinterpret_cast<float2*>(w);
+  w += align16(rows * p.chunks * 8);
+  p.keys = reinterpret_cast<Key*>(w);
+  w += align16(rows * p.chunks * a->n_beams * 8);
+  p.row_cand = reinterpret_cast<float*>(w);
+  w += align16(rows * a->n_beams * 4);
+  p.row_idx = reinterpret_cast<int*>(w);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.chunks, static_cast<unsigned>(rows));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = (flags & RB_FLAG_PDL) ? 1 : 0;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  void (*kern)(SelectParams) = a->logits_dtype == RB_F32    ? beam_select_kernel<float>
+                               : a->logits_dtype == RB_BF16 ? beam_select_kernel<__nv_bfloat16>
+                                                            : beam_select_kernel<__half>;
+  return cudaLaunchKernelEx(&cfg, kern, p) == cudaSuccess ? RB_OK : RB_ERR_LAUNCH;
+}
+
+int launch_beam_reorder(const rb_beam_tensor* t, int count, int64_t requests, int nb, int64_t cache_len,
+                        const int64_t* parents, const int64_t* slots, int num_sms, int flags, cudaStream_t stream) {
+  using namespace bm;
+  for (int done = 0; done < count;) {
+    ReorderParams p = {};
+    p.parents = parents;
+    p.slots = slots;
+    p.nb = nb;
+    p.cache_len = cache_len;
+    int lines = 0;
+    int64_t widest = 0;
+    for (; done < count && p.count < kMaxTensors; ++done) {
+      const rb_beam_tensor& s = t[done];
+      Tensor& d = p.t[p.count++];
+      d.p = static_cast<uint8_t*>(s.p);
+      d.heads = s.n_heads;
+      d.row_bytes = s.row_bytes;
+      d.line = cache_len * s.row_bytes;
+      d.line0 = lines;
+      // the widest access that every (beam, head) of the tensor is aligned to
+      const uint64_t mix = static_cast<uint64_t>(reinterpret_cast<uintptr_t>(s.p)) | static_cast<uint64_t>(d.line) |
+                           static_cast<uint64_t>(s.row_bytes);
+      d.unit = mix % 16 == 0 ? 16 : mix % 8 == 0 ? 8 : mix % 4 == 0 ? 4 : 2;
+      lines += s.n_heads;
+      widest = std::max<int64_t>(widest, d.line / d.unit);
+    }
+    // about eight CTAs an SM, and no more pieces of a line than it has columns for
+    int64_t pieces = (8 * static_cast<int64_t>(num_sms) + lines * requests - 1) / (lines * requests);
+    pieces = std::max<int64_t>(1, std::min<int64_t>(pieces, (widest + kThreads - 1) / kThreads));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(lines, static_cast<unsigned>(pieces), static_cast<unsigned>(requests));
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = (flags & RB_FLAG_PDL) ? 1 : 0;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    void (*kern)(ReorderParams) = nb <= 4    ? beam_reorder_kernel<4>
+                                  : nb <= 8  ? beam_reorder_kernel<8>
+                                  : nb <= 16 ? beam_reorder_kernel<16>
+                                             : beam_reorder_kernel<32>;
+    if (cudaLaunchKernelEx(&cfg, kern, p) != cudaSuccess) return RB_ERR_LAUNCH;
+  }
+  return RB_OK;
+}
+
+}  // namespace rb

@@ -559,6 +559,152 @@ int rb_decode_layers(const rb_decode_step* st, int dtype, int flags, void* strea
   return s;
 }
 
+static int check_kv_cache(const rb_kv_cache* c) {
+  if (!c) return RB_ERR_NULL;
+  if (!act_dtype_ok(c->dtype)) return RB_ERR_DTYPE;
+  if (c->fmt != RB_KV_PLAIN && c->fmt != RB_KV_INT8 && c->fmt != RB_KV_INT4) return RB_ERR_SHAPE;
+  if (c->head_dim != 64 && c->head_dim != 128) return RB_ERR_SHAPE;
+  if (c->n_seqs < 0 || c->n_seqs > (1 << 20) || c->n_kv_heads < 1 || c->n_kv_heads > 256 || c->cache_len < 0 ||
+      c->cache_len > (int64_t(1) << 31) - 1024)
+    return RB_ERR_SHAPE;
+  if (c->n_seqs == 0 || c->cache_len == 0) return RB_OK;  // no row: pointers may be NULL
+  if (!c->k || !c->v) return RB_ERR_NULL;
+  if (!aligned16(c->k) || !aligned16(c->v)) return RB_ERR_ALIGN;
+  if (c->fmt != RB_KV_PLAIN) {
+    if (!c->k_par || !c->v_par) return RB_ERR_NULL;
+    const uintptr_t mask = c->fmt == RB_KV_INT8 ? 1u : 3u;
+    if (((reinterpret_cast<uintptr_t>(c->k_par) | reinterpret_cast<uintptr_t>(c->v_par)) & mask) != 0) return RB_ERR_ALIGN;
+  }
+  return RB_OK;
+}
+
+int rb_kv_write(const rb_kv_cache* cache, const void* k, const void* v, const int64_t* k_stride,
+                const int64_t* v_stride, int64_t n_tokens, const int64_t* pos, int flags, void* stream) {
+  int st = check_kv_cache(cache);
+  if (st != RB_OK) return st;
+  if (n_tokens < 0 || n_tokens > (int64_t(1) << 31)) return RB_ERR_SHAPE;
+  if (n_tokens == 0 || cache->n_seqs == 0) return RB_OK;
+  if (!k || !v || !k_stride || !v_stride || !pos) return RB_ERR_NULL;
+  if (cache->cache_len == 0) return RB_ERR_SHAPE;
+  if (!aligned16(k) || !aligned16(v)) return RB_ERR_ALIGN;
+  for (int i = 0; i < 3; ++i)
+    if (k_stride[i] % 8 != 0 || v_stride[i] % 8 != 0) return RB_ERR_ALIGN;
+  int sms = 0;
+  if ((st = device_sms(&sms)) != RB_OK) return st;
+  st = rb::launch_kv_write(cache, k, v, k_stride, v_stride, n_tokens, pos, sms, flags, static_cast<cudaStream_t>(stream));
+  if (st == RB_OK && cudaGetLastError() != cudaSuccess) st = RB_ERR_LAUNCH;
+  return st;
+}
+
+int rb_kv_read(const rb_kv_cache* cache, void* k_out, void* v_out, int64_t start, int64_t count, int flags,
+               void* stream) {
+  int st = check_kv_cache(cache);
+  if (st != RB_OK) return st;
+  if (start < 0 || count < 0 || start > cache->cache_len || count > cache->cache_len - start) return RB_ERR_SHAPE;
+  if (count == 0 || cache->n_seqs == 0) return RB_OK;
+  if (!k_out || !v_out) return RB_ERR_NULL;
+  if (!aligned16(k_out) || !aligned16(v_out)) return RB_ERR_ALIGN;
+  int sms = 0;
+  if ((st = device_sms(&sms)) != RB_OK) return st;
+  st = rb::launch_kv_read(cache, k_out, v_out, start, count, sms, flags, static_cast<cudaStream_t>(stream));
+  if (st == RB_OK && cudaGetLastError() != cudaSuccess) st = RB_ERR_LAUNCH;
+  return st;
+}
+
+// What rb_prefix_attn and its workspace query both need: the caches and the head counts.
+static int check_prefix_attn(const rb_prefix_attn_args* a) {
+  if (!a || (!a->prefix && !a->own)) return RB_ERR_NULL;
+  const rb_kv_cache* both[2] = {a->prefix, a->own};
+  for (const rb_kv_cache* c : both) {
+    if (!c) continue;
+    const int st = check_kv_cache(c);
+    if (st != RB_OK) return st;
+  }
+  if (a->n_seqs < 0 || a->n_seqs > 1024) return RB_ERR_SHAPE;
+  if (a->prefix && a->prefix->n_seqs != 1) return RB_ERR_SHAPE;
+  if (a->own && a->own->n_seqs != a->n_seqs) return RB_ERR_SHAPE;
+  if (a->prefix && a->own &&
+      (a->prefix->fmt != a->own->fmt || a->prefix->dtype != a->own->dtype || a->prefix->n_kv_heads != a->own->n_kv_heads ||
+       a->prefix->head_dim != a->own->head_dim))
+    return RB_ERR_SHAPE;
+  const rb_kv_cache* c = a->prefix ? a->prefix : a->own;
+  if (a->n_q_heads < 1 || a->n_q_heads % c->n_kv_heads != 0 || a->n_q_heads / c->n_kv_heads > 16) return RB_ERR_SHAPE;
+  return RB_OK;
+}
+
+int64_t rb_prefix_attn_workspace(const rb_prefix_attn_args* a) {
+  int st = check_prefix_attn(a), sms = 0;
+  if (st == RB_OK) st = device_sms(&sms);
+  return st == RB_OK ? rb::prefix_attn_workspace(a, sms) : -st;
+}
+
+int rb_prefix_attn(const rb_prefix_attn_args* a, int flags, void* stream) {
+  int st = check_prefix_attn(a);
+  if (st != RB_OK) return st;
+  if (a->n_seqs == 0) return RB_OK;
+  if (!a->q || !a->out || !a->ws || (a->prefix && !a->prefix_len) || (a->own && !a->own_len)) return RB_ERR_NULL;
+  const int64_t row = static_cast<int64_t>(a->n_q_heads) * (a->prefix ? a->prefix : a->own)->head_dim;
+  if (a->n_seqs > 1 && (a->ldq < row || a->ldo < row)) return RB_ERR_SHAPE;
+  if (!(a->scale >= -3.4e38f && a->scale <= 3.4e38f)) return RB_ERR_SHAPE;
+  if (!aligned16(a->q) || !aligned16(a->out) || !aligned16(a->ws)) return RB_ERR_ALIGN;
+  if (a->n_seqs > 1 && (a->ldq % 8 != 0 || a->ldo % 8 != 0)) return RB_ERR_ALIGN;
+  int sms = 0;
+  if ((st = device_sms(&sms)) != RB_OK) return st;
+  if (a->ws_bytes < rb::prefix_attn_workspace(a, sms)) return RB_ERR_SHAPE;
+  st = rb::launch_prefix_attn(a, sms, flags, static_cast<cudaStream_t>(stream));
+  if (st == RB_OK && cudaGetLastError() != cudaSuccess) st = RB_ERR_LAUNCH;
+  return st;
+}
+
+static bool beam_shape_ok(int64_t requests, int n_beams) {
+  return requests >= 0 && n_beams >= 1 && n_beams <= 32 && requests * n_beams <= 65535;
+}
+
+int64_t rb_beam_select_workspace(int64_t requests, int n_beams, int64_t n_vocab) {
+  if (requests < 0 || requests > 65535 || !beam_shape_ok(requests, n_beams) || n_vocab < 1 || n_vocab > (1 << 20))
+    return -RB_ERR_SHAPE;
+  return rb::beam_select_workspace(requests, n_beams, n_vocab);
+}
+
+int rb_beam_select(const rb_beam_select_args* a, int flags, void* stream) {
+  if (!a) return RB_ERR_NULL;
+  if (a->requests < 0 || a->requests > 65535 || !beam_shape_ok(a->requests, a->n_beams)) return RB_ERR_SHAPE;
+  if (a->n_vocab < 1 || a->n_vocab > (1 << 20) || a->end_idx < 0 || a->end_idx >= a->n_vocab) return RB_ERR_SHAPE;
+  if (a->logits_dtype != RB_F16 && a->logits_dtype != RB_BF16 && a->logits_dtype != RB_F32) return RB_ERR_DTYPE;
+  if (a->requests * a->n_beams > 1 && a->ld < a->n_vocab) return RB_ERR_SHAPE;
+  if (a->requests == 0) return RB_OK;
+  if (!a->logits || !a->scores || !a->done || !a->out_scores || !a->out_parents || !a->out_tokens || !a->out_done || !a->ws)
+    return RB_ERR_NULL;
+  if ((reinterpret_cast<uintptr_t>(a->logits) & (a->logits_dtype == RB_F32 ? 3u : 1u)) != 0 || !aligned16(a->ws))
+    return RB_ERR_ALIGN;
+  if (a->ws_bytes < rb::beam_select_workspace(a->requests, a->n_beams, a->n_vocab)) return RB_ERR_SHAPE;
+  int sms = 0, st = device_sms(&sms);
+  if (st != RB_OK) return st;
+  st = rb::launch_beam_select(a, flags, static_cast<cudaStream_t>(stream));
+  if (st == RB_OK && cudaGetLastError() != cudaSuccess) st = RB_ERR_LAUNCH;
+  return st;
+}
+
+int rb_beam_reorder(const rb_beam_tensor* tensors, int count, int64_t requests, int n_beams, int64_t cache_len,
+                    const int64_t* parents, const int64_t* slots, int flags, void* stream) {
+  if (count < 0 || requests < 0 || requests > 65535 || !beam_shape_ok(requests, n_beams)) return RB_ERR_SHAPE;
+  if (cache_len < 0 || cache_len > (int64_t(1) << 31)) return RB_ERR_SHAPE;
+  if (count == 0 || requests == 0 || cache_len == 0) return RB_OK;
+  if (!tensors || !parents || !slots) return RB_ERR_NULL;
+  for (int i = 0; i < count; ++i) {
+    const rb_beam_tensor& t = tensors[i];
+    if (!t.p) return RB_ERR_NULL;
+    if (t.n_heads < 1 || t.n_heads > 65536 || t.row_bytes < 2 || t.row_bytes % 2 != 0 || t.row_bytes > 65536) return RB_ERR_SHAPE;
+    if ((reinterpret_cast<uintptr_t>(t.p) & 1u) != 0) return RB_ERR_ALIGN;
+  }
+  int sms = 0, st = device_sms(&sms);
+  if (st != RB_OK) return st;
+  st = rb::launch_beam_reorder(tensors, count, requests, n_beams, cache_len, parents, slots, sms, flags,
+                               static_cast<cudaStream_t>(stream));
+  if (st == RB_OK && cudaGetLastError() != cudaSuccess) st = RB_ERR_LAUNCH;
+  return st;
+}
+
 int rb_set_wait_limit(uint64_t ns, void* stream) {
   if (ns == 0) ns = rb::kMaxWaitNs;
   if (ns < 1000 || ns > 60000000000ull) return RB_ERR_SHAPE;

@@ -65,6 +65,18 @@ int64_t decode_layers_workspace(const rb_decode_step* d, int num_sms);
 int launch_decode_layers(const rb_decode_step* d, int dtype, int flags, int num_sms, cudaStream_t stream);
 int launch_attn_decode(const void* q, const void* kc, const void* vc, const int64_t* pos, void* out, int nq, int nkv,
                        int64_t S, float scale, void* ws, int dtype, int flags, int num_sms, cudaStream_t stream);
+// Caches of a batch of sequences (kv_cache.cu), its attention (prefix_attn.cu) and a beam search's step (beams.cu);
+// arguments as in the header, already checked.
+int launch_kv_write(const rb_kv_cache* c, const void* k, const void* v, const int64_t* ks, const int64_t* vs,
+                    int64_t n_tokens, const int64_t* pos, int num_sms, int flags, cudaStream_t stream);
+int launch_kv_read(const rb_kv_cache* c, void* k_out, void* v_out, int64_t start, int64_t count, int num_sms, int flags,
+                   cudaStream_t stream);
+int64_t prefix_attn_workspace(const rb_prefix_attn_args* a, int num_sms);
+int launch_prefix_attn(const rb_prefix_attn_args* a, int num_sms, int flags, cudaStream_t stream);
+int64_t beam_select_workspace(int64_t requests, int nb, int64_t V);
+int launch_beam_select(const rb_beam_select_args* a, int flags, cudaStream_t stream);
+int launch_beam_reorder(const rb_beam_tensor* t, int count, int64_t requests, int nb, int64_t cache_len,
+                        const int64_t* parents, const int64_t* slots, int num_sms, int flags, cudaStream_t stream);
 // The add + LayerNorm of rb_add_layernorm (one CTA), bit-identical to the prologue of rb_gemv_int4_fused.
 int launch_add_ln(const rb_add_ln* ln, int dtype, int flags, cudaStream_t stream);
 // epi (per entry, may be null) and ln (may be null): the fused decode-layer glue of rb_gemv_int4_fused; a call

@@ -11,8 +11,8 @@
 // O = sum 2^(t - R) v in fp32 (t: the score times log2 e). R is only raised when a score exceeds it by more than 2^8,
 // so the accumulators are rarely rescaled; any R gives the same O / l.
 //
-// Work is cut along the slots so that every SM streams a share of the caches: CTAs take (key-value head, 16 kMt kWm
-// rows, split of the prefix) or (sequence, key-value head, split of its own rows) items and leave an fp32 partial
+// Work is cut along the slots so that every SM streams a share of the caches: CTAs take (key-value head, 16 wm rows,
+// split of the prefix) or (sequence, key-value head, split of its own rows) items and leave an fp32 partial
 // (R, l, O) each, which prefix_attn_merge joins in split order (deterministic).
 #include "common.cuh"
 #include "tc.cuh"
@@ -24,7 +24,7 @@ namespace pfx {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kMaxSeqs = 1024;
+constexpr int kCtasPerSm = 3;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.f;     // a row's reference is raised when a score exceeds it by this (log2)
 constexpr float kLowestE = -90.f; // exponent range of the value scales folded into the reference
@@ -46,7 +46,7 @@ struct Params {
   Side pre, own;
   int n_seqs, n_q, n_kv, rep, bf16;
   float scale;
-  int tiles_m;       // row tiles of the prefix's M = n_seqs rep rows
+  int wm, tiles_m;   // warps along the rows of a tile, row tiles of the prefix's M = n_seqs rep rows
   int max_np;        // most splits of the prefix
   int max_ns;        // most splits of a sequence's own rows
   float* o;          // partials: prefix items [n_kv][tiles_m][max_np][rows][hd], then own [n_seqs][n_kv][max_ns][rep][hd]
@@ -71,15 +71,32 @@ __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0
 
 __device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
 }
 __device__ __forceinline__ void ldsm4t(uint32_t a, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+}
+// Shared-memory loads without a memory clobber: volatile keeps them between the barriers that guard the data, and
+// nothing that is held in registers is loaded again after them.
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
 }
 __device__ __forceinline__ uint2 lds64(uint32_t a) {
   uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ float2 lds64f(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint4 lds128v(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
   return v;
 }
 
@@ -133,18 +150,14 @@ struct Fmt {
     return byte ^ (x << 4);
   }
 
-  // Column of q . k held by lane column c at k16 step ks, register pair p (k = 2c, 2c+1 | 2c+8, 2c+9), element e;
-  // inverse: where column d goes.
-  __device__ static void q_place(int d, int& ks, int& c, int& p, int& e) {
-    if constexpr (kPlain) {
-      ks = d >> 4, p = (d >> 3) & 1, c = (d >> 1) & 3, e = d & 1;
-    } else if constexpr (kFmt == RB_KV_INT8) {
-      ks = ((d >> 6) << 2) | ((d >> 2) & 3), c = (d >> 4) & 3, p = (d >> 1) & 1, e = d & 1;
-    } else {
-      const int per = kHd / 4;  // columns of a lane: kHd / 32 words of eight
-      c = d / per, e = (d >> 2) & 1, p = d & 1;
-      ks = (((d % per) >> 3) << 1) | ((d >> 1) & 1);
-    }
+  // The query columns that lane column c holds at k16 step ks as register pair q (k = 2c, 2c + 1 | 2c + 8, 2c + 9).
+  __device__ static uint32_t q_pair(const uint16_t* row, int ks, int c, int q) {
+    if constexpr (kPlain) return __ldcg(reinterpret_cast<const unsigned int*>(row + ks * 16 + q * 8 + 2 * c));
+    if constexpr (kFmt == RB_KV_INT8)
+      return __ldcg(reinterpret_cast<const unsigned int*>(row + (ks >> 2) * 64 + c * 16 + (ks & 3) * 4 + q * 2));
+    // a word of eight 4-bit codes: nibbles i and i + 4 are the pair
+    const uint16_t* at = row + c * (kHd / 4) + (ks >> 1) * 8 + (ks & 1) * 2 + q;
+    return static_cast<uint32_t>(__ldcg(at)) | (static_cast<uint32_t>(__ldcg(at + 4)) << 16);
   }
   // Output column of accumulator tile u, column n
   __device__ static int o_col(int u, int n) { return kPlain ? u * 8 + n : n * kNv + u; }
@@ -166,7 +179,7 @@ struct Fmt {
         } else {
 #pragma unroll
           for (int i = 0; i < kRow / 64; ++i) {
-            const uint4 v = lds128_a(tile + k_at(r, c + 4 * i));
+            const uint4 v = lds128v(tile + k_at(r, c + 4 * i));
             raw.w[t][4 * i] = v.x, raw.w[t][4 * i + 1] = v.y, raw.w[t][4 * i + 2] = v.z, raw.w[t][4 * i + 3] = v.w;
           }
         }
@@ -216,13 +229,13 @@ struct Fmt {
       for (int i = 0; i < 4; ++i) {
         const int r = row0 + 2 * c + (i & 1) + ((i >> 1) << 3);
         if constexpr (kB == 16) {
-          const uint4 v = lds128_a(tile + v_at(r, g));
+          const uint4 v = lds128v(tile + v_at(r, g));
           w[i][0] = v.x, w[i][1] = v.y, w[i][2] = v.z, w[i][3] = v.w;
         } else if constexpr (kB == 8) {
           const uint2 v = lds64(tile + v_at(r, g >> 1) + (g & 1) * 8);
           w[i][0] = v.x, w[i][1] = v.y;
         } else {
-          w[i][0] = lds32_a(tile + v_at(r, g >> 2) + (g & 3) * 4);
+          w[i][0] = lds32(tile + v_at(r, g >> 2) + (g & 3) * 4);
         }
       }
       if constexpr (kFmt == RB_KV_INT8) {
@@ -275,47 +288,52 @@ struct Item {
   float2* rl;
 };
 
-// kMt 16-row tiles a warp, kWm warps along the rows, kWk = 4 / kWm along the slots of a stage.
-template <typename F, int kMt, int kWm>
+// A CTA's four warps: each takes 16 query rows; wm of them stand along the rows (1, 2 or 4), the other 4 / wm along the
+// slots of a stage. Three CTAs an SM: one's loads and barriers hide behind the others' products.
+template <typename F>
 struct Tile {
-  static constexpr int kWk = kWarps / kWm;
-  static constexpr int kRows = 16 * kMt * kWm;
-  static constexpr int kPerWarp = F::kTile / kWk;             // slots of a warp in a stage
-  static constexpr int kBlock = kPerWarp < 32 ? kPerWarp : 32;  // slots of one softmax step
+  static constexpr int kBlock = F::kPlain ? 16 : 32;          // slots of one softmax step
   static constexpr int kNt = kBlock / 8;
-  static constexpr int kQ = kRows * F::kHd * 2;
   static constexpr int kMergeRow = (F::kNv * 33) * 16;        // a warp's 16-row accumulator tile, padded
-  static constexpr int kMerge = kWarps * kMt * kMergeRow;
-  static constexpr int kStages = (kQ + 3 * F::kStage > 108 * 1024) ? 2 : 3;
+  static constexpr int kStages = F::kStage <= 20 * 1024 ? 3 : 2;
   static constexpr int kRing = kStages * F::kStage;
-  static constexpr int kOffQ = kRing > kMerge ? kRing : kMerge;  // the merge reuses the ring
-  static constexpr int kOffRow = kOffQ + kQ;                  // rowf, qsum [kRows], then (R, l) [kWk][kRows]
-  static constexpr int kSmem = kOffRow + kRows * 8 + kWk * kRows * 8;
+  static constexpr int kMerge = kWarps * kMergeRow;
+  static constexpr int kOffRl = kRing > kMerge ? kRing : kMerge;  // the merge reuses the ring; (R, l) [4][16]
+  static constexpr int kSmem = kOffRl + kWarps * 16 * 8;
 };
 
-template <typename F, int kMt, int kWm>
-__device__ __noinline__ void run_item(const Params& p, const Item& it, uint8_t* smem) {
-  using T = Tile<F, kMt, kWm>;
+template <typename F>
+__device__ __forceinline__ void run_item(const Params& p, const Item it, const int wm_n, uint8_t* smem) {
+  using T = Tile<F>;
   constexpr int kHd = F::kHd;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
-  const int wm = warp % kWm, wk = warp / kWm;
+  const int wm = warp & (wm_n - 1), wk = warp / wm_n, per_warp = F::kTile * wm_n / kWarps;
   const uint32_t s0 = smem_u32(smem);
-  float* rowf = reinterpret_cast<float*>(smem + T::kOffRow);
-  float* qsum = rowf + T::kRows;
-  float2* rl = reinterpret_cast<float2*>(qsum + T::kRows);
+  float2* rl = reinterpret_cast<float2*>(smem + T::kOffRl);
 
-  auto stage = [&](int i) { return s0 + (i % T::kStages) * F::kStage; };
-  auto load_rows = [&](int t) {  // stage t's keys and values
-    const uint32_t dst = stage(t - it.t0);
-    const int64_t first = static_cast<int64_t>(t) * F::kTile;
+  uint32_t ld_slot = 0, rd_slot = 0;  // byte offsets of the stage to fill and of the stage to read in the ring
+  auto load_rows = [&](int t) {       // stage t's keys and values
+    const uint32_t dst = s0 + ld_slot;
+    const int64_t left = it.n - static_cast<int64_t>(t) * F::kTile;
+    const uint8_t* k = it.k + static_cast<int64_t>(t) * F::kSide + tid * 16;
+    const uint8_t* v = it.v + static_cast<int64_t>(t) * F::kSide + tid * 16;
+    // a stage's rows are contiguous; kThreads chunks on, the swizzle of a chunk is the same
+    static_assert(kThreads / F::kChunks % 8 == 0, "the swizzle repeats every eight rows");
+    const uint32_t kd = dst + F::k_at(tid / F::kChunks, tid % F::kChunks), vd = dst + F::kSide + F::v_at(tid / F::kChunks, tid % F::kChunks);
+    if (left >= F::kTile) {
 #pragma unroll
-    for (int i = 0; i < F::kTile * F::kChunks / kThreads; ++i) {
-      const int x = i * kThreads + tid, r = x / F::kChunks, ch = x % F::kChunks;
-      const bool on = first + r < it.n;
-      const int64_t off = on ? (first + r) * F::kRow + ch * 16 : 0;
-      cp_async16(dst + F::k_at(r, ch), it.k + off, on);
-      cp_async16(dst + F::kSide + F::v_at(r, ch), it.v + off, on);
+      for (int i = 0; i < F::kSide / 16 / kThreads; ++i) {
+        cp_async16(kd + i * kThreads * 16, k + i * kThreads * 16, true);
+        cp_async16(vd + i * kThreads * 16, v + i * kThreads * 16, true);
+      }
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < F::kSide / 16 / kThreads; ++i) {
+        const bool on = (i * kThreads + tid) / F::kChunks < left;
+        cp_async16(kd + i * kThreads * 16, on ? k + i * kThreads * 16 : it.k, on);
+        cp_async16(vd + i * kThreads * 16, on ? v + i * kThreads * 16 : it.v, on);
+      }
     }
   };
   // A stage's row parameters: loaded into registers ahead, stored as fp32 behind its rows (2-byte scales of an odd
@@ -329,14 +347,14 @@ __device__ __noinline__ void run_item(const Params& p, const Item& it, uint8_t* 
       for (int s = 0; s < 2; ++s) {
         const void* src = s ? it.v_par : it.k_par;
         par[s] = 0u;
-        if (on) par[s] = F::kFmt == RB_KV_INT8 ? static_cast<uint32_t>(__ldg(reinterpret_cast<const unsigned short*>(src) + it.par0 + r))
-                                               : __ldg(reinterpret_cast<const uint32_t*>(src) + it.par0 + r);
+        if (on) par[s] = F::kFmt == RB_KV_INT8 ? static_cast<uint32_t>(__ldcg(reinterpret_cast<const unsigned short*>(src) + it.par0 + r))
+                                               : __ldcg(reinterpret_cast<const unsigned int*>(src) + it.par0 + r);
       }
     }
   };
-  auto store_par = [&](int t) {
+  auto store_par = [&]() {  // behind the rows of the stage last loaded
     if constexpr (!F::kPlain) {
-      float* dst = reinterpret_cast<float*>(smem + ((t - it.t0) % T::kStages) * F::kStage + 2 * F::kSide);
+      float* dst = reinterpret_cast<float*>(smem + ld_slot + 2 * F::kSide);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const float sc = __uint_as_float(par[s] << 16);
@@ -347,321 +365,271 @@ __device__ __noinline__ void run_item(const Params& p, const Item& it, uint8_t* 
       }
     }
   };
+  auto next = [](uint32_t slot) { return slot + F::kStage == T::kRing ? 0u : slot + F::kStage; };
   static_assert(F::kPlain || F::kTile == kThreads, "one thread a slot's parameters");
 
   __syncthreads();  // the previous item's merge has been read
-#pragma unroll
+#pragma unroll 1
   for (int i = 0; i < T::kStages - 1; ++i) {
     if (it.t0 + i < it.t1) {
       load_rows(it.t0 + i);
       load_par(it.t0 + i);
-      store_par(it.t0 + i);
+      store_par();
+      ld_slot = next(ld_slot);
     }
     cp_commit();
   }
 
-  // ---- the queries, in the order of the A fragments ----
-  for (int r = warp; r < T::kRows; r += kWarps) {
+  // ---- the warp's queries (rows g, g + 8 of its 16) as A fragments, straight from global memory ----
+  uint32_t qa[F::kKs][4];
+  float fr[2], qs[2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int r = wm * 16 + x * 8 + g;
     const bool on = r < it.rows;
     const int row = it.row0 + r;
     const int b = it.seq >= 0 ? it.seq : (on ? row / p.rep : 0), j = it.seq >= 0 ? r : row % p.rep;
-    constexpr int kE = kHd / 32;
-    const int64_t at = b * p.ldq + static_cast<int64_t>(it.kv * p.rep + (on ? j : 0)) * kHd + lane * kE;
-    uint32_t raw[kE / 2];
+    const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) + b * p.ldq + static_cast<int64_t>(it.kv * p.rep + (on ? j : 0)) * kHd;
 #pragma unroll
-    for (int e = 0; e < kE / 2; ++e) raw[e] = on ? __ldcg(reinterpret_cast<const unsigned int*>(reinterpret_cast<const uint16_t*>(p.q) + at) + e) : 0u;
-    if (p.scale < 0.f) {
+    for (int ks = 0; ks < F::kKs; ++ks)
 #pragma unroll
-      for (int e = 0; e < kE / 2; ++e) raw[e] ^= 0x80008000u;
-    }
+      for (int q = 0; q < 2; ++q) qa[ks][2 * q + x] = on ? F::q_pair(src, ks, c, q) : 0u;
+  }
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
     float f = fmaxf(fabsf(p.scale) * kLog2e, 1e-30f);
+    float sum = 0.f;
     if constexpr (!F::kPlain) {
       // fp16 queries for the codes' product: scaled by a power of two so that the row's largest is in [1, 2) - exact
       // but for elements 2^-24 below it
-      float v[kE], top = 0.f, sum = 0.f;
+      uint32_t top = 0u;
 #pragma unroll
-      for (int e = 0; e < kE; ++e) {
-        const uint32_t u = raw[e / 2] >> (16 * (e & 1)) & 0xffffu;
-        v[e] = p.bf16 ? __uint_as_float(u << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(u)));
-        top = fmaxf(top, fabsf(v[e]));
-      }
-      const uint32_t ex = __reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23;
+      for (int ks = 0; ks < F::kKs; ++ks)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) top = __vmaxu2(top, qa[ks][2 * q + x] & 0x7fff7fffu);
+      top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const uint32_t t16 = max(top & 0xffffu, top >> 16);
+      const uint32_t ex = __float_as_uint(p.bf16 ? __uint_as_float(t16 << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(t16)))) >> 23;
       const uint32_t exc = ex < 30u ? 30u : (ex > 220u ? 220u : ex);
       const float down = __uint_as_float((254u - exc) << 23);
       f *= __uint_as_float(exc << 23);
 #pragma unroll
-      for (int e = 0; e < kE; ++e) {
-        const __half h = __float2half_rn(v[e] * down);
-        sum += __half2float(h);
-        const uint32_t u = __half_as_ushort(h);
-        raw[e / 2] = (e & 1) ? raw[e / 2] | (u << 16) : u;
+      for (int ks = 0; ks < F::kKs; ++ks)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const uint32_t u = qa[ks][2 * q + x];
+          float2 v;
+          if (p.bf16) v = make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+          else v = __half22float2(*reinterpret_cast<const __half2*>(&u));
+          const uint32_t h = pack2<false>(v.x * down, v.y * down);
+          if constexpr (F::kFmt == RB_KV_INT4) {
+            const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&h));
+            sum += w.x + w.y;
+          }
+          qa[ks][2 * q + x] = h ^ flip;
+        }
+      if constexpr (F::kFmt == RB_KV_INT4) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        if (flip) sum = -sum;
       }
+    } else {
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (lane == 0) qsum[r] = sum;
+      for (int ks = 0; ks < F::kKs; ++ks) qa[ks][x] ^= flip, qa[ks][2 + x] ^= flip;
     }
-    if (lane == 0) rowf[r] = f;
-    uint16_t* qf = reinterpret_cast<uint16_t*>(smem + T::kOffQ);
-    const int mt = r >> 4, half = (r >> 3) & 1;
-#pragma unroll
-    for (int e = 0; e < kE; ++e) {
-      int ks, qc, qp, qe;
-      F::q_place(lane * kE + e, ks, qc, qp, qe);
-      qf[(((mt * F::kKs + ks) * 32 + (r & 7) * 4 + qc) * 4 + qp * 2 + half) * 2 + qe] =
-          static_cast<uint16_t>(raw[e / 2] >> (16 * (e & 1)));
-    }
+    fr[x] = f;
+    qs[x] = sum;
   }
 
-  float o[kMt][F::kNv][4], l[kMt][2], w[kMt][2], ref[kMt][2], fr[kMt][2], qs[kMt][2];
+  float o[F::kNv][4], l[2], w[2], ref[2];
   float ve = F::kPlain ? 0.f : kLowestE;  // exponent of the value scales seen, part of every row's reference
 #pragma unroll
-  for (int m = 0; m < kMt; ++m) {
+  for (int u = 0; u < F::kNv; ++u)
 #pragma unroll
-    for (int u = 0; u < F::kNv; ++u)
+    for (int e = 0; e < 4; ++e) o[u][e] = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[m][u][e] = 0.f;
-#pragma unroll
-    for (int x = 0; x < 2; ++x) l[m][x] = w[m][x] = 0.f, ref[m][x] = -INFINITY;
-  }
-  uint32_t qreg[kMt == 1 ? F::kKs : 1][4];
+  for (int x = 0; x < 2; ++x) l[x] = w[x] = 0.f, ref[x] = -INFINITY;
 
+#pragma unroll 1
   for (int t = it.t0; t < it.t1; ++t) {
     cp_wait<T::kStages - 2>();
     __syncthreads();  // stage t is there for everybody, stage t - 1 is free
-    const int ahead = t + T::kStages - 1;
-    if (ahead < it.t1) {
-      load_rows(ahead);
-      load_par(ahead);
+    const bool more = t + T::kStages - 1 < it.t1;
+    if (more) {
+      load_rows(t + T::kStages - 1);
+      load_par(t + T::kStages - 1);
     }
     cp_commit();
-    if (t == it.t0) {
-#pragma unroll
-      for (int m = 0; m < kMt; ++m)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int r = (wm * kMt + m) * 16 + x * 8 + g;
-          fr[m][x] = rowf[r];
-          qs[m][x] = F::kFmt == RB_KV_INT4 ? qsum[r] : 0.f;
-        }
-      if constexpr (kMt == 1) {
-#pragma unroll
-        for (int ks = 0; ks < F::kKs; ++ks) {
-          const uint4 v = lds128_a(s0 + T::kOffQ + ((wm * F::kKs + ks) * 32 + lane) * 16);
-          qreg[ks][0] = v.x, qreg[ks][1] = v.y, qreg[ks][2] = v.z, qreg[ks][3] = v.w;
-        }
-      }
-    }
-    const uint32_t kt = stage(t - it.t0), vt = kt + F::kSide, pt = vt + F::kSide;
-    const int64_t left = it.n - static_cast<int64_t>(t) * F::kTile;
+    const uint32_t kt = s0 + rd_slot, vt = kt + F::kSide, pt = vt + F::kSide;
+    rd_slot = next(rd_slot);
+    const int64_t left64 = it.n - static_cast<int64_t>(t) * F::kTile;
+    const int left = left64 < F::kTile ? static_cast<int>(left64) : F::kTile;
+    const int b1 = min((wk + 1) * per_warp, left);
 #pragma unroll 1
-    for (int b0 = wk * T::kPerWarp; b0 < (wk + 1) * T::kPerWarp; b0 += T::kBlock) {
-      if (b0 >= left) break;
-      float s[kMt][T::kNt][4];
+    for (int b0 = wk * per_warp; b0 < b1; b0 += T::kBlock) {
+      float s[T::kNt][4];
 #pragma unroll
-      for (int m = 0; m < kMt; ++m)
+      for (int n = 0; n < T::kNt; ++n)
 #pragma unroll
-        for (int n = 0; n < T::kNt; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[m][n][e] = 0.f;
+        for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
       // ---- scores ----
       typename F::KRaw raw[T::kNt / 2];
 #pragma unroll
       for (int n = 0; n < T::kNt / 2; ++n) F::k_raw(kt, b0 + 16 * n, lane, raw[n]);
 #pragma unroll
-      for (int ks = 0; ks < F::kKs; ++ks) {
-        uint32_t a[kMt][4];
-        if constexpr (kMt == 1) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) a[0][e] = qreg[ks][e];
-        } else {
-#pragma unroll
-          for (int m = 0; m < kMt; ++m) {
-            const uint4 v = lds128_a(s0 + T::kOffQ + (((wm * kMt + m) * F::kKs + ks) * 32 + lane) * 16);
-            a[m][0] = v.x, a[m][1] = v.y, a[m][2] = v.z, a[m][3] = v.w;
-          }
-        }
+      for (int ks = 0; ks < F::kKs; ++ks)
 #pragma unroll
         for (int n = 0; n < T::kNt / 2; ++n) {
           uint32_t b[2][2];
           F::k_frag(kt, b0 + 16 * n, lane, ks, raw[n], b);
+          mma16816<F::kBf16>(s[2 * n], qa[ks], b[0][0], b[0][1]);
+          mma16816<F::kBf16>(s[2 * n + 1], qa[ks], b[1][0], b[1][1]);
+        }
+      // ---- scales, mask, largest ----
+      float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-          for (int m = 0; m < kMt; ++m) {
-            mma16816<F::kBf16>(s[m][2 * n], a[m], b[0][0], b[0][1]);
-            mma16816<F::kBf16>(s[m][2 * n + 1], a[m], b[1][0], b[1][1]);
+      for (int n = 0; n < T::kNt; ++n) {
+        if constexpr (!F::kPlain) {
+          const int col = b0 + 8 * n + 2 * c;
+          const float2 ks = lds64f(pt + col * 4);
+          float2 km = make_float2(0.f, 0.f);
+          if constexpr (F::kFmt == RB_KV_INT4) km = lds64f(pt + (2 * F::kTile + col) * 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float sc = (e & 1) ? ks.y : ks.x;
+            if constexpr (F::kFmt == RB_KV_INT4)
+              s[n][e] = fmaf(s[n][e], sc, ((e & 1) ? km.y : km.x) * qs[e >> 1]);
+            else
+              s[n][e] *= sc;
           }
         }
       }
-      // ---- scales, mask, largest ----
-      bool raise = false;
-      float top[kMt][2];
+      if (b0 + T::kBlock > left) {
 #pragma unroll
-      for (int m = 0; m < kMt; ++m) top[m][0] = top[m][1] = -INFINITY;
+        for (int n = 0; n < T::kNt; ++n)
 #pragma unroll
-      for (int n = 0; n < T::kNt; ++n) {
-        const int col = b0 + 8 * n + 2 * c;
-        if constexpr (!F::kPlain) {
-          const float2 ks = lds64f_a(pt + col * 4);
-          float2 km = make_float2(0.f, 0.f);
-          if constexpr (F::kFmt == RB_KV_INT4) km = lds64f_a(pt + (2 * F::kTile + col) * 4);
-#pragma unroll
-          for (int m = 0; m < kMt; ++m)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float sc = (e & 1) ? ks.y : ks.x;
-              if constexpr (F::kFmt == RB_KV_INT4)
-                s[m][n][e] = fmaf(s[m][n][e], sc, ((e & 1) ? km.y : km.x) * qs[m][e >> 1]);
-              else
-                s[m][n][e] *= sc;
-            }
-        }
-        if (b0 + T::kBlock > left) {
-#pragma unroll
-          for (int m = 0; m < kMt; ++m)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (col + (e & 1) >= left) s[m][n][e] = -INFINITY;
-        }
-#pragma unroll
-        for (int m = 0; m < kMt; ++m)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) top[m][e >> 1] = fmaxf(top[m][e >> 1], s[m][n][e]);
+          for (int e = 0; e < 4; ++e)
+            if (b0 + 8 * n + 2 * c + (e & 1) >= left) s[n][e] = -INFINITY;
       }
 #pragma unroll
-      for (int m = 0; m < kMt; ++m)
+      for (int n = 0; n < T::kNt; ++n)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) raise |= top[m][x] * fr[m][x] > ref[m][x] + kSlack;
+        for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
+      bool raise = top[0] * fr[0] > ref[0] + kSlack || top[1] * fr[1] > ref[1] + kSlack;
       float ven = ve;
       if constexpr (!F::kPlain) {
         // the block's largest value scale (NaN left out: it shows by itself): its exponent goes into the reference,
         // so that the 16-bit p s stay within fp16's range whatever the size of the values
-        const float vs = lane < T::kBlock ? __uint_as_float(lds32_a(pt + (F::kTile + b0 + lane) * 4)) : 0.f;
+        const float vs = __uint_as_float(lds32(pt + (F::kTile + b0 + lane) * 4));
         const uint32_t hi = __reduce_max_sync(0xffffffffu, vs == vs ? __float_as_uint(vs) : 0u);
         ven = fmaxf(ve, fminf(fmaxf(static_cast<float>(static_cast<int>(hi >> 23) - 127), kLowestE), kHighestE));
         raise |= ven > ve;
       }
       if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
-        for (int m = 0; m < kMt; ++m)
+        for (int x = 0; x < 2; ++x) {
+          float v = top[x];
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+          const float nr = fmaxf(ref[x], v * fr[x]);
+          const float f = ref[x] == -INFINITY ? 0.f : ex2((ref[x] - nr) + (ve - ven));
+          ref[x] = nr;
+          l[x] *= f;
+          w[x] *= f;
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            float v = top[m][x];
-            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
-            const float nr = fmaxf(ref[m][x], v * fr[m][x]);
-            const float f = ref[m][x] == -INFINITY ? 0.f : ex2((ref[m][x] - nr) + (ve - ven));
-            ref[m][x] = nr;
-            l[m][x] *= f;
-            w[m][x] *= f;
-#pragma unroll
-            for (int u = 0; u < F::kNv; ++u) o[m][u][2 * x] *= f, o[m][u][2 * x + 1] *= f;
-          }
+          for (int u = 0; u < F::kNv; ++u) o[u][2 * x] *= f, o[u][2 * x + 1] *= f;
+        }
         ve = ven;
       }
       // ---- probabilities ----
-      float base[kMt][2];
+      float base[2];
 #pragma unroll
-      for (int m = 0; m < kMt; ++m)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) base[m][x] = ref[m][x] == -INFINITY ? 0.f : -(ref[m][x] + ve);
+      for (int x = 0; x < 2; ++x) base[x] = ref[x] == -INFINITY ? 0.f : -(ref[x] + ve);
 #pragma unroll
       for (int n = 0; n < T::kNt; ++n) {
         const int col = b0 + 8 * n + 2 * c;
         float2 vs = make_float2(1.f, 1.f), vm = make_float2(0.f, 0.f);
-        if constexpr (!F::kPlain) vs = lds64f_a(pt + (F::kTile + col) * 4);
-        if constexpr (F::kFmt == RB_KV_INT4) vm = lds64f_a(pt + (3 * F::kTile + col) * 4);
+        if constexpr (!F::kPlain) vs = lds64f(pt + (F::kTile + col) * 4);
+        if constexpr (F::kFmt == RB_KV_INT4) vm = lds64f(pt + (3 * F::kTile + col) * 4);
 #pragma unroll
-        for (int m = 0; m < kMt; ++m)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float pr = ex2(fmaf(s[m][n][e], fr[m][e >> 1], base[m][e >> 1]));
-            l[m][e >> 1] += pr;
-            if constexpr (F::kFmt == RB_KV_INT4) w[m][e >> 1] = fmaf(pr, (e & 1) ? vm.y : vm.x, w[m][e >> 1]);
-            if constexpr (!F::kPlain) pr *= (e & 1) ? vs.y : vs.x;
-            s[m][n][e] = pr;
-          }
+        for (int e = 0; e < 4; ++e) {
+          float pr = ex2(fmaf(s[n][e], fr[e >> 1], base[e >> 1]));
+          l[e >> 1] += pr;
+          if constexpr (F::kFmt == RB_KV_INT4) w[e >> 1] = fmaf(pr, (e & 1) ? vm.y : vm.x, w[e >> 1]);
+          if constexpr (!F::kPlain) pr *= (e & 1) ? vs.y : vs.x;
+          s[n][e] = pr;
+        }
       }
       // ---- O += p v ----
 #pragma unroll
       for (int n = 0; n < T::kNt / 2; ++n) {
-        uint32_t a[kMt][4];
+        uint32_t a[4];
 #pragma unroll
-        for (int m = 0; m < kMt; ++m) {
-          a[m][0] = pack2<F::kBf16>(s[m][2 * n][0], s[m][2 * n][1]);
-          a[m][1] = pack2<F::kBf16>(s[m][2 * n][2], s[m][2 * n][3]);
-          a[m][2] = pack2<F::kBf16>(s[m][2 * n + 1][0], s[m][2 * n + 1][1]);
-          a[m][3] = pack2<F::kBf16>(s[m][2 * n + 1][2], s[m][2 * n + 1][3]);
-        }
+        for (int e = 0; e < 4; ++e) a[e] = pack2<F::kBf16>(s[2 * n + (e >> 1)][2 * (e & 1)], s[2 * n + (e >> 1)][2 * (e & 1) + 1]);
         // 4-bit rows: a value's part s (c - 8) may be far larger than the value, so the rounding of p s to fp16 is
         // made up for by a second term
-        uint32_t a2[F::kFmt == RB_KV_INT4 ? kMt : 1][4];
+        uint32_t a2[4] = {0u, 0u, 0u, 0u};
         if constexpr (F::kFmt == RB_KV_INT4) {
 #pragma unroll
-          for (int m = 0; m < kMt; ++m)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&a[m][e]));
-              a2[m][e] = pack2<false>(s[m][2 * n + (e >> 1)][2 * (e & 1)] - hi.x, s[m][2 * n + (e >> 1)][2 * (e & 1) + 1] - hi.y);
-            }
+          for (int e = 0; e < 4; ++e) {
+            const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&a[e]));
+            a2[e] = pack2<false>(s[2 * n + (e >> 1)][2 * (e & 1)] - hi.x, s[2 * n + (e >> 1)][2 * (e & 1) + 1] - hi.y);
+          }
         }
         F::v_frags(vt, b0 + 16 * n, lane, [&](int u, uint32_t f0, uint32_t f1) {
-#pragma unroll
-          for (int m = 0; m < kMt; ++m) mma16816<F::kBf16>(o[m][u], a[m], f0, f1);
-          if constexpr (F::kFmt == RB_KV_INT4) {
-#pragma unroll
-            for (int m = 0; m < kMt; ++m) mma16816<false>(o[m][u], a2[m], f0, f1);
-          }
+          mma16816<F::kBf16>(o[u], a, f0, f1);
+          if constexpr (F::kFmt == RB_KV_INT4) mma16816<false>(o[u], a2, f0, f1);
         });
       }
     }
-    if (ahead < it.t1) store_par(ahead);
+    if (more) {
+      store_par();
+      ld_slot = next(ld_slot);
+    }
   }
   cp_wait<0>();
 
   // ---- join the warps along the slots, in their order, and leave the item's partial ----
 #pragma unroll
-  for (int m = 0; m < kMt; ++m)
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      l[m][x] += __shfl_xor_sync(0xffffffffu, l[m][x], 1);
-      l[m][x] += __shfl_xor_sync(0xffffffffu, l[m][x], 2);
-      if constexpr (F::kFmt == RB_KV_INT4) {
-        w[m][x] += __shfl_xor_sync(0xffffffffu, w[m][x], 1);
-        w[m][x] += __shfl_xor_sync(0xffffffffu, w[m][x], 2);
-      }
-      if (c == 0) rl[wk * T::kRows + (wm * kMt + m) * 16 + x * 8 + g] =
-          make_float2(ref[m][x] == -INFINITY && l[m][x] == 0.f ? -INFINITY : (ref[m][x] == -INFINITY ? 0.f : ref[m][x] + ve), l[m][x]);
+  for (int x = 0; x < 2; ++x) {
+    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+    if constexpr (F::kFmt == RB_KV_INT4) {
+      w[x] += __shfl_xor_sync(0xffffffffu, w[x], 1);
+      w[x] += __shfl_xor_sync(0xffffffffu, w[x], 2);
     }
+    if (c == 0)
+      rl[warp * 16 + x * 8 + g] =
+          make_float2(ref[x] == -INFINITY && l[x] == 0.f ? -INFINITY : (ref[x] == -INFINITY ? 0.f : ref[x] + ve), l[x]);
+  }
   __syncthreads();
-#pragma unroll
-  for (int m = 0; m < kMt; ++m) {
+  {
     float f[2];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      const int r = (wm * kMt + m) * 16 + x * 8 + g;
       float hi = -INFINITY;
-#pragma unroll
-      for (int k = 0; k < T::kWk; ++k) hi = fmaxf(hi, rl[k * T::kRows + r].x);
-      const float mine = rl[wk * T::kRows + r].x;
+      for (int k = wm; k < kWarps; k += wm_n) hi = fmaxf(hi, rl[k * 16 + x * 8 + g].x);
+      const float mine = rl[warp * 16 + x * 8 + g].x;
       f[x] = mine == -INFINITY ? 0.f : ex2(mine - hi);
     }
-    uint8_t* dst = smem + (warp * kMt + m) * T::kMergeRow;
+    uint8_t* dst = smem + warp * T::kMergeRow;
 #pragma unroll
     for (int u = 0; u < F::kNv; ++u)
       *reinterpret_cast<float4*>(dst + (u * 33 + lane) * 16) =
-          make_float4((o[m][u][0] + w[m][0]) * f[0], (o[m][u][1] + w[m][0]) * f[0], (o[m][u][2] + w[m][1]) * f[1],
-                      (o[m][u][3] + w[m][1]) * f[1]);
+          make_float4((o[u][0] + w[0]) * f[0], (o[u][1] + w[0]) * f[0], (o[u][2] + w[1]) * f[1], (o[u][3] + w[1]) * f[1]);
   }
   __syncthreads();
+#pragma unroll 2
   for (int x = tid; x < it.rows * (kHd / 2); x += kThreads) {
     const int r = x / (kHd / 2), d2 = x % (kHd / 2);
-    const int mt = r >> 4, m = mt % kMt, rw = mt / kMt, half = (r >> 3) & 1;
     // columns o_col(u, n), o_col(u, n + 1) of the fragments: a pair in the plain order, strided in the codes' order
     float2 acc = make_float2(0.f, 0.f);
     const int u = F::kPlain ? d2 >> 2 : d2 % F::kNv, n = F::kPlain ? (d2 & 3) * 2 : (d2 / F::kNv) * 2;
-#pragma unroll
-    for (int k = 0; k < T::kWk; ++k) {
-      const float2 v = *reinterpret_cast<const float2*>(smem + ((k * kWm + rw) * kMt + m) * T::kMergeRow +
-                                                        (u * 33 + (r & 7) * 4 + n / 2) * 16 + half * 8);
+    const uint8_t* src = smem + (r >> 4) * T::kMergeRow + (u * 33 + (r & 7) * 4 + n / 2) * 16 + ((r >> 3) & 1) * 8;
+    for (int k = 0; k < kWarps; k += wm_n) {
+      const float2 v = *reinterpret_cast<const float2*>(src + k * T::kMergeRow);
       acc.x += v.x, acc.y += v.y;
     }
     float* dst = it.o + static_cast<int64_t>(r) * kHd;
@@ -674,11 +642,9 @@ __device__ __noinline__ void run_item(const Params& p, const Item& it, uint8_t* 
   }
   for (int r = tid; r < it.rows; r += kThreads) {
     float hi = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int k = 0; k < T::kWk; ++k) hi = fmaxf(hi, rl[k * T::kRows + r].x);
-#pragma unroll
-    for (int k = 0; k < T::kWk; ++k) {
-      const float2 v = rl[k * T::kRows + r];
+    for (int k = r >> 4; k < kWarps; k += wm_n) hi = fmaxf(hi, rl[k * 16 + (r & 15)].x);
+    for (int k = r >> 4; k < kWarps; k += wm_n) {
+      const float2 v = rl[k * 16 + (r & 15)];
       sum += v.x == -INFINITY ? 0.f : v.y * ex2(v.x - hi);
     }
     it.rl[r] = make_float2(hi, sum);
@@ -731,8 +697,8 @@ __device__ __forceinline__ Plan make_plan(const Params& p, int grid) {
   return pl;
 }
 
-template <typename F, int kMt, int kWm>
-__global__ void __launch_bounds__(kThreads, 2) prefix_attn_kernel(const __grid_constant__ Params p) {
+template <typename F>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) prefix_attn_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
   griddep_wait();
   griddep_launch_dependents();
@@ -748,54 +714,55 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attn_kernel(const __grid_c
   int i = cta, step = grid;
   if (apart && cta >= pl.prefix_items) step = grid - pl.prefix_items;
   const int end = apart && cta < pl.prefix_items ? pl.prefix_items : pl.prefix_items + pl.own_items;
+#pragma unroll 1
   for (; i < end; i += step) {
     Item it;
-    if (i < pl.prefix_items) {
+    int wm = 1;
+    const bool pre = i < pl.prefix_items;
+    const Side& S = pre ? p.pre : p.own;
+    int64_t head;
+    if (pre) {
       const int lane_i = i / pl.np, sp = i % pl.np;
       it.kv = lane_i / p.tiles_m;
       const int rt = lane_i % p.tiles_m;
-      constexpr int kRows = Tile<F, kMt, kWm>::kRows;
-      const int64_t row = static_cast<int64_t>(it.kv) * p.pre.cache_len;
-      it.k = p.pre.k + row * F::kRow;
-      it.v = p.pre.v + row * F::kRow;
-      it.k_par = p.pre.k_par;
-      it.v_par = p.pre.v_par;
-      it.par0 = row;
-      it.n = *p.pre.len;
+      head = it.kv;
+      it.n = *S.len;
       it.t0 = sp * pl.pt;
-      it.t1 = min(static_cast<int>((it.n + F::kTile - 1) / F::kTile), it.t0 + pl.pt);
+      it.t1 = it.t0 + pl.pt;
       it.seq = -1;
-      it.row0 = rt * kRows;
-      it.rows = min(kRows, p.n_seqs * p.rep - it.row0);
-      const int64_t slot = static_cast<int64_t>(lane_i) * p.max_np + sp;
-      it.o = p.o + slot * kRows * F::kHd;
-      it.rl = p.rl + slot * kRows;
-      run_item<F, kMt, kWm>(p, it, smem);
+      wm = p.wm;
+      const int tile = 16 * wm;
+      it.row0 = rt * tile;
+      it.rows = min(tile, p.n_seqs * p.rep - it.row0);
+      const int64_t slot = (static_cast<int64_t>(lane_i) * p.max_np + sp) * tile;
+      it.o = p.o + slot * F::kHd;
+      it.rl = p.rl + slot;
     } else {
       const int x = i - pl.prefix_items, sp = x % pl.ns;
       it.kv = (x / pl.ns) % p.n_kv;
       it.seq = x / pl.ns / p.n_kv;
-      it.n = p.own.len[it.seq];
-      if (it.n < 0 || it.n > p.own.cache_len) {
+      it.n = S.len[it.seq];
+      if (it.n < 0 || it.n > S.cache_len) {
         if (threadIdx.x == 0) atomicOr(&g_device_error, static_cast<unsigned>(ERR_ARG));
         continue;
       }
       it.t0 = sp * pl.ot;
-      it.t1 = min(static_cast<int>((it.n + F::kTile - 1) / F::kTile), it.t0 + pl.ot);
-      if (it.t0 >= it.t1) continue;
-      const int64_t head = static_cast<int64_t>(it.seq) * p.n_kv + it.kv, row = head * p.own.cache_len;
-      it.k = p.own.k + row * F::kRow;
-      it.v = p.own.v + row * F::kRow;
-      it.k_par = p.own.k_par;
-      it.v_par = p.own.v_par;
-      it.par0 = row;
+      it.t1 = it.t0 + pl.ot;
+      head = static_cast<int64_t>(it.seq) * p.n_kv + it.kv;
       it.row0 = 0;
       it.rows = p.rep;
-      const int64_t slot = head * p.max_ns + sp;
-      it.o = p.o + p.own_o + slot * p.rep * F::kHd;
-      it.rl = p.rl + p.own_rl + slot * p.rep;
-      run_item<F, 1, 1>(p, it, smem);
+      const int64_t slot = (head * p.max_ns + sp) * p.rep;
+      it.o = p.o + p.own_o + slot * F::kHd;
+      it.rl = p.rl + p.own_rl + slot;
     }
+    it.t1 = min(static_cast<int>((it.n + F::kTile - 1) / F::kTile), it.t1);
+    if (it.t0 >= it.t1) continue;
+    it.par0 = head * S.cache_len;
+    it.k = S.k + it.par0 * F::kRow;
+    it.v = S.v + it.par0 * F::kRow;
+    it.k_par = S.k_par;
+    it.v_par = S.v_par;
+    run_item<F>(p, it, wm, smem);
   }
   // an own length outside its cache with no item of its own (no split at all) is reported here
   if (cta == 0 && pl.ns == 0 && p.own.k)
@@ -803,84 +770,94 @@ __global__ void __launch_bounds__(kThreads, 2) prefix_attn_kernel(const __grid_c
       if (p.own.len[b] < 0 || p.own.len[b] > p.own.cache_len) atomicOr(&g_device_error, static_cast<unsigned>(ERR_ARG));
 }
 
-// One warp joins the partials of one (sequence, query head): prefix splits, then own splits, in order.
+// A CTA joins the partials of one (sequence, query head): prefix splits, then own splits. Warp w takes every fourth
+// one, eight loads at a time; their sums are added in warp order.
 template <int kHd>
 __global__ void __launch_bounds__(kThreads) prefix_attn_merge(const __grid_constant__ Params p, int tile_rows, int stage) {
+  constexpr int kE = kHd / 32;
+  __shared__ float so[kWarps][kHd], sl[kWarps];
   griddep_wait();
   griddep_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  const int row = blockIdx.x * kWarps + (threadIdx.x >> 5);
-  if (row >= p.n_seqs * p.n_q) return;
-  const int b = row / p.n_q, h = row % p.n_q, kv = h / p.rep, j = h % p.rep;
-  const int64_t n_pre = p.pre.k ? *p.pre.len : 0, n_own = p.own.k ? p.own.len[b] : 0;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int b = blockIdx.x / p.n_q, h = blockIdx.x % p.n_q, kv = h / p.rep, j = h % p.rep;
+  const int64_t n_pre = p.pre.k ? __ldcg(p.pre.len) : 0, n_own = p.own.k ? __ldcg(p.own.len + b) : 0;
+  const int np = __ldcg(p.plan), ot = __ldcg(p.plan + 3);
   if (n_pre < 0 || n_pre > p.pre.cache_len || n_own < 0 || n_own > p.own.cache_len) return;
-  const int np = p.plan[0], ot = p.plan[3];
   const int ns = n_own ? static_cast<int>(((n_own + stage - 1) / stage + ot - 1) / ot) : 0;
   const int r = b * p.rep + j, rt = r / tile_rows;
-  const int64_t slot0 = (static_cast<int64_t>(kv) * p.tiles_m + rt) * p.max_np;
-  const int64_t own0 = (static_cast<int64_t>(b) * p.n_kv + kv) * p.max_ns;
-  auto rl_of = [&](int i) {
-    return i < np ? p.rl + (slot0 + i) * tile_rows + r % tile_rows : p.rl + p.own_rl + (own0 + i - np) * p.rep + j;
-  };
-  auto o_of = [&](int i) {
-    return i < np ? p.o + ((slot0 + i) * tile_rows + r % tile_rows) * kHd : p.o + p.own_o + ((own0 + i - np) * p.rep + j) * kHd;
-  };
+  // partial i: row x0 + i xs of the prefix's, then own row y0 + (i - np) rep
+  const int64_t x0 = (static_cast<int64_t>(kv) * p.tiles_m + rt) * p.max_np * tile_rows + r % tile_rows;
+  const int64_t y0 = p.own_rl + (static_cast<int64_t>(b) * p.n_kv + kv) * p.max_ns * p.rep + j;
+  auto at = [&](int i) { return i < np ? x0 + static_cast<int64_t>(i) * tile_rows : y0 + static_cast<int64_t>(i - np) * p.rep; };
   const int n = np + ns;
   float hi = -INFINITY;
-  for (int i = lane; i < n; i += 32) hi = fmaxf(hi, __ldcg(rl_of(i)).x);
+  for (int i = lane; i < n; i += 32) hi = fmaxf(hi, __ldcg(p.rl + at(i)).x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-  constexpr int kE = kHd / 32;
   float acc[kE], l = 0.f;
 #pragma unroll
   for (int e = 0; e < kE; ++e) acc[e] = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) {
-    const float2 v = __ldcg(rl_of(i));
-    const float f = v.x == -INFINITY ? 0.f : ex2(v.x - hi);
-    l = fmaf(v.y, f, l);
-    const float* src = o_of(i) + lane * kE;
-    if constexpr (kE == 4) {
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(src));
-      acc[0] = fmaf(x.x, f, acc[0]), acc[1] = fmaf(x.y, f, acc[1]), acc[2] = fmaf(x.z, f, acc[2]), acc[3] = fmaf(x.w, f, acc[3]);
-    } else {
-      const float2 x = __ldcg(reinterpret_cast<const float2*>(src));
-      acc[0] = fmaf(x.x, f, acc[0]), acc[1] = fmaf(x.y, f, acc[1]);
+  for (int i0 = warp; i0 < n; i0 += 8 * kWarps) {
+    float2 v[8];
+    float x[8][kE];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int i = i0 + k * kWarps;
+      v[k] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int e = 0; e < kE; ++e) x[k][e] = 0.f;
+      if (i < n) {
+        const int64_t a = at(i);
+        v[k] = __ldcg(p.rl + a);
+        if constexpr (kE == 4) {
+          const float4 y = __ldcg(reinterpret_cast<const float4*>(p.o + a * kHd) + lane);
+          x[k][0] = y.x, x[k][1] = y.y, x[k][2] = y.z, x[k][3] = y.w;
+        } else {
+          const float2 y = __ldcg(reinterpret_cast<const float2*>(p.o + a * kHd) + lane);
+          x[k][0] = y.x, x[k][1] = y.y;
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float f = v[k].x == -INFINITY ? 0.f : ex2(v[k].x - hi);
+      l = fmaf(v[k].y, f, l);
+#pragma unroll
+      for (int e = 0; e < kE; ++e) acc[e] = fmaf(x[k][e], f, acc[e]);
     }
   }
-  const float inv = n_pre + n_own == 0 ? 0.f : 1.f / l;
-  uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(p.out) + b * p.ldo + static_cast<int64_t>(h) * kHd + lane * kE);
 #pragma unroll
-  for (int e = 0; e < kE; e += 2) {
-    const float x = n_pre + n_own == 0 ? 0.f : acc[e] * inv, y = n_pre + n_own == 0 ? 0.f : acc[e + 1] * inv;
-    dst[e / 2] = p.bf16 ? pack2<true>(x, y) : pack2<false>(x, y);
+  for (int e = 0; e < kE; ++e) so[warp][lane * kE + e] = acc[e];
+  if (lane == 0) sl[warp] = l;
+  __syncthreads();
+  if (threadIdx.x < kHd / 2) {
+    const int d = 2 * threadIdx.x;
+    float x = 0.f, y = 0.f, lt = 0.f;
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) x += so[k][d], y += so[k][d + 1], lt += sl[k];
+    const bool none = n_pre + n_own == 0;
+    x = none ? 0.f : x / lt;
+    y = none ? 0.f : y / lt;
+    uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + b * p.ldo + static_cast<int64_t>(h) * kHd + d;
+    *reinterpret_cast<uint32_t*>(dst) = p.bf16 ? pack2<true>(x, y) : pack2<false>(x, y);
   }
 }
 
-struct Config {
-  int mt, wm;
-};
-// The narrowest tile that holds the batch's rows: a warp of one or two 16-row tiles reads each key once; beyond 32 rows
-// two or four warps share the keys.
-inline Config config_of(int64_t rows) {
-  if (rows <= 16) return {1, 1};
-  if (rows <= 32) return {2, 1};
-  if (rows <= 64) return {2, 2};
-  return {2, 4};
-}
+// Warps along the rows: the fewest whose 16-row tiles hold the batch's rows, at most four.
+inline int warps_m(int64_t rows) { return rows <= 16 ? 1 : (rows <= 32 ? 2 : 4); }
 
 struct Layout {
-  int grid, tile_rows, tiles_m, max_np, max_ns;
+  int grid, wm, tile_rows, tiles_m, max_np, max_ns;
   int64_t pre_slots, own_slots, rl_bytes, o_bytes, total;
 };
 inline Layout layout_of(const rb_prefix_attn_args* a, int num_sms) {
   const rb_kv_cache* c = a->prefix ? a->prefix : a->own;
   const int rep = a->n_q_heads / c->n_kv_heads;
   const int64_t rows = a->n_seqs * rep;
-  const Config cf = config_of(rows);
   Layout L = {};
-  L.grid = 2 * num_sms;
-  L.tile_rows = 16 * cf.mt * cf.wm;
+  L.grid = kCtasPerSm * num_sms;
+  L.wm = warps_m(rows);
+  L.tile_rows = 16 * L.wm;
   L.tiles_m = static_cast<int>((rows + L.tile_rows - 1) / L.tile_rows);
   const int64_t lanes = static_cast<int64_t>(c->n_kv_heads) * L.tiles_m, heads = a->n_seqs * c->n_kv_heads;
   L.max_np = a->prefix ? static_cast<int>(std::max<int64_t>(1, L.grid / std::max<int64_t>(lanes, 1))) : 0;
@@ -893,42 +870,28 @@ inline Layout layout_of(const rb_prefix_attn_args* a, int num_sms) {
   return L;
 }
 
-template <typename F, int kMt, int kWm>
-int launch_main(const Params& p, int grid, int flags, cudaStream_t stream) {
-  constexpr int smem = Tile<F, kMt, kWm>::kSmem > Tile<F, 1, 1>::kSmem ? Tile<F, kMt, kWm>::kSmem : Tile<F, 1, 1>::kSmem;
-  static_assert(smem <= 113 * 1024, "two CTAs an SM");
-  void (*kern)(Params) = prefix_attn_kernel<F, kMt, kWm>;
-  if (ensure_smem_limit(reinterpret_cast<const void*>(kern), smem) != cudaSuccess) return RB_ERR_LAUNCH;
+inline cudaLaunchConfig_t launch_config(int grid, int smem, int flags, cudaStream_t stream, cudaLaunchAttribute* attr) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = (flags & RB_FLAG_PDL) ? 1 : 0;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, p) == cudaSuccess ? RB_OK : RB_ERR_LAUNCH;
+  return cfg;
 }
 
 template <typename F>
-int launch_format(const Params& p, const Layout& L, Config cf, int flags, cudaStream_t stream) {
-  int st;
-  if (cf.mt == 1) st = launch_main<F, 1, 1>(p, L.grid, flags, stream);
-  else if (cf.wm == 1) st = launch_main<F, 2, 1>(p, L.grid, flags, stream);
-  else if (cf.wm == 2) st = launch_main<F, 2, 2>(p, L.grid, flags, stream);
-  else st = launch_main<F, 2, 4>(p, L.grid, flags, stream);
-  if (st != RB_OK) return st;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((p.n_seqs * p.n_q + kWarps - 1) / kWarps);
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = stream;
+int launch_format(const Params& p, const Layout& L, int flags, cudaStream_t stream) {
+  constexpr int smem = Tile<F>::kSmem;
+  static_assert((smem + 1024) * kCtasPerSm <= 227 * 1024, "CTAs an SM");
   cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = (flags & RB_FLAG_PDL) ? 1 : 0;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  if (ensure_smem_limit(reinterpret_cast<const void*>(prefix_attn_kernel<F>), smem) != cudaSuccess) return RB_ERR_LAUNCH;
+  cudaLaunchConfig_t cfg = launch_config(L.grid, smem, flags, stream, attr);
+  if (cudaLaunchKernelEx(&cfg, prefix_attn_kernel<F>, p) != cudaSuccess) return RB_ERR_LAUNCH;
+  cfg = launch_config(p.n_seqs * p.n_q, 0, flags, stream, attr);
   return cudaLaunchKernelEx(&cfg, prefix_attn_merge<F::kHd>, p, L.tile_rows, F::kTile) == cudaSuccess ? RB_OK : RB_ERR_LAUNCH;
 }
 
@@ -965,21 +928,21 @@ int launch_prefix_attn(const rb_prefix_attn_args* a, int num_sms, int flags, cud
   p.o = reinterpret_cast<float*>(w + 256 + L.rl_bytes);
   p.own_rl = L.pre_slots;
   p.own_o = L.pre_slots * c->head_dim;
-  const Config cf = config_of(a->n_seqs * p.rep);
+  p.wm = L.wm;
   const bool wide = c->head_dim == 128;
   switch (c->fmt) {
     case RB_KV_INT8:
-      return wide ? launch_format<Fmt<128, RB_KV_INT8, false>>(p, L, cf, flags, stream)
-                  : launch_format<Fmt<64, RB_KV_INT8, false>>(p, L, cf, flags, stream);
+      return wide ? launch_format<Fmt<128, RB_KV_INT8, false>>(p, L, flags, stream)
+                  : launch_format<Fmt<64, RB_KV_INT8, false>>(p, L, flags, stream);
     case RB_KV_INT4:
-      return wide ? launch_format<Fmt<128, RB_KV_INT4, false>>(p, L, cf, flags, stream)
-                  : launch_format<Fmt<64, RB_KV_INT4, false>>(p, L, cf, flags, stream);
+      return wide ? launch_format<Fmt<128, RB_KV_INT4, false>>(p, L, flags, stream)
+                  : launch_format<Fmt<64, RB_KV_INT4, false>>(p, L, flags, stream);
     default:
       if (p.bf16)
-        return wide ? launch_format<Fmt<128, RB_KV_PLAIN, true>>(p, L, cf, flags, stream)
-                    : launch_format<Fmt<64, RB_KV_PLAIN, true>>(p, L, cf, flags, stream);
-      return wide ? launch_format<Fmt<128, RB_KV_PLAIN, false>>(p, L, cf, flags, stream)
-                  : launch_format<Fmt<64, RB_KV_PLAIN, false>>(p, L, cf, flags, stream);
+        return wide ? launch_format<Fmt<128, RB_KV_PLAIN, true>>(p, L, flags, stream)
+                    : launch_format<Fmt<64, RB_KV_PLAIN, true>>(p, L, flags, stream);
+      return wide ? launch_format<Fmt<128, RB_KV_PLAIN, false>>(p, L, flags, stream)
+                  : launch_format<Fmt<64, RB_KV_PLAIN, false>>(p, L, flags, stream);
   }
 }
 

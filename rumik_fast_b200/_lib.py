@@ -174,7 +174,13 @@ def dtype_code(dt):
         raise TypeError(f"unsupported dtype {dt}") from None
 
 
+# the current stream's handle without building a Stream object (a call of a microsecond in a launch of a few)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_ptr(device):
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 

@@ -18,13 +18,13 @@ namespace rb {
 namespace bm {
 
 using Key = unsigned long long;
-constexpr int kThreads = 128;
-constexpr int kPer = 32;                       // logits of a thread, held in registers
+constexpr int kThreads = 256;
+constexpr int kPer = 16;                       // logits of a thread, held in registers
 constexpr int kChunk = kThreads * kPer;        // 4096 rows a CTA
 constexpr int kMaxBeams = 32;
 constexpr int kMaxChunks = 256;                // V <= 2^20
-constexpr int kCap = kMaxBeams * (kMaxChunks * kMaxBeams / kThreads);  // keys that may pass a threshold (2048)
-static_assert(kCap >= kMaxBeams * kPer, "a chunk's own candidates fit as well");
+constexpr int kCap = kThreads / 32 * kMaxBeams * kPer;                // keys that may pass a bound: 4096
+static_assert(kCap >= kMaxBeams * (kMaxChunks * kMaxBeams / kThreads), "those of a beam's merged lists as well");
 
 struct SelectParams {
   const void* logits;
@@ -58,57 +58,77 @@ __device__ __forceinline__ float key_value(Key key) {
 __device__ __forceinline__ uint32_t key_row(Key key) { return 0xffffffffu - static_cast<uint32_t>(key); }
 
 struct Shared {
-  Key top[kThreads];
   Key cand[kCap];
-  Key threshold;
+  Key top[kThreads];
+  Key bound[kThreads / 32];
   float2 red[kThreads / 32];
   int n;
   int last;
 };
 
-// The k largest of the CTA's keys, best first, through `out(rank, key)`. get(i) is this thread's i-th key (0: none),
-// i < count. The k-th largest of the threads' own maxima bounds the k-th largest key from below, and at most k
-// threads hold a key at or above it, so at most k count keys are ranked against one another.
-template <int kCount, typename Get, typename Out>
-__device__ __forceinline__ void cta_top(Shared& sh, int k, int count, Get get, Out out) {
-  const int tid = threadIdx.x;
-  Key best = 0;
-#pragma unroll
-  for (int i = 0; i < kCount; ++i)
-    if (i < count) {
-      const Key v = get(i);
-      best = v > best ? v : best;
-    }
-  sh.top[tid] = best;
-  if (tid == 0) {
-    sh.threshold = 1;
-    sh.n = 0;
-  }
-  __syncthreads();
+// A bound that at least k of the CTA's keys reach. `best` is this thread's largest key (0: none). kWide: the k-th
+// largest of all threads' own (at most k threads hold a key that reaches it); else the largest, over the warps, of the
+// k-th largest of a warp's (at most k lanes of each warp do): an eighth of the comparisons.
+template <bool kWide>
+__device__ __forceinline__ Key cta_bound(Shared& sh, int k, Key best) {
+  constexpr int kN = kWide ? kThreads : 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  sh.top[threadIdx.x] = best;
+  if (threadIdx.x == 0) sh.n = 0;
+  if (lane == 0) sh.bound[warp] = 1;
+  if (kWide) __syncthreads();
+  else __syncwarp();
   int rank = 0;
+  const ulonglong2* all = reinterpret_cast<const ulonglong2*>(sh.top + (kWide ? 0 : warp * 32));
 #pragma unroll 8
-  for (int j = 0; j < kThreads; ++j) rank += sh.top[j] > best;
-  if (rank == k - 1 && best != 0) sh.threshold = best;  // keys differ: one thread has this rank
-  __syncthreads();
-  const Key lim = sh.threshold;
-  if (best >= lim) {
-#pragma unroll
-    for (int i = 0; i < kCount; ++i)
-      if (i < count) {
-        const Key v = get(i);
-        if (v >= lim) sh.cand[atomicAdd(&sh.n, 1)] = v;
-      }
+  for (int j = 0; j < kN / 2; ++j) {
+    const ulonglong2 v = all[j];
+    rank += v.x > best;
+    rank += v.y > best;
   }
+  if (rank == k - 1 && best != 0) sh.bound[warp] = best;  // keys differ: one thread has this rank
+  __syncthreads();
+  Key lim = 1;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) lim = sh.bound[w] > lim ? sh.bound[w] : lim;
+  return lim;
+}
+
+// The k largest of the keys in sh.cand, best first, through out(rank, key); ranks without a key get 0.
+template <typename Out>
+__device__ __forceinline__ void cta_rank(Shared& sh, int k, Out out) {
   __syncthreads();
   const int n = sh.n;
-  for (int c = tid; c < n; c += kThreads) {
+#pragma unroll 1
+  for (int c = threadIdx.x; c < n; c += kThreads) {
     const Key v = sh.cand[c];
     int r = 0;
+#pragma unroll 4
     for (int j = 0; j < n; ++j) r += sh.cand[j] > v;
     if (r < k) out(r, v);
   }
-  for (int r = n + tid; r < k; r += kThreads) out(r, Key(0));
+  for (int r = n + threadIdx.x; r < k; r += kThreads) out(r, Key(0));
   __syncthreads();
+}
+
+// The k largest of n keys get(0) .. get(n - 1) (0: none).
+template <typename Get, typename Out>
+__device__ __forceinline__ void cta_top(Shared& sh, int k, int n, Get get, Out out) {
+  Key best = 0;
+#pragma unroll 1
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const Key v = get(i);
+    best = v > best ? v : best;
+  }
+  const Key lim = cta_bound<true>(sh, k, best);
+  if (best >= lim) {
+#pragma unroll 1
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const Key v = get(i);
+      if (v >= lim) sh.cand[atomicAdd(&sh.n, 1)] = v;
+    }
+  }
+  cta_rank(sh, k, out);
 }
 
 // Whether this CTA is the last of `of` to arrive at the ticket, which is then zero again. What the others wrote
@@ -126,10 +146,13 @@ __device__ __forceinline__ bool last_to_arrive(Shared& sh, unsigned int* ticket,
   return sh.last != 0;
 }
 
+__device__ __forceinline__ float exp_of(float x) { return exp2f(x * 1.4426950408889634f); }
+
+// (maximum, sum of exponentials) of two parts; a maximum of +inf marks a part without a distribution.
 __device__ __forceinline__ float2 merge_sums(float2 a, float2 b) {
   const float m = fmaxf(a.x, b.x);
-  if (m == -INFINITY) return make_float2(m, 0.f);
-  return make_float2(m, a.y * expf(a.x - m) + b.y * expf(b.x - m));
+  if (m == -INFINITY || m == INFINITY) return make_float2(m, 0.f);
+  return make_float2(m, a.y * exp_of(a.x - m) + b.y * exp_of(b.x - m));
 }
 
 template <typename T>
@@ -145,44 +168,52 @@ __global__ void __launch_bounds__(kThreads) beam_select_kernel(const __grid_cons
   const bool done = p.done[row] != 0;
   const bool dead = !(score > -INFINITY && score < INFINITY);  // no candidate of this beam counts
   if (!done && !dead) {
-    const T* x = reinterpret_cast<const T*>(p.logits) + row * p.ld;
     const int first = chunk * kChunk + tid;
+    const T* x = reinterpret_cast<const T*>(p.logits) + row * p.ld + first;
     float v[kPer];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int at = first + i * kThreads;
-      v[i] = at < p.V ? static_cast<float>(x[at]) : -INFINITY;
-    }
-    float top = -INFINITY;
-    bool odd = false;
+    for (int i = 0; i < kPer; ++i) v[i] = first + i * kThreads < p.V ? static_cast<float>(x[i * kThreads]) + 0.f : -INFINITY;  // -0 -> +0
+    if (early) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      if (early && first + i * kThreads == p.end_idx) v[i] = -INFINITY;
-      odd |= !(v[i] < INFINITY);  // NaN or +inf: the row has no distribution
-      top = fmaxf(top, v[i]);
+      for (int i = 0; i < kPer; ++i)
+        if (first + i * kThreads == p.end_idx) v[i] = -INFINITY;
     }
-    float sum = 0.f;
-    if (top > -INFINITY) {
+    float top = v[0];
+    int at = 0;
+    bool odd = !(v[0] < INFINITY);  // NaN or +inf: the row has no distribution
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) sum += expf(v[i] - top);
+    for (int i = 1; i < kPer; ++i) {
+      odd |= !(v[i] < INFINITY);
+      if (v[i] > top) top = v[i], at = i;  // the lowest row among equals
     }
-    float2 ms = odd ? make_float2(INFINITY, 0.f) : make_float2(top, sum);
+    float2 ms = make_float2(odd ? INFINITY : top, 0.f);
+    if (!odd && top > -INFINITY) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float2 b = make_float2(__shfl_xor_sync(0xffffffffu, ms.x, o), __shfl_xor_sync(0xffffffffu, ms.y, o));
-      ms = ms.x == INFINITY || b.x == INFINITY ? make_float2(INFINITY, 0.f) : merge_sums(ms, b);
+      for (int i = 0; i < kPer; ++i) ms.y += exp_of(v[i] - top);
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+      ms = merge_sums(ms, make_float2(__shfl_xor_sync(0xffffffffu, ms.x, o), __shfl_xor_sync(0xffffffffu, ms.y, o)));
     if (lane == 0) sh.red[warp] = ms;
-    __syncthreads();
+    // rows past the vocabulary hold -inf like masked ones, but no key
+    const Key best = first < p.V ? make_key(top, first + at * kThreads) : Key(0);
+    const Key lim = cta_bound<false>(sh, nb, best);
     if (tid == 0) {
-      for (int w = 1; w < kThreads / 32; ++w)
-        ms = ms.x == INFINITY || sh.red[w].x == INFINITY ? make_float2(INFINITY, 0.f) : merge_sums(ms, sh.red[w]);
+#pragma unroll 1
+      for (int w = 1; w < kThreads / 32; ++w) ms = merge_sums(ms, sh.red[w]);
       p.part[static_cast<int64_t>(row) * p.chunks + chunk] = ms;
     }
+    if (best >= lim) {
+      const float least = key_value(lim);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if ((!(v[i] < least) || lim == 1) && first + i * kThreads < p.V) {
+          const Key key = make_key(v[i], first + i * kThreads);
+          if (key >= lim) sh.cand[atomicAdd(&sh.n, 1)] = key;
+        }
+    }
     Key* dst = p.keys + (static_cast<int64_t>(row) * p.chunks + chunk) * nb;
-    cta_top<kPer>(sh, nb, kPer,
-                  [&](int i) { const int at = first + i * kThreads; return at < p.V ? make_key(v[i], at) : Key(0); },
-                  [&](int r, Key key) { dst[r] = key; });
+    cta_rank(sh, nb, [&](int r, Key key) { dst[r] = key; });
   }
   if (!last_to_arrive(sh, p.tickets + row, p.chunks)) return;
 
@@ -192,20 +223,20 @@ __global__ void __launch_bounds__(kThreads) beam_select_kernel(const __grid_cons
   float2 ms = make_float2(-INFINITY, 0.f);
   bool odd = false;
   if (!done && !dead) {
-    for (int c = 0; c < p.chunks; ++c) {  // in chunk order, by every thread: the same sum everywhere
-      const float2 b = __ldcg(p.part + static_cast<int64_t>(row) * p.chunks + c);
-      odd |= b.x == INFINITY;
-      if (!odd) ms = merge_sums(ms, b);
-    }
+    // every warp merges the chunks' sums, lane l those of chunks l, l + 32, ...: the same sum everywhere
+#pragma unroll 1
+    for (int c = lane; c < p.chunks; c += 32) ms = merge_sums(ms, __ldcg(p.part + static_cast<int64_t>(row) * p.chunks + c));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+      ms = merge_sums(ms, make_float2(__shfl_xor_sync(0xffffffffu, ms.x, o), __shfl_xor_sync(0xffffffffu, ms.y, o)));
+    odd = ms.x == INFINITY;
     if (odd && tid == 0) atomicOr(&g_device_error, static_cast<unsigned>(ERR_ARG));
   }
   if (!done && !dead && !odd && ms.x > -INFINITY) {
-    const float lse = ms.x + logf(ms.y);
+    const float lse = ms.x + logf(ms.y);  // ms.y >= 1 up to rounding: the largest logit's own term
     const Key* src = p.keys + static_cast<int64_t>(row) * p.chunks * nb;
-    const int n = p.chunks * nb, count = (n + kThreads - 1) / kThreads;
-    cta_top<kMaxChunks * kMaxBeams / kThreads>(
-        sh, nb, count,
-        [&](int i) { const int at = i * kThreads + tid; return at < n ? __ldcg(src + at) : Key(0); },
+    cta_top(
+        sh, nb, p.chunks * nb, [&](int i) { return __ldcg(src + i); },
         [&](int r, Key key) {
           cand[r] = key ? (key_value(key) - lse) + score : -INFINITY;
           idx[r] = key ? static_cast<int>(key_row(key)) : -1;
@@ -223,14 +254,10 @@ __global__ void __launch_bounds__(kThreads) beam_select_kernel(const __grid_cons
   if (!last_to_arrive(sh, p.tickets + gridDim.y + req, nb)) return;
 
   // ---- the request's nb best: keys of (candidate, place in the order beam, rank within the beam) ----
-  const int n = nb * nb, count = (n + kThreads - 1) / kThreads;
   const int64_t base = static_cast<int64_t>(req) * nb * nb;
-  cta_top<kMaxBeams * kMaxBeams / kThreads>(
-      sh, nb, count,
-      [&](int i) {
-        const int at = i * kThreads + tid;
-        return at < n && __ldcg(p.row_idx + base + at) >= 0 ? make_key(__ldcg(p.row_cand + base + at), at) : Key(0);
-      },
+  cta_top(
+      sh, nb, nb * nb,
+      [&](int i) { return __ldcg(p.row_idx + base + i) >= 0 ? make_key(__ldcg(p.row_cand + base + i), i) : Key(0); },
       [&](int r, Key key) {
         if (key == 0) return;  // not reached: every beam gives min(nb, V) rows
         const int at = static_cast<int>(key_row(key)), parent = at / nb;
@@ -244,6 +271,8 @@ __global__ void __launch_bounds__(kThreads) beam_select_kernel(const __grid_cons
 }
 
 // ---- reordering ----
+
+constexpr int kReorderThreads = 128;
 
 struct Tensor {
   uint8_t* p;
@@ -263,8 +292,8 @@ static_assert(sizeof(ReorderParams) < 4096, "kernel parameters");
 template <typename U, int kBeams>
 __device__ __forceinline__ void reorder_line(uint8_t* base, int64_t beam_bytes, const int* parent, const int64_t* bytes,
                                              uint32_t needed, int nb, int64_t most, int piece, int pieces) {
-  for (int64_t at = (static_cast<int64_t>(piece) * kThreads + threadIdx.x) * sizeof(U); at < most;
-       at += static_cast<int64_t>(pieces) * kThreads * sizeof(U)) {
+  for (int64_t at = (static_cast<int64_t>(piece) * kReorderThreads + threadIdx.x) * sizeof(U); at < most;
+       at += static_cast<int64_t>(pieces) * kReorderThreads * sizeof(U)) {
     // one column of every beam that another one takes over, all read before any is written: the columns of a line
     // are independent, so the beams change places in place
     U v[kBeams];
@@ -281,7 +310,7 @@ __device__ __forceinline__ void reorder_line(uint8_t* base, int64_t beam_bytes, 
 }
 
 template <int kBeams>
-__global__ void __launch_bounds__(kThreads) beam_reorder_kernel(const __grid_constant__ ReorderParams p) {
+__global__ void __launch_bounds__(kReorderThreads) beam_reorder_kernel(const __grid_constant__ ReorderParams p) {
   __shared__ int parent[kMaxBeams];
   __shared__ int64_t bytes[kMaxBeams];
   griddep_wait();
@@ -408,10 +437,10 @@ int launch_beam_reorder(const rb_beam_tensor* t, int count, int64_t requests, in
     }
     // about eight CTAs an SM, and no more pieces of a line than it has columns for
     int64_t pieces = (8 * static_cast<int64_t>(num_sms) + lines * requests - 1) / (lines * requests);
-    pieces = std::max<int64_t>(1, std::min<int64_t>(pieces, (widest + kThreads - 1) / kThreads));
+    pieces = std::max<int64_t>(1, std::min<int64_t>(pieces, (widest + kReorderThreads - 1) / kReorderThreads));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(lines, static_cast<unsigned>(pieces), static_cast<unsigned>(requests));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(kReorderThreads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -591,7 +591,7 @@ int rb_kv_write(const rb_kv_cache* cache, const void* k, const void* v, const in
     if (k_stride[i] % 8 != 0 || v_stride[i] % 8 != 0) return RB_ERR_ALIGN;
   int sms = 0;
   if ((st = device_sms(&sms)) != RB_OK) return st;
-  st = rb::launch_kv_write(cache, k, v, k_stride, v_stride, n_tokens, pos, sms, flags, static_cast<cudaStream_t>(stream));
+  st = rb::launch_kv_write(cache, k, v, k_stride, v_stride, n_tokens, pos, flags, static_cast<cudaStream_t>(stream));
   if (st == RB_OK && cudaGetLastError() != cudaSuccess) st = RB_ERR_LAUNCH;
   return st;
 }
@@ -606,7 +606,7 @@ int rb_kv_read(const rb_kv_cache* cache, void* k_out, void* v_out, int64_t start
   if (!aligned16(k_out) || !aligned16(v_out)) return RB_ERR_ALIGN;
   int sms = 0;
   if ((st = device_sms(&sms)) != RB_OK) return st;
-  st = rb::launch_kv_read(cache, k_out, v_out, start, count, sms, flags, static_cast<cudaStream_t>(stream));
+  st = rb::launch_kv_read(cache, k_out, v_out, start, count, flags, static_cast<cudaStream_t>(stream));
   if (st == RB_OK && cudaGetLastError() != cudaSuccess) st = RB_ERR_LAUNCH;
   return st;
 }

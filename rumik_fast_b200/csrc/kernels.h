@@ -68,8 +68,8 @@ int launch_attn_decode(const void* q, const void* kc, const void* vc, const int6
 // Caches of a batch of sequences (kv_cache.cu), its attention (prefix_attn.cu) and a beam search's step (beams.cu);
 // arguments as in the header, already checked.
 int launch_kv_write(const rb_kv_cache* c, const void* k, const void* v, const int64_t* ks, const int64_t* vs,
-                    int64_t n_tokens, const int64_t* pos, int num_sms, int flags, cudaStream_t stream);
-int launch_kv_read(const rb_kv_cache* c, void* k_out, void* v_out, int64_t start, int64_t count, int num_sms, int flags,
+                    int64_t n_tokens, const int64_t* pos, int flags, cudaStream_t stream);
+int launch_kv_read(const rb_kv_cache* c, void* k_out, void* v_out, int64_t start, int64_t count, int flags,
                    cudaStream_t stream);
 int64_t prefix_attn_workspace(const rb_prefix_attn_args* a, int num_sms);
 int launch_prefix_attn(const rb_prefix_attn_args* a, int num_sms, int flags, cudaStream_t stream);

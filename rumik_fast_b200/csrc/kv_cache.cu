@@ -8,7 +8,8 @@
 // The scale is rounded to bf16 BEFORE the codes are computed against it, so its 8 bits cost nothing (127 s and 15 s
 // stay within half a step of the largest value) and it keeps fp32's range, which an fp16 scale would not. x (11 bits)
 // over s (8 bits) is either exactly a half-integer or at least 2^-16 of itself away from one, so the codes do not
-// depend on how wide the quotient is computed.
+// depend on how wide the quotient is computed; away from ties x times the reciprocal of s gives the same code, and a
+// thread divides only where one of its eight is near one.
 // A row with a NaN or an infinity gets s = NaN and codes of zero: all of it reads back as NaN, in this kernel and in
 // the attention. s == 0 (a row of equal values, or of zeros) gives codes of zero.
 #include "common.cuh"
@@ -30,15 +31,15 @@ struct Rows {  // one of k, v: the row source (or destination) and the cache sid
 struct WriteParams {
   Rows r[2];
   const int64_t* pos;
-  int64_t n_seqs, n_tokens, cache_len;
-  int n_heads, bf16;
+  int64_t n_seqs, n_tokens, cache_len, tiles;  // tiles: CTAs of one (key or value, sequence)
+  int n_heads, bf16, by_head;
 };
 
 struct ReadParams {
   const void* c[2];
   const void* par[2];
   void* out[2];
-  int64_t n_seqs, start, count, cache_len;
+  int64_t n_seqs, start, count, cache_len, tiles;  // tiles: CTAs of one (key or value, sequence, head)
   int n_heads, bf16;
 };
 
@@ -58,88 +59,125 @@ __device__ __forceinline__ bool group_any(bool b) {
 
 __device__ __forceinline__ float bf16_round(float v) { return __bfloat162float(__float2bfloat16_rn(v)); }
 
-// kLanes lanes hold a row, 8 values each (one 16-byte load).
+// rint(x / s) clamped to [lo, hi] for a thread's eight values; s > 0.
+__device__ __forceinline__ void quantise8(const float (&x)[8], float s, float lo, float hi, float (&q)[8]) {
+  const float inv = __frcp_rn(s);
+  bool near = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float t = x[e] * inv;  // within 2^-22 of x / s (and at most 128 of them here): 1e-4 decides
+    q[e] = rintf(t);
+    near |= !(fabsf(t - q[e]) <= 0.4999f);  // also where the reciprocal overflowed
+  }
+  if (near) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q[e] = rintf(__fdiv_rn(x[e], s));
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) q[e] = fminf(fmaxf(q[e], lo), hi);
+}
+
+// kLanes lanes hold a row, 8 values each (one 16-byte load). A CTA takes kGroups x kRows rows of one (key or value,
+// sequence): consecutive tokens of one head, whose parameters then leave as one contiguous store, or, when there are
+// fewer tokens than kGroups (a decode step), rows in (token, head) order. All of a thread's loads go out first.
+constexpr int kRows = 4;
+
 template <int kHd, int kFmt>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constant__ WriteParams p) {
-  constexpr int kLanes = kHd / 8;
+  constexpr int kLanes = kHd / 8, kGroups = kThreads / kLanes, kTile = kGroups * kRows;
+  __shared__ uint32_t par[kTile];
   griddep_wait();
   griddep_launch_dependents();
-  const int sub = threadIdx.x % kLanes;
-  const int64_t rows = 2 * p.n_seqs * p.n_tokens * p.n_heads;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * (kThreads / kLanes);
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * (kThreads / kLanes);
-  // every lane of a warp takes part in the row reductions: the loop bound is the same for the whole CTA
-  for (int64_t base = first; base < rows; base += step) {
-    const int64_t row = base + threadIdx.x / kLanes;
-    const bool in = row < rows;
-    int64_t i = in ? row : 0;
-    const int h = static_cast<int>(i % p.n_heads);
-    i /= p.n_heads;
-    const int64_t t = i % p.n_tokens;
-    i /= p.n_tokens;
-    const int64_t b = i % p.n_seqs;
-    const Rows& R = p.r[i / p.n_seqs];
-    const int64_t at = p.pos[b];
+  const int sub = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
+  const int64_t which_seq = blockIdx.x / p.tiles;
+  const int64_t tile = blockIdx.x - which_seq * p.tiles;
+  const int64_t b = which_seq % p.n_seqs;
+  const Rows& R = p.r[which_seq >= p.n_seqs];
+  const int64_t at = __ldcg(p.pos + b);
+  int64_t t0, limit;  // the tile's first token (by_head) or row, and the end
+  int h0 = 0;
+  if (p.by_head) {
+    h0 = static_cast<int>(tile % p.n_heads);
+    t0 = tile / p.n_heads * kTile;
+    limit = p.n_tokens;
+  } else {
+    t0 = tile * kTile;
+    limit = p.n_tokens * p.n_heads;
+  }
+  uint4 raw[kRows];
+  int64_t dst[kRows];  // the row in the cache; -1: nothing to store
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int64_t x = t0 + i * kGroups + grp;
+    const bool in = x < limit;
+    const int64_t t = in ? (p.by_head ? x : x / p.n_heads) : 0;
+    const int h = p.by_head ? h0 : static_cast<int>(in ? x % p.n_heads : 0);
     const bool fits = at >= -t && at < p.cache_len - t;  // 0 <= at + t < cache_len, without the sum (at may be any)
     if (in && !fits && sub == 0) atomicOr(&g_device_error, static_cast<unsigned>(ERR_ARG));
-    const int64_t slot = fits ? at + t : 0;
-    const uint4 raw = ldg_cg_128(reinterpret_cast<const uint16_t*>(R.x) + b * R.s_seq + t * R.s_tok + h * R.s_head + sub * 8);
-    const int64_t dst = (b * p.n_heads + h) * p.cache_len + slot;
-    const bool store = in && fits;
+    dst[i] = in && fits ? (b * p.n_heads + h) * p.cache_len + at + t : -1;
+    raw[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (dst[i] >= 0)
+      raw[i] = ldg_cg_128(reinterpret_cast<const uint16_t*>(R.x) + b * R.s_seq + t * R.s_tok + h * R.s_head + sub * 8);
+  }
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
     if constexpr (kFmt == RB_KV_PLAIN) {
-      if (store) reinterpret_cast<uint4*>(R.c)[dst * kLanes + sub] = raw;
-      continue;
-    }
-    float x[8];
-    raw_to_f32(raw, p.bf16 != 0, x);
-    if constexpr (kFmt == RB_KV_INT8) {
-      float top = 0.f;
-      bool odd = false;  // NaN or infinity
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        top = fmaxf(top, fabsf(x[e]));
-        odd |= !(fabsf(x[e]) <= 3.402823466e38f);
-      }
-      top = group_max<kLanes>(top);
-      odd = group_any<kLanes>(odd);
-      const float s = odd ? __int_as_float(0x7fc00000) : bf16_round(__fdiv_rn(top, 127.f));
-      uint32_t w[2] = {0u, 0u};
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float q = s > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(x[e], s)), -127.f), 127.f) : 0.f;
-        w[e >> 2] |= static_cast<uint32_t>(static_cast<int>(q) + 128) << (8 * (e & 3));
-      }
-      if (store) {
-        reinterpret_cast<uint2*>(R.c)[dst * kLanes + sub] = make_uint2(w[0], w[1]);
-        if (sub == 0) reinterpret_cast<__nv_bfloat16*>(R.par)[dst] = __float2bfloat16_rn(s);
-      }
+      if (dst[i] >= 0) reinterpret_cast<uint4*>(R.c)[dst[i] * kLanes + sub] = raw[i];
     } else {
+      float x[8], q[8];
+      raw_to_f32(raw[i], p.bf16 != 0, x);
       float hi = x[0], lo = -x[0];
-      bool odd = false;
+      bool odd = false;  // NaN or infinity
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         hi = fmaxf(hi, x[e]);
         lo = fmaxf(lo, -x[e]);
         odd |= !(fabsf(x[e]) <= 3.402823466e38f);
       }
-      hi = group_max<kLanes>(hi);
-      const float m = -group_max<kLanes>(lo);
-      odd = group_any<kLanes>(odd);
-      const float range = hi - m;
-      const float s = odd || !(range <= 3.402823466e38f) ? __int_as_float(0x7fc00000) : bf16_round(__fdiv_rn(range, 15.f));
-      uint32_t w = 0u;
+      float m = 0.f, s;
+      if constexpr (kFmt == RB_KV_INT8) {
+        s = bf16_round(__fdiv_rn(group_max<kLanes>(fmaxf(hi, lo)), 127.f));
+      } else {
+        hi = group_max<kLanes>(hi);
+        m = -group_max<kLanes>(lo);
+        const float range = hi - m;
+        odd |= !(range <= 3.402823466e38f);
+        s = bf16_round(__fdiv_rn(range, 15.f));
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float q = s > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(x[e] - m, s)), 0.f), 15.f) : 0.f;
-        w |= static_cast<uint32_t>(static_cast<int>(q)) << (4 * e);
+        for (int e = 0; e < 8; ++e) x[e] -= m;
       }
-      if (store) {
-        reinterpret_cast<uint32_t*>(R.c)[dst * kLanes + sub] = w;
-        if (sub == 0) {
-          const uint32_t mb = p.bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(m)) : __half_as_ushort(__float2half_rn(m));
-          reinterpret_cast<uint32_t*>(R.par)[dst] = __bfloat16_as_ushort(__float2bfloat16_rn(s)) | (mb << 16);
-        }
+      if (group_any<kLanes>(odd)) s = __int_as_float(0x7fc00000);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) q[e] = 0.f;
+      if (s > 0.f) quantise8(x, s, kFmt == RB_KV_INT8 ? -127.f : 0.f, kFmt == RB_KV_INT8 ? 127.f : 15.f, q);
+      uint32_t w[2] = {0u, 0u}, word = __bfloat16_as_ushort(__float2bfloat16_rn(s));
+      if constexpr (kFmt == RB_KV_INT8) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e >> 2] |= static_cast<uint32_t>(static_cast<int>(q[e]) + 128) << (8 * (e & 3));
+        if (dst[i] >= 0) reinterpret_cast<uint2*>(R.c)[dst[i] * kLanes + sub] = make_uint2(w[0], w[1]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[0] |= static_cast<uint32_t>(static_cast<int>(q[e])) << (4 * e);
+        if (dst[i] >= 0) reinterpret_cast<uint32_t*>(R.c)[dst[i] * kLanes + sub] = w[0];
+        word |= static_cast<uint32_t>(p.bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(m)) : __half_as_ushort(__float2half_rn(m))) << 16;
       }
+      if (p.by_head) {
+        if (sub == 0) par[i * kGroups + grp] = word;
+      } else if (sub == 0 && dst[i] >= 0) {
+        if constexpr (kFmt == RB_KV_INT8) reinterpret_cast<uint16_t*>(R.par)[dst[i]] = static_cast<uint16_t>(word);
+        else reinterpret_cast<uint32_t*>(R.par)[dst[i]] = word;
+      }
+    }
+  }
+  if constexpr (kFmt != RB_KV_PLAIN) {
+    if (!p.by_head) return;
+    __syncthreads();
+    for (int i = threadIdx.x; i < kTile; i += kThreads) {
+      const int64_t t = t0 + i;
+      if (t >= limit || !(at >= -t && at < p.cache_len - t)) continue;
+      const int64_t row = (b * p.n_heads + h0) * p.cache_len + at + t;
+      if constexpr (kFmt == RB_KV_INT8) reinterpret_cast<uint16_t*>(R.par)[row] = static_cast<uint16_t>(par[i]);
+      else reinterpret_cast<uint32_t*>(R.par)[row] = par[i];
     }
   }
 }
@@ -158,52 +196,68 @@ __device__ __forceinline__ uint32_t pack_act2(float a, float b, bool bf16) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// A CTA reads kThreads x kUnits pieces of eight values of one (key or value, sequence, head); its loads go out first.
+constexpr int kUnits = 4;
+
 template <int kHd, int kFmt>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant__ ReadParams p) {
   constexpr int kLanes = kHd / 8;
   griddep_wait();
   griddep_launch_dependents();
-  const int64_t units = 2 * p.n_seqs * p.n_heads * p.count * kLanes;  // 8 values each
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
-  for (int64_t u = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; u < units; u += step) {
-    const int sub = static_cast<int>(u % kLanes);
-    const int64_t row = u / kLanes;
-    const int64_t t = row % p.count;
-    int64_t i = row / p.count;
-    const int64_t bh = i % (p.n_seqs * p.n_heads);
-    const int which = static_cast<int>(i / (p.n_seqs * p.n_heads));
-    const int64_t src = bh * p.cache_len + p.start + t;
-    uint4* out = reinterpret_cast<uint4*>(p.out[which]) + (bh * p.count + t) * kLanes + sub;
+  const int64_t line = blockIdx.x / p.tiles;
+  const int64_t u0 = (blockIdx.x - line * p.tiles) * (kThreads * kUnits) + threadIdx.x, units = p.count * kLanes;
+  const int64_t heads = p.n_seqs * p.n_heads;
+  const int which = line >= heads;
+  const int64_t bh = which ? line - heads : line, src = bh * p.cache_len + p.start;
+  uint4* out = reinterpret_cast<uint4*>(p.out[which]) + bh * units;
+  uint4 raw[kUnits];
+  uint32_t word[kUnits];
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    const int64_t u = u0 + i * kThreads;
+    raw[i] = make_uint4(0u, 0u, 0u, 0u);
+    word[i] = 0u;
+    if (u >= units) continue;
+    const int64_t at = src * kLanes + u;
     if constexpr (kFmt == RB_KV_PLAIN) {
-      *out = ldg_cg_128(reinterpret_cast<const uint4*>(p.c[which]) + src * kLanes + sub);
+      raw[i] = ldg_cg_128(reinterpret_cast<const uint4*>(p.c[which]) + at);
+    } else if constexpr (kFmt == RB_KV_INT8) {
+      const uint2 w = __ldcg(reinterpret_cast<const uint2*>(p.c[which]) + at);
+      raw[i].x = w.x, raw[i].y = w.y;
+      word[i] = __ldcg(reinterpret_cast<const unsigned short*>(p.par[which]) + src + u / kLanes);
+    } else {
+      raw[i].x = __ldcg(reinterpret_cast<const unsigned int*>(p.c[which]) + at);
+      word[i] = __ldcg(reinterpret_cast<const unsigned int*>(p.par[which]) + src + u / kLanes);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    const int64_t u = u0 + i * kThreads;
+    if (u >= units) continue;
+    if constexpr (kFmt == RB_KV_PLAIN) {
+      out[u] = raw[i];
     } else {
       float v[8];
+      const float s = __uint_as_float(word[i] << 16);
       if constexpr (kFmt == RB_KV_INT8) {
-        const uint2 w = __ldcg(reinterpret_cast<const uint2*>(p.c[which]) + src * kLanes + sub);
-        const float s = __uint_as_float(static_cast<uint32_t>(__ldcg(reinterpret_cast<const unsigned short*>(p.par[which]) + src)) << 16);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t c = ((e < 4 ? w.x : w.y) >> (8 * (e & 3))) & 255u;
-          v[e] = static_cast<float>(static_cast<int>(c) - 128) * s;
-        }
+        for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(static_cast<int>(((e < 4 ? raw[i].x : raw[i].y) >> (8 * (e & 3))) & 255u) - 128) * s;
       } else {
-        const uint32_t w = __ldcg(reinterpret_cast<const uint32_t*>(p.c[which]) + src * kLanes + sub);
-        const uint32_t sm = __ldcg(reinterpret_cast<const uint32_t*>(p.par[which]) + src);
-        const float s = __uint_as_float(sm << 16);
-        const float m = p.bf16 ? __uint_as_float(sm & 0xffff0000u) : __half2float(__ushort_as_half(static_cast<unsigned short>(sm >> 16)));
+        const float m = p.bf16 ? __uint_as_float(word[i] & 0xffff0000u) : __half2float(__ushort_as_half(static_cast<unsigned short>(word[i] >> 16)));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = fmaf(static_cast<float>((w >> (4 * e)) & 15u), s, m);
+        for (int e = 0; e < 8; ++e) v[e] = fmaf(static_cast<float>((raw[i].x >> (4 * e)) & 15u), s, m);
       }
-      *out = make_uint4(pack_act2(v[0], v[1], p.bf16), pack_act2(v[2], v[3], p.bf16), pack_act2(v[4], v[5], p.bf16),
-                        pack_act2(v[6], v[7], p.bf16));
+      out[u] = make_uint4(pack_act2(v[0], v[1], p.bf16), pack_act2(v[2], v[3], p.bf16), pack_act2(v[4], v[5], p.bf16),
+                          pack_act2(v[6], v[7], p.bf16));
     }
   }
 }
 
 template <typename P>
-int launch(void (*kern)(P), const P& p, int64_t blocks, int num_sms, int flags, cudaStream_t stream) {
+int launch(void (*kern)(P), const P& p, int64_t blocks, int flags, cudaStream_t stream) {
+  if (blocks > (int64_t(1) << 31) - 1) return RB_ERR_SHAPE;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(blocks, 16 * static_cast<int64_t>(num_sms))));
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -217,7 +271,7 @@ int launch(void (*kern)(P), const P& p, int64_t blocks, int num_sms, int flags, 
 }  // namespace kvc
 
 int launch_kv_write(const rb_kv_cache* c, const void* k, const void* v, const int64_t* ks, const int64_t* vs,
-                    int64_t n_tokens, const int64_t* pos, int num_sms, int flags, cudaStream_t stream) {
+                    int64_t n_tokens, const int64_t* pos, int flags, cudaStream_t stream) {
   using namespace kvc;
   WriteParams p = {};
   p.r[0] = {k, ks[0], ks[1], ks[2], c->k, c->k_par};
@@ -228,8 +282,10 @@ int launch_kv_write(const rb_kv_cache* c, const void* k, const void* v, const in
   p.cache_len = c->cache_len;
   p.n_heads = c->n_kv_heads;
   p.bf16 = c->dtype == RB_BF16;
-  const int64_t per = kThreads / (c->head_dim / 8);
-  const int64_t blocks = (2 * c->n_seqs * n_tokens * c->n_kv_heads + per - 1) / per;
+  const int64_t groups = kThreads / (c->head_dim / 8), tile = groups * kRows;
+  p.by_head = n_tokens >= groups;
+  p.tiles = p.by_head ? (n_tokens + tile - 1) / tile * c->n_kv_heads : (n_tokens * c->n_kv_heads + tile - 1) / tile;
+  const int64_t blocks = 2 * c->n_seqs * p.tiles;
   void (*kern)(WriteParams) = nullptr;
   if (c->head_dim == 128)
     kern = c->fmt == RB_KV_INT8 ? kv_write_kernel<128, RB_KV_INT8>
@@ -237,10 +293,10 @@ int launch_kv_write(const rb_kv_cache* c, const void* k, const void* v, const in
   else
     kern = c->fmt == RB_KV_INT8 ? kv_write_kernel<64, RB_KV_INT8>
                                 : (c->fmt == RB_KV_INT4 ? kv_write_kernel<64, RB_KV_INT4> : kv_write_kernel<64, RB_KV_PLAIN>);
-  return launch(kern, p, blocks, num_sms, flags, stream);
+  return launch(kern, p, blocks, flags, stream);
 }
 
-int launch_kv_read(const rb_kv_cache* c, void* k_out, void* v_out, int64_t start, int64_t count, int num_sms, int flags,
+int launch_kv_read(const rb_kv_cache* c, void* k_out, void* v_out, int64_t start, int64_t count, int flags,
                    cudaStream_t stream) {
   using namespace kvc;
   ReadParams p = {};
@@ -256,7 +312,8 @@ int launch_kv_read(const rb_kv_cache* c, void* k_out, void* v_out, int64_t start
   p.cache_len = c->cache_len;
   p.n_heads = c->n_kv_heads;
   p.bf16 = c->dtype == RB_BF16;
-  const int64_t blocks = (2 * c->n_seqs * c->n_kv_heads * count * (c->head_dim / 8) + kThreads - 1) / kThreads;
+  p.tiles = (count * (c->head_dim / 8) + kThreads * kUnits - 1) / (kThreads * kUnits);
+  const int64_t blocks = 2 * c->n_seqs * c->n_kv_heads * p.tiles;
   void (*kern)(ReadParams) = nullptr;
   if (c->head_dim == 128)
     kern = c->fmt == RB_KV_INT8 ? kv_read_kernel<128, RB_KV_INT8>
@@ -264,7 +321,7 @@ int launch_kv_read(const rb_kv_cache* c, void* k_out, void* v_out, int64_t start
   else
     kern = c->fmt == RB_KV_INT8 ? kv_read_kernel<64, RB_KV_INT8>
                                 : (c->fmt == RB_KV_INT4 ? kv_read_kernel<64, RB_KV_INT4> : kv_read_kernel<64, RB_KV_PLAIN>);
-  return launch(kern, p, blocks, num_sms, flags, stream);
+  return launch(kern, p, blocks, flags, stream);
 }
 
 }  // namespace rb

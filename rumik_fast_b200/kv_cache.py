@@ -20,6 +20,7 @@ import torch
 from . import _lib, config
 from .cuda_gemv import _on_device, _require
 
+_Strides = ctypes.c_int64 * 3
 FORMATS = {"plain": _lib.KV_PLAIN, "int8": _lib.KV_INT8, "int4": _lib.KV_INT4}
 
 
@@ -87,39 +88,44 @@ class KVCache:
         return [t for t in (self.k, self.v, self.k_par, self.v_par) if t is not None]
 
     def _rows(self, x, nm):
-        if x.dim() == 3:   # one token: [n_seqs, n_kv_heads, head_dim]
+        shape = x.shape
+        if len(shape) == 3:   # one token: [n_seqs, n_kv_heads, head_dim]
             x = x.unsqueeze(1)
-        _require(x.device == self.device and x.dtype == self.dtype, f"{nm} must be a {self.dtype} tensor on {self.device}")
-        _require(x.dim() == 4 and x.shape[0] == self.n_seqs and x.shape[2:] == (self.n_kv_heads, self.head_dim),
-                 f"{nm} must be [{self.n_seqs}, T, {self.n_kv_heads}, {self.head_dim}] (or without T), got {tuple(x.shape)}")
-        _require(x.stride(3) == 1, f"{nm} must have unit stride in its last dimension")
-        return x
+            shape = x.shape
+        if x.dtype != self.dtype or x.device != self.device:
+            _require(False, f"{nm} must be a {self.dtype} tensor on {self.device}")
+        if len(shape) != 4 or shape[0] != self.n_seqs or shape[2] != self.n_kv_heads or shape[3] != self.head_dim:
+            _require(False, f"{nm} must be [{self.n_seqs}, T, {self.n_kv_heads}, {self.head_dim}] (or without T), got {tuple(shape)}")
+        s0, s1, s2, s3 = x.stride()
+        _require(s3 == 1, "k and v must have unit stride in their last dimension")
+        return x, shape[1], _Strides(s0, s1, s2)
 
     def write(self, k, v, pos):
         """Rows k, v [n_seqs, T, n_kv_heads, head_dim] (or [n_seqs, n_kv_heads, head_dim]: one token) into the slots
         pos[b] .. pos[b] + T - 1 (pos: int64 [n_seqs] on the device). A slot outside the cache is not written and sets
         the RB_DEVERR_ARG bit of device_error()."""
-        k, v = self._rows(k, "k"), self._rows(v, "v")
-        T = k.shape[1]
-        _require(v.shape[1] == T, "k and v must hold the same number of tokens")
-        _require(pos.dtype == torch.int64 and pos.device == self.device and pos.numel() == self.n_seqs and pos.is_contiguous(),
-                 f"pos must be a contiguous int64 [{self.n_seqs}] tensor on {self.device}")
-        arr = ctypes.c_int64 * 3
+        k, T, ks = self._rows(k, "k")
+        v, Tv, vs = self._rows(v, "v")
+        _require(Tv == T, "k and v must hold the same number of tokens")
+        if pos.dtype != torch.int64 or pos.device != self.device or pos.numel() != self.n_seqs or not pos.is_contiguous():
+            _require(False, f"pos must be a contiguous int64 [{self.n_seqs}] tensor on {self.device}")
         with _on_device(self.device):
-            st = _lib.lib().rb_kv_write(self._ref, k.data_ptr(), v.data_ptr(), arr(*k.stride()[:3]), arr(*v.stride()[:3]), T,
-                                        pos.data_ptr(), config.flags(), _lib.stream_ptr(self.device))
+            st = _lib.lib().rb_kv_write(self._ref, k.data_ptr(), v.data_ptr(), ks, vs, T, pos.data_ptr(), config.flags(),
+                                        _lib.stream_ptr(self.device))
         _lib.check("rb_kv_write", st)
 
     def read(self, start, count, out=None):
         """(k, v) of the slots start .. start + count - 1, [n_seqs, n_kv_heads, count, head_dim] in the cache's dtype."""
-        _require(0 <= start and 0 <= count and start + count <= self.cache_len,
-                 f"slots {start} .. {start + count - 1} are not in a cache of {self.cache_len}")
+        if not (0 <= start and 0 <= count and start + count <= self.cache_len):
+            _require(False, f"slots {start} .. {start + count - 1} are not in a cache of {self.cache_len}")
         shape = (self.n_seqs, self.n_kv_heads, count, self.head_dim)
         if out is None:
-            out = tuple(torch.empty(shape, dtype=self.dtype, device=self.device) for _ in range(2))
-        for t in out:
-            _require(t.shape == shape and t.dtype == self.dtype and t.device == self.device and t.is_contiguous(),
-                     f"out must hold two contiguous {self.dtype} {shape} tensors on {self.device}")
+            both = torch.empty((2,) + shape, dtype=self.dtype, device=self.device)
+            out = (both[0], both[1])
+        else:
+            for t in out:
+                _require(t.shape == shape and t.dtype == self.dtype and t.device == self.device and t.is_contiguous(),
+                         f"out must hold two contiguous {self.dtype} {shape} tensors on {self.device}")
         with _on_device(self.device):
             st = _lib.lib().rb_kv_read(self._ref, out[0].data_ptr(), out[1].data_ptr(), start, count, config.flags(),
                                        _lib.stream_ptr(self.device))

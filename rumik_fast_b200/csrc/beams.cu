@@ -223,12 +223,14 @@ __global__ void __launch_bounds__(kThreads) beam_select_kernel(const __grid_cons
   float2 ms = make_float2(-INFINITY, 0.f);
   bool odd = false;
   if (!done && !dead) {
-    // every warp merges the chunks' sums, lane l those of chunks l, l + 32, ...: the same sum everywhere
+    // every warp merges the chunks' sums, lane l those of chunks l, l + 32, ...
 #pragma unroll 1
     for (int c = lane; c < p.chunks; c += 32) ms = merge_sums(ms, __ldcg(p.part + static_cast<int64_t>(row) * p.chunks + c));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
       ms = merge_sums(ms, make_float2(__shfl_xor_sync(0xffffffffu, ms.x, o), __shfl_xor_sync(0xffffffffu, ms.y, o)));
+    // lane 0's: the lanes add in different orders, and which thread writes which candidate is not fixed
+    ms = make_float2(__shfl_sync(0xffffffffu, ms.x, 0), __shfl_sync(0xffffffffu, ms.y, 0));
     odd = ms.x == INFINITY;
     if (odd && tid == 0) atomicOr(&g_device_error, static_cast<unsigned>(ERR_ARG));
   }

@@ -32,7 +32,7 @@ struct WriteParams {
   Rows r[2];
   const int64_t* pos;
   int64_t n_seqs, n_tokens, cache_len, tiles;  // tiles: CTAs of one (key or value, sequence)
-  int n_heads, bf16, by_head;
+  int n_heads, by_head;
 };
 
 struct ReadParams {
@@ -43,38 +43,59 @@ struct ReadParams {
   int n_heads, bf16;
 };
 
-// Largest value of the group of kLanes lanes that share a row.
-template <int kLanes>
-__device__ __forceinline__ float group_max(float v) {
-#pragma unroll
-  for (int o = kLanes / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
-template <int kLanes>
-__device__ __forceinline__ bool group_any(bool b) {
-  const unsigned m = __ballot_sync(0xffffffffu, b);
-  const int first = (threadIdx.x & 31) / kLanes * kLanes;
-  return (m >> first) & (kLanes == 32 ? 0xffffffffu : (1u << kLanes) - 1u);
-}
-
 __device__ __forceinline__ float bf16_round(float v) { return __bfloat162float(__float2bfloat16_rn(v)); }
 
-// rint(x / s) clamped to [lo, hi] for a thread's eight values; s > 0.
-__device__ __forceinline__ void quantise8(const float (&x)[8], float s, float lo, float hi, float (&q)[8]) {
+// The row's result in every one of the kLanes lanes that share it.
+template <int kLanes, typename Op>
+__device__ __forceinline__ uint32_t row_all(uint32_t v, Op op) {
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// Largest and smallest of a thread's eight values as the 16-bit types order them, NaN winning.
+template <bool kBf16, bool kMax>
+__device__ __forceinline__ uint32_t pick2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  if constexpr (kBf16) {
+    if constexpr (kMax) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    else asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  } else {
+    if constexpr (kMax) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    else asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  }
+  return d;
+}
+
+__device__ __forceinline__ float act_of(uint32_t bits16, bool bf16) {
+  return bf16 ? __uint_as_float(bits16 << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(bits16)));
+}
+
+constexpr float kRint = 12582912.f;  // 1.5 2^23: a sum with it is rounded to an integer, held in its low bits
+
+// rint(x / s) of a thread's eight values, clamped to [lo, hi], as integers in the low byte; s > 0. Rounding by the sum
+// with kRint and keeping the integer bits takes no conversion instruction (they run at a quarter of the rate).
+__device__ __forceinline__ void quantise8(const float (&x)[8], float s, int lo, int hi, uint32_t (&q)[8]) {
   const float inv = __frcp_rn(s);
-  bool near = false;
+  float off = 0.f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float t = x[e] * inv;  // within 2^-22 of x / s (and at most 128 of them here): 1e-4 decides
-    q[e] = rintf(t);
-    near |= !(fabsf(t - q[e]) <= 0.4999f);  // also where the reciprocal overflowed
+    const float t = x[e] * inv, r = t + kRint;  // t: within 2^-22 of x / s, relatively, and at most 128: 1e-4 decides
+    off = fmaxf(off, fabsf(t - (r - kRint)));
+    q[e] = __float_as_uint(r);
   }
-  if (near) {
+  // near a tie, or a scale so small that it is not a full bf16 or has no reciprocal: divide and clamp. Elsewhere
+  // |x| <= 127.25 s (15.03 s), so that no code is out of range.
+  if (!(off <= 0.4999f) || s < 1e-36f) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) q[e] = rintf(__fdiv_rn(x[e], s));
+    for (int e = 0; e < 8; ++e)
+      q[e] = static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(rintf(__fdiv_rn(x[e], s)), static_cast<float>(lo)), static_cast<float>(hi))));
   }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) q[e] = fminf(fmaxf(q[e], lo), hi);
+}
+
+// The low bytes of four words.
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
 // kLanes lanes hold a row, 8 values each (one 16-byte load). A CTA takes kGroups x kRows rows of one (key or value,
@@ -82,7 +103,7 @@ __device__ __forceinline__ void quantise8(const float (&x)[8], float s, float lo
 // fewer tokens than kGroups (a decode step), rows in (token, head) order. All of a thread's loads go out first.
 constexpr int kRows = 4;
 
-template <int kHd, int kFmt>
+template <int kHd, int kFmt, bool kBf16>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constant__ WriteParams p) {
   constexpr int kLanes = kHd / 8, kGroups = kThreads / kLanes, kTile = kGroups * kRows;
   __shared__ uint32_t par[kTile];
@@ -124,42 +145,42 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constan
     if constexpr (kFmt == RB_KV_PLAIN) {
       if (dst[i] >= 0) reinterpret_cast<uint4*>(R.c)[dst[i] * kLanes + sub] = raw[i];
     } else {
-      float x[8], q[8];
-      raw_to_f32(raw[i], p.bf16 != 0, x);
-      float hi = x[0], lo = -x[0];
-      bool odd = false;  // NaN or infinity
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        hi = fmaxf(hi, x[e]);
-        lo = fmaxf(lo, -x[e]);
-        odd |= !(fabsf(x[e]) <= 3.402823466e38f);
-      }
-      float m = 0.f, s;
+      const uint32_t r4[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+      float x[8], m = 0.f, s;
+      raw_to_f32(raw[i], kBf16, x);
+      uint32_t word = 0u;
       if constexpr (kFmt == RB_KV_INT8) {
-        s = bf16_round(__fdiv_rn(group_max<kLanes>(fmaxf(hi, lo)), 127.f));
+        // the order of the magnitudes' bits is the order of the magnitudes, with infinity and NaN above the others
+        uint32_t top = 0u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = __vmaxu2(top, r4[e] & 0x7fff7fffu);
+        top = row_all<kLanes>(max(top & 0xffffu, top >> 16), [](uint32_t a, uint32_t c) { return max(a, c); });
+        s = bf16_round(__fdiv_rn(act_of(top, kBf16), 127.f));
+        if (top >= (kBf16 ? 0x7f80u : 0x7c00u)) s = __int_as_float(0x7fc00000);
       } else {
-        hi = group_max<kLanes>(hi);
-        m = -group_max<kLanes>(lo);
-        const float range = hi - m;
-        odd |= !(range <= 3.402823466e38f);
-        s = bf16_round(__fdiv_rn(range, 15.f));
+        uint32_t hi2 = r4[0], lo2 = r4[0];
+#pragma unroll
+        for (int e = 1; e < 4; ++e) hi2 = pick2<kBf16, true>(hi2, r4[e]), lo2 = pick2<kBf16, false>(lo2, r4[e]);
+        hi2 = row_all<kLanes>(hi2, [](uint32_t a, uint32_t c) { return pick2<kBf16, true>(a, c); });
+        lo2 = row_all<kLanes>(lo2, [](uint32_t a, uint32_t c) { return pick2<kBf16, false>(a, c); });
+        const uint32_t lo = pick2<kBf16, false>(lo2, lo2 >> 16) & 0xffffu;
+        m = act_of(lo, kBf16);
+        const float range = act_of(pick2<kBf16, true>(hi2, hi2 >> 16) & 0xffffu, kBf16) - m;
+        s = range <= 3.402823466e38f ? bf16_round(__fdiv_rn(range, 15.f)) : __int_as_float(0x7fc00000);
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] -= m;
+        word = lo << 16;
       }
-      if (group_any<kLanes>(odd)) s = __int_as_float(0x7fc00000);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) q[e] = 0.f;
-      if (s > 0.f) quantise8(x, s, kFmt == RB_KV_INT8 ? -127.f : 0.f, kFmt == RB_KV_INT8 ? 127.f : 15.f, q);
-      uint32_t w[2] = {0u, 0u}, word = __bfloat16_as_ushort(__float2bfloat16_rn(s));
-      if constexpr (kFmt == RB_KV_INT8) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e >> 2] |= static_cast<uint32_t>(static_cast<int>(q[e]) + 128) << (8 * (e & 3));
-        if (dst[i] >= 0) reinterpret_cast<uint2*>(R.c)[dst[i] * kLanes + sub] = make_uint2(w[0], w[1]);
+      word |= __bfloat16_as_ushort(__float2bfloat16_rn(s));
+      uint32_t q[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+      if (s > 0.f) quantise8(x, s, kFmt == RB_KV_INT8 ? -127 : 0, kFmt == RB_KV_INT8 ? 127 : 15, q);
+      if constexpr (kFmt == RB_KV_INT8) {  // + 128 of a signed byte: its top bit turned over
+        if (dst[i] >= 0)
+          reinterpret_cast<uint2*>(R.c)[dst[i] * kLanes + sub] =
+              make_uint2(low_bytes(q[0], q[1], q[2], q[3]) ^ 0x80808080u, low_bytes(q[4], q[5], q[6], q[7]) ^ 0x80808080u);
       } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[0] |= static_cast<uint32_t>(static_cast<int>(q[e])) << (4 * e);
-        if (dst[i] >= 0) reinterpret_cast<uint32_t*>(R.c)[dst[i] * kLanes + sub] = w[0];
-        word |= static_cast<uint32_t>(p.bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(m)) : __half_as_ushort(__float2half_rn(m))) << 16;
+        const uint32_t even = low_bytes(q[0], q[2], q[4], q[6]), odd = low_bytes(q[1], q[3], q[5], q[7]);
+        if (dst[i] >= 0) reinterpret_cast<uint32_t*>(R.c)[dst[i] * kLanes + sub] = even | (odd << 4);
       }
       if (p.by_head) {
         if (sub == 0) par[i * kGroups + grp] = word;
@@ -241,11 +262,12 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant
       const float s = __uint_as_float(word[i] << 16);
       if constexpr (kFmt == RB_KV_INT8) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(static_cast<int>(((e < 4 ? raw[i].x : raw[i].y) >> (8 * (e & 3))) & 255u) - 128) * s;
+        for (int e = 0; e < 8; ++e)  // byte e under 2^23's exponent, less 2^23 + 128
+          v[e] = (__uint_as_float(__byte_perm(e < 4 ? raw[i].x : raw[i].y, 0x4B000000u, 0x7440 + (e & 3))) - 8388736.f) * s;
       } else {
         const float m = p.bf16 ? __uint_as_float(word[i] & 0xffff0000u) : __half2float(__ushort_as_half(static_cast<unsigned short>(word[i] >> 16)));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = fmaf(static_cast<float>((raw[i].x >> (4 * e)) & 15u), s, m);
+        for (int e = 0; e < 8; ++e) v[e] = fmaf(__uint_as_float(((raw[i].x >> (4 * e)) & 15u) | 0x4B000000u) - 8388608.f, s, m);
       }
       out[u] = make_uint4(pack_act2(v[0], v[1], p.bf16), pack_act2(v[2], v[3], p.bf16), pack_act2(v[4], v[5], p.bf16),
                           pack_act2(v[6], v[7], p.bf16));
@@ -281,18 +303,20 @@ int launch_kv_write(const rb_kv_cache* c, const void* k, const void* v, const in
   p.n_tokens = n_tokens;
   p.cache_len = c->cache_len;
   p.n_heads = c->n_kv_heads;
-  p.bf16 = c->dtype == RB_BF16;
   const int64_t groups = kThreads / (c->head_dim / 8), tile = groups * kRows;
   p.by_head = n_tokens >= groups;
   p.tiles = p.by_head ? (n_tokens + tile - 1) / tile * c->n_kv_heads : (n_tokens * c->n_kv_heads + tile - 1) / tile;
   const int64_t blocks = 2 * c->n_seqs * p.tiles;
-  void (*kern)(WriteParams) = nullptr;
-  if (c->head_dim == 128)
-    kern = c->fmt == RB_KV_INT8 ? kv_write_kernel<128, RB_KV_INT8>
-                                : (c->fmt == RB_KV_INT4 ? kv_write_kernel<128, RB_KV_INT4> : kv_write_kernel<128, RB_KV_PLAIN>);
+  const bool bf = c->dtype == RB_BF16, wide = c->head_dim == 128;
+  void (*kern)(WriteParams);
+  if (c->fmt == RB_KV_PLAIN)
+    kern = wide ? kv_write_kernel<128, RB_KV_PLAIN, false> : kv_write_kernel<64, RB_KV_PLAIN, false>;
+  else if (c->fmt == RB_KV_INT8)
+    kern = wide ? (bf ? kv_write_kernel<128, RB_KV_INT8, true> : kv_write_kernel<128, RB_KV_INT8, false>)
+                : (bf ? kv_write_kernel<64, RB_KV_INT8, true> : kv_write_kernel<64, RB_KV_INT8, false>);
   else
-    kern = c->fmt == RB_KV_INT8 ? kv_write_kernel<64, RB_KV_INT8>
-                                : (c->fmt == RB_KV_INT4 ? kv_write_kernel<64, RB_KV_INT4> : kv_write_kernel<64, RB_KV_PLAIN>);
+    kern = wide ? (bf ? kv_write_kernel<128, RB_KV_INT4, true> : kv_write_kernel<128, RB_KV_INT4, false>)
+                : (bf ? kv_write_kernel<64, RB_KV_INT4, true> : kv_write_kernel<64, RB_KV_INT4, false>);
   return launch(kern, p, blocks, flags, stream);
 }
 

@@ -60,22 +60,24 @@ __device__ __forceinline__ uint32_t key_row(Key key) { return 0xffffffffu - stat
 struct Shared {
   Key cand[kCap];
   Key top[kThreads];
-  Key bound[kThreads / 32];
+  Key bound[kThreads / 32], each[kThreads / 32];
   float2 red[kThreads / 32];
   int n;
   int last;
 };
 
 // A bound that at least k of the CTA's keys reach. `best` is this thread's largest key (0: none). kWide: the k-th
-// largest of all threads' own (at most k threads hold a key that reaches it); else the largest, over the warps, of the
-// k-th largest of a warp's (at most k lanes of each warp do): an eighth of the comparisons.
+// largest of all threads' own (at most k threads hold a key that reaches it); else, from the ranks within the warps (an
+// eighth of the comparisons), the larger of two such bounds: the largest over the warps of a warp's k-th (at most k
+// lanes of each warp reach it), and the smallest over the warps of a warp's ceil(k / 8)-th (8 ceil(k / 8) keys do), which
+// is the closer one on ordinary logits - about 2 k keys pass it.
 template <bool kWide>
 __device__ __forceinline__ Key cta_bound(Shared& sh, int k, Key best) {
   constexpr int kN = kWide ? kThreads : 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   sh.top[threadIdx.x] = best;
   if (threadIdx.x == 0) sh.n = 0;
-  if (lane == 0) sh.bound[warp] = 1;
+  if (lane == 0) sh.bound[warp] = 1, sh.each[warp] = 0;
   if (kWide) __syncthreads();
   else __syncwarp();
   int rank = 0;
@@ -87,11 +89,15 @@ __device__ __forceinline__ Key cta_bound(Shared& sh, int k, Key best) {
     rank += v.y > best;
   }
   if (rank == k - 1 && best != 0) sh.bound[warp] = best;  // keys differ: one thread has this rank
+  if (!kWide && rank == (k + kThreads / 32 - 1) / (kThreads / 32) - 1) sh.each[warp] = best;
   __syncthreads();
-  Key lim = 1;
+  Key lim = 1, least = ~Key(0);
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) lim = sh.bound[w] > lim ? sh.bound[w] : lim;
-  return lim;
+  for (int w = 0; w < kThreads / 32; ++w) {
+    lim = sh.bound[w] > lim ? sh.bound[w] : lim;
+    least = sh.each[w] < least ? sh.each[w] : least;
+  }
+  return !kWide && least > lim ? least : lim;
 }
 
 // The k largest of the keys in sh.cand, best first, through out(rank, key); ranks without a key get 0.
@@ -114,18 +120,25 @@ __device__ __forceinline__ void cta_rank(Shared& sh, int k, Out out) {
 // The k largest of n keys get(0) .. get(n - 1) (0: none).
 template <typename Get, typename Out>
 __device__ __forceinline__ void cta_top(Shared& sh, int k, int n, Get get, Out out) {
-  Key best = 0;
-#pragma unroll 1
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const Key v = get(i);
-    best = v > best ? v : best;
-  }
-  const Key lim = cta_bound<true>(sh, k, best);
-  if (best >= lim) {
+  if (n <= kThreads) {  // a key a thread: all of them are ranked
+    if (threadIdx.x == 0) sh.n = 0;
+    __syncthreads();
+    const Key v = threadIdx.x < n ? get(threadIdx.x) : Key(0);
+    if (v) sh.cand[atomicAdd(&sh.n, 1)] = v;
+  } else {
+    Key best = 0;
 #pragma unroll 1
     for (int i = threadIdx.x; i < n; i += kThreads) {
       const Key v = get(i);
-      if (v >= lim) sh.cand[atomicAdd(&sh.n, 1)] = v;
+      best = v > best ? v : best;
+    }
+    const Key lim = n <= kPer * kThreads ? cta_bound<false>(sh, k, best) : cta_bound<true>(sh, k, best);
+    if (best >= lim) {
+#pragma unroll 1
+      for (int i = threadIdx.x; i < n; i += kThreads) {
+        const Key v = get(i);
+        if (v >= lim) sh.cand[atomicAdd(&sh.n, 1)] = v;
+      }
     }
   }
   cta_rank(sh, k, out);
@@ -146,7 +159,12 @@ __device__ __forceinline__ bool last_to_arrive(Shared& sh, unsigned int* ticket,
   return sh.last != 0;
 }
 
-__device__ __forceinline__ float exp_of(float x) { return exp2f(x * 1.4426950408889634f); }
+// exp(x), x <= 0: the hardware's 2^x (relative error 2^-22)
+__device__ __forceinline__ float exp_of(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+  return y;
+}
 
 // (maximum, sum of exponentials) of two parts; a maximum of +inf marks a part without a distribution.
 __device__ __forceinline__ float2 merge_sums(float2 a, float2 b) {
@@ -171,8 +189,13 @@ __global__ void __launch_bounds__(kThreads) beam_select_kernel(const __grid_cons
     const int first = chunk * kChunk + tid;
     const T* x = reinterpret_cast<const T*>(p.logits) + row * p.ld + first;
     float v[kPer];
+    if (chunk * kChunk + kChunk <= p.V) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) v[i] = first + i * kThreads < p.V ? static_cast<float>(x[i * kThreads]) + 0.f : -INFINITY;  // -0 -> +0
+      for (int i = 0; i < kPer; ++i) v[i] = static_cast<float>(x[i * kThreads]) + 0.f;  // -0 -> +0
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) v[i] = first + i * kThreads < p.V ? static_cast<float>(x[i * kThreads]) + 0.f : -INFINITY;
+    }
     if (early) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i)

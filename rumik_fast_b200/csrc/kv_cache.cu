@@ -31,16 +31,18 @@ struct Rows {  // one of k, v: the row source (or destination) and the cache sid
 struct WriteParams {
   Rows r[2];
   const int64_t* pos;
-  int64_t n_seqs, n_tokens, cache_len, tiles;  // tiles: CTAs of one (key or value, sequence)
-  int n_heads, by_head;
+  int64_t n_tokens, cache_len;
+  uint32_t n_seqs, n_heads, tiles;  // tiles: CTAs of one (key or value, sequence)
+  int by_head;
 };
 
 struct ReadParams {
   const void* c[2];
   const void* par[2];
   void* out[2];
-  int64_t n_seqs, start, count, cache_len, tiles;  // tiles: CTAs of one (key or value, sequence, head)
-  int n_heads, bf16;
+  int64_t start, count, cache_len;
+  uint32_t heads, tiles;  // sequences x heads; CTAs of one (key or value, sequence, head)
+  int bf16;
 };
 
 __device__ __forceinline__ float bf16_round(float v) { return __bfloat162float(__float2bfloat16_rn(v)); }
@@ -76,11 +78,12 @@ constexpr float kRint = 12582912.f;  // 1.5 2^23: a sum with it is rounded to an
 // rint(x / s) of a thread's eight values, clamped to [lo, hi], as integers in the low byte; s > 0. Rounding by the sum
 // with kRint and keeping the integer bits takes no conversion instruction (they run at a quarter of the rate).
 __device__ __forceinline__ void quantise8(const float (&x)[8], float s, int lo, int hi, uint32_t (&q)[8]) {
-  const float inv = __frcp_rn(s);
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
   float off = 0.f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float t = x[e] * inv, r = t + kRint;  // t: within 2^-22 of x / s, relatively, and at most 128: 1e-4 decides
+    const float t = x[e] * inv, r = t + kRint;  // t: within 2^-21 of x / s, relatively, and at most 128: 1e-4 decides
     off = fmaxf(off, fabsf(t - (r - kRint)));
     q[e] = __float_as_uint(r);
   }
@@ -110,36 +113,45 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constan
   griddep_wait();
   griddep_launch_dependents();
   const int sub = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
-  const int64_t which_seq = blockIdx.x / p.tiles;
-  const int64_t tile = blockIdx.x - which_seq * p.tiles;
-  const int64_t b = which_seq % p.n_seqs;
-  const Rows& R = p.r[which_seq >= p.n_seqs];
+  const uint32_t which_seq = blockIdx.x / p.tiles, tile = blockIdx.x - which_seq * p.tiles;
+  const bool second = which_seq >= p.n_seqs;
+  const int64_t b = second ? which_seq - p.n_seqs : which_seq;
+  const Rows& R = p.r[second];
   const int64_t at = __ldcg(p.pos + b);
   int64_t t0, limit;  // the tile's first token (by_head) or row, and the end
-  int h0 = 0;
+  uint32_t h0 = 0;
   if (p.by_head) {
-    h0 = static_cast<int>(tile % p.n_heads);
-    t0 = tile / p.n_heads * kTile;
+    const uint32_t tt = tile / p.n_heads;
+    h0 = tile - tt * p.n_heads;
+    t0 = static_cast<int64_t>(tt) * kTile;
     limit = p.n_tokens;
   } else {
-    t0 = tile * kTile;
+    t0 = static_cast<int64_t>(tile) * kTile;
     limit = p.n_tokens * p.n_heads;
   }
+  const uint16_t* src = reinterpret_cast<const uint16_t*>(R.x) + b * R.s_seq + sub * 8;
+  const int64_t row0 = b * p.n_heads * p.cache_len + at;  // token t of head h: row0 + h cache_len + t
   uint4 raw[kRows];
   int64_t dst[kRows];  // the row in the cache; -1: nothing to store
+  bool lost = false;
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
     const int64_t x = t0 + i * kGroups + grp;
     const bool in = x < limit;
-    const int64_t t = in ? (p.by_head ? x : x / p.n_heads) : 0;
-    const int h = p.by_head ? h0 : static_cast<int>(in ? x % p.n_heads : 0);
+    int64_t t = in ? x : 0;
+    uint32_t h = h0;
+    if (!p.by_head) {  // fewer than kGroups tokens: 32 bits hold a row's index
+      const uint32_t xr = static_cast<uint32_t>(t);
+      t = xr / p.n_heads;
+      h = xr - static_cast<uint32_t>(t) * p.n_heads;
+    }
     const bool fits = at >= -t && at < p.cache_len - t;  // 0 <= at + t < cache_len, without the sum (at may be any)
-    if (in && !fits && sub == 0) atomicOr(&g_device_error, static_cast<unsigned>(ERR_ARG));
-    dst[i] = in && fits ? (b * p.n_heads + h) * p.cache_len + at + t : -1;
+    lost |= in && !fits;
+    dst[i] = in && fits ? row0 + h * p.cache_len + t : -1;
     raw[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (dst[i] >= 0)
-      raw[i] = ldg_cg_128(reinterpret_cast<const uint16_t*>(R.x) + b * R.s_seq + t * R.s_tok + h * R.s_head + sub * 8);
+    if (dst[i] >= 0) raw[i] = ldg_cg_128(src + t * R.s_tok + h * R.s_head);
   }
+  if (lost && sub == 0) atomicOr(&g_device_error, static_cast<unsigned>(ERR_ARG));
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
     if constexpr (kFmt == RB_KV_PLAIN) {
@@ -155,7 +167,8 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constan
 #pragma unroll
         for (int e = 0; e < 4; ++e) top = __vmaxu2(top, r4[e] & 0x7fff7fffu);
         top = row_all<kLanes>(max(top & 0xffffu, top >> 16), [](uint32_t a, uint32_t c) { return max(a, c); });
-        s = bf16_round(__fdiv_rn(act_of(top, kBf16), 127.f));
+        // no 11-bit value is 127 times a 9-bit one: top / 127 is never near a tie of bf16, and the product rounds as it does
+        s = bf16_round(act_of(top, kBf16) * (1.f / 127.f));
         if (top >= (kBf16 ? 0x7f80u : 0x7c00u)) s = __int_as_float(0x7fc00000);
       } else {
         uint32_t hi2 = r4[0], lo2 = r4[0];
@@ -225,11 +238,10 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant
   constexpr int kLanes = kHd / 8;
   griddep_wait();
   griddep_launch_dependents();
-  const int64_t line = blockIdx.x / p.tiles;
-  const int64_t u0 = (blockIdx.x - line * p.tiles) * (kThreads * kUnits) + threadIdx.x, units = p.count * kLanes;
-  const int64_t heads = p.n_seqs * p.n_heads;
-  const int which = line >= heads;
-  const int64_t bh = which ? line - heads : line, src = bh * p.cache_len + p.start;
+  const uint32_t line = blockIdx.x / p.tiles;
+  const int64_t u0 = static_cast<int64_t>(blockIdx.x - line * p.tiles) * (kThreads * kUnits) + threadIdx.x, units = p.count * kLanes;
+  const int which = line >= p.heads;
+  const int64_t bh = which ? line - p.heads : line, src = bh * p.cache_len + p.start;
   uint4* out = reinterpret_cast<uint4*>(p.out[which]) + bh * units;
   uint4 raw[kUnits];
   uint32_t word[kUnits];
@@ -277,7 +289,6 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant
 
 template <typename P>
 int launch(void (*kern)(P), const P& p, int64_t blocks, int flags, cudaStream_t stream) {
-  if (blocks > (int64_t(1) << 31) - 1) return RB_ERR_SHAPE;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks));
   cfg.blockDim = dim3(kThreads);
@@ -299,14 +310,16 @@ int launch_kv_write(const rb_kv_cache* c, const void* k, const void* v, const in
   p.r[0] = {k, ks[0], ks[1], ks[2], c->k, c->k_par};
   p.r[1] = {v, vs[0], vs[1], vs[2], c->v, c->v_par};
   p.pos = pos;
-  p.n_seqs = c->n_seqs;
   p.n_tokens = n_tokens;
   p.cache_len = c->cache_len;
-  p.n_heads = c->n_kv_heads;
+  p.n_heads = static_cast<uint32_t>(c->n_kv_heads);
+  p.n_seqs = static_cast<uint32_t>(c->n_seqs);
   const int64_t groups = kThreads / (c->head_dim / 8), tile = groups * kRows;
   p.by_head = n_tokens >= groups;
-  p.tiles = p.by_head ? (n_tokens + tile - 1) / tile * c->n_kv_heads : (n_tokens * c->n_kv_heads + tile - 1) / tile;
-  const int64_t blocks = 2 * c->n_seqs * p.tiles;
+  const int64_t tiles = p.by_head ? (n_tokens + tile - 1) / tile * c->n_kv_heads : (n_tokens * c->n_kv_heads + tile - 1) / tile;
+  const int64_t blocks = 2 * c->n_seqs * tiles;
+  if (blocks > (int64_t(1) << 31) - 1) return RB_ERR_SHAPE;
+  p.tiles = static_cast<uint32_t>(tiles);
   const bool bf = c->dtype == RB_BF16, wide = c->head_dim == 128;
   void (*kern)(WriteParams);
   if (c->fmt == RB_KV_PLAIN)
@@ -330,14 +343,15 @@ int launch_kv_read(const rb_kv_cache* c, void* k_out, void* v_out, int64_t start
   p.par[1] = c->v_par;
   p.out[0] = k_out;
   p.out[1] = v_out;
-  p.n_seqs = c->n_seqs;
   p.start = start;
   p.count = count;
   p.cache_len = c->cache_len;
-  p.n_heads = c->n_kv_heads;
+  p.heads = static_cast<uint32_t>(c->n_seqs * c->n_kv_heads);
   p.bf16 = c->dtype == RB_BF16;
-  p.tiles = (count * (c->head_dim / 8) + kThreads * kUnits - 1) / (kThreads * kUnits);
-  const int64_t blocks = 2 * c->n_seqs * c->n_kv_heads * p.tiles;
+  const int64_t tiles = (count * (c->head_dim / 8) + kThreads * kUnits - 1) / (kThreads * kUnits);
+  const int64_t blocks = 2 * c->n_seqs * c->n_kv_heads * tiles;
+  if (blocks > (int64_t(1) << 31) - 1) return RB_ERR_SHAPE;
+  p.tiles = static_cast<uint32_t>(tiles);
   void (*kern)(ReadParams) = nullptr;
   if (c->head_dim == 128)
     kern = c->fmt == RB_KV_INT8 ? kv_read_kernel<128, RB_KV_INT8>

@@ -8,8 +8,7 @@
 // The scale is rounded to bf16 BEFORE the codes are computed against it, so its 8 bits cost nothing (127 s and 15 s
 // stay within half a step of the largest value) and it keeps fp32's range, which an fp16 scale would not. x (11 bits)
 // over s (8 bits) is either exactly a half-integer or at least 2^-16 of itself away from one, so the codes do not
-// depend on how wide the quotient is computed; away from ties x times the reciprocal of s gives the same code, and a
-// thread divides only where one of its eight is near one.
+// depend on how wide the quotient is computed.
 // A row with a NaN or an infinity gets s = NaN and codes of zero: all of it reads back as NaN, in this kernel and in
 // the attention. s == 0 (a row of equal values, or of zeros) gives codes of zero.
 #include "common.cuh"
@@ -73,26 +72,53 @@ __device__ __forceinline__ float act_of(uint32_t bits16, bool bf16) {
   return bf16 ? __uint_as_float(bits16 << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(bits16)));
 }
 
+// Two fp32 operations in one instruction (sm_100a): a b + c on both halves.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)),
+        "l"(*reinterpret_cast<unsigned long long*>(&c)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+
+// The 16-bit pair as fp32.
+template <bool kBf16>
+__device__ __forceinline__ float2 pair_of(uint32_t w) {
+  if constexpr (kBf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
 constexpr float kRint = 12582912.f;  // 1.5 2^23: a sum with it is rounded to an integer, held in its low bits
 
-// rint(x / s) of a thread's eight values, clamped to [lo, hi], as integers in the low byte; s > 0. Rounding by the sum
-// with kRint and keeping the integer bits takes no conversion instruction (they run at a quarter of the rate).
-__device__ __forceinline__ void quantise8(const float (&x)[8], float s, int lo, int hi, uint32_t (&q)[8]) {
+// rint(x / s) of a thread's eight values, clamped to [lo, hi], as integers in the low byte; s > 0. The quotient is the
+// product with the reciprocal, corrected once by its exact remainder x - t s (Markstein's method, IBM J. Res. Dev. 34,
+// 1990): it is x / s rounded to fp32, so that exact half-integers, 0.3 % of 16-bit values, go to the even code. Rounding
+// by the sum with kRint and keeping the integer bits takes no conversion instruction (a quarter of the rate).
+__device__ __forceinline__ void quantise8(const float2 (&x)[4], float s, float lo, float hi, uint32_t (&q)[8]) {
   float inv;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
-  float off = 0.f;
+  const float2 inv2 = make_float2(inv, inv), s2 = make_float2(-s, -s), c2 = make_float2(kRint, kRint);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float t = x[e] * inv, r = t + kRint;  // t: within 2^-21 of x / s, relatively, and at most 128: 1e-4 decides
-    off = fmaxf(off, fabsf(t - (r - kRint)));
-    q[e] = __float_as_uint(r);
+  for (int e = 0; e < 4; ++e) {
+    const float2 t = fma2(x[e], inv2, make_float2(0.f, 0.f));
+    const float2 r = add2(fma2(fma2(t, s2, x[e]), inv2, t), c2);
+    q[2 * e] = __float_as_uint(r.x);
+    q[2 * e + 1] = __float_as_uint(r.y);
   }
-  // near a tie, or a scale so small that it is not a full bf16 or has no reciprocal: divide and clamp. Elsewhere
+  // a scale so small that the remainder or the scale itself is not a normal number: divide and clamp. Above it
   // |x| <= 127.25 s (15.03 s), so that no code is out of range.
-  if (!(off <= 0.4999f) || s < 1e-36f) {
+  if (s < 1e-28f) {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      q[e] = static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(rintf(__fdiv_rn(x[e], s)), static_cast<float>(lo)), static_cast<float>(hi))));
+      q[e] = static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(rintf(__fdiv_rn((e & 1) ? x[e >> 1].y : x[e >> 1].x, s)), lo), hi)));
   }
 }
 
@@ -101,15 +127,65 @@ __device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-// kLanes lanes hold a row, 8 values each (one 16-byte load). A CTA takes kGroups x kRows rows of one (key or value,
-// sequence): consecutive tokens of one head, whose parameters then leave as one contiguous store, or, when there are
-// fewer tokens than kGroups (a decode step), rows in (token, head) order. All of a thread's loads go out first.
+// A row of kLanes lanes, eight values (16 bytes) each: its codes to `c` (this lane's) and, from lane 0, its parameters'
+// word through `out`.
+template <int kLanes, int kFmt, bool kBf16, typename Out>
+__device__ __forceinline__ void quantise_row(const uint4 raw, bool store, void* c, Out out) {
+  if constexpr (kFmt == RB_KV_PLAIN) {
+    if (store) *reinterpret_cast<uint4*>(c) = raw;
+  } else {
+    const uint32_t r4[4] = {raw.x, raw.y, raw.z, raw.w};
+    float2 x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = pair_of<kBf16>(r4[e]);
+    float s;
+    uint32_t word = 0u;
+    if constexpr (kFmt == RB_KV_INT8) {
+      // the order of the magnitudes' bits is the order of the magnitudes, with infinity and NaN above the others
+      uint32_t top = __vmaxu2(__vmaxu2(r4[0] & 0x7fff7fffu, r4[1] & 0x7fff7fffu), __vmaxu2(r4[2] & 0x7fff7fffu, r4[3] & 0x7fff7fffu));
+      top = row_all<kLanes>(max(top & 0xffffu, top >> 16), [](uint32_t a, uint32_t d) { return max(a, d); });
+      // no 11-bit value is 127 times a 9-bit one: top / 127 is never near a tie of bf16, and the product rounds as it does
+      s = bf16_round(act_of(top, kBf16) * (1.f / 127.f));
+      if (top >= (kBf16 ? 0x7f80u : 0x7c00u)) s = __int_as_float(0x7fc00000);
+    } else {
+      uint32_t hi2 = r4[0], lo2 = r4[0];
+#pragma unroll
+      for (int e = 1; e < 4; ++e) hi2 = pick2<kBf16, true>(hi2, r4[e]), lo2 = pick2<kBf16, false>(lo2, r4[e]);
+      hi2 = row_all<kLanes>(hi2, [](uint32_t a, uint32_t d) { return pick2<kBf16, true>(a, d); });
+      lo2 = row_all<kLanes>(lo2, [](uint32_t a, uint32_t d) { return pick2<kBf16, false>(a, d); });
+      const uint32_t lo = pick2<kBf16, false>(lo2, lo2 >> 16) & 0xffffu;
+      const float m = act_of(lo, kBf16), range = act_of(pick2<kBf16, true>(hi2, hi2 >> 16) & 0xffffu, kBf16) - m;
+      s = range <= 3.402823466e38f ? bf16_round(__fdiv_rn(range, 15.f)) : __int_as_float(0x7fc00000);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = add2(x[e], make_float2(-m, -m));
+      word = lo << 16;
+    }
+    word |= __bfloat16_as_ushort(__float2bfloat16_rn(s));
+    uint32_t q[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+    if (s > 0.f) quantise8(x, s, kFmt == RB_KV_INT8 ? -127.f : 0.f, kFmt == RB_KV_INT8 ? 127.f : 15.f, q);
+    if constexpr (kFmt == RB_KV_INT8) {  // + 128 of a signed byte: its top bit turned over
+      if (store)
+        *reinterpret_cast<uint2*>(c) =
+            make_uint2(low_bytes(q[0], q[1], q[2], q[3]) ^ 0x80808080u, low_bytes(q[4], q[5], q[6], q[7]) ^ 0x80808080u);
+    } else {
+      const uint32_t even = low_bytes(q[0], q[2], q[4], q[6]), odd = low_bytes(q[1], q[3], q[5], q[7]);
+      if (store) *reinterpret_cast<uint32_t*>(c) = even | (odd << 4);
+    }
+    out(word);
+  }
+}
+
+// A CTA takes kGroups x kRows rows of one (key or value, sequence); all of a thread's loads go out first. kByHead:
+// consecutive tokens of one head - addresses a constant apart, the parameters one contiguous store. Otherwise (fewer
+// than kGroups tokens, a decode step) rows in (token, head) order.
 constexpr int kRows = 4;
 
-template <int kHd, int kFmt, bool kBf16>
+template <int kHd, int kFmt, bool kBf16, bool kByHead>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constant__ WriteParams p) {
   constexpr int kLanes = kHd / 8, kGroups = kThreads / kLanes, kTile = kGroups * kRows;
-  __shared__ uint32_t par[kTile];
+  constexpr int kRowBytes = kFmt == RB_KV_PLAIN ? 2 * kHd : (kFmt == RB_KV_INT8 ? kHd : kHd / 2);
+  constexpr int kParBytes = kFmt == RB_KV_INT8 ? 2 : 4;
+  __shared__ uint32_t par[kByHead ? kTile : 1];
   griddep_wait();
   griddep_launch_dependents();
   const int sub = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
@@ -118,100 +194,67 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constan
   const int64_t b = second ? which_seq - p.n_seqs : which_seq;
   const Rows& R = p.r[second];
   const int64_t at = __ldcg(p.pos + b);
-  int64_t t0, limit;  // the tile's first token (by_head) or row, and the end
-  uint32_t h0 = 0;
-  if (p.by_head) {
-    const uint32_t tt = tile / p.n_heads;
-    h0 = tile - tt * p.n_heads;
-    t0 = static_cast<int64_t>(tt) * kTile;
-    limit = p.n_tokens;
-  } else {
-    t0 = static_cast<int64_t>(tile) * kTile;
-    limit = p.n_tokens * p.n_heads;
-  }
+  // the tokens with a slot: 0 <= at + t < cache_len (at may be any value: no sum of it is formed before it is known)
+  const int64_t t_lo = at >= 0 ? 0 : (at < -p.n_tokens ? p.n_tokens : -at);
+  const int64_t t_end = at >= p.cache_len ? 0 : min(p.n_tokens, at < 0 ? p.cache_len + t_lo : p.cache_len - at);
+  if (tile == 0 && threadIdx.x == 0 && (t_lo > 0 || t_end < p.n_tokens)) atomicOr(&g_device_error, static_cast<unsigned>(ERR_ARG));
   const uint16_t* src = reinterpret_cast<const uint16_t*>(R.x) + b * R.s_seq + sub * 8;
-  const int64_t row0 = b * p.n_heads * p.cache_len + at;  // token t of head h: row0 + h cache_len + t
+  uint8_t* codes = static_cast<uint8_t*>(R.c) + sub * (kRowBytes / kLanes);
   uint4 raw[kRows];
-  int64_t dst[kRows];  // the row in the cache; -1: nothing to store
-  bool lost = false;
+  if constexpr (kByHead) {
+    const uint32_t tt = tile / p.n_heads, h = tile - tt * p.n_heads;
+    const int64_t t0 = static_cast<int64_t>(tt) * kTile;
+    // relative to the tile: rows [lo, hi) have a slot
+    const int lo = static_cast<int>(min(max(t_lo - t0, int64_t(0)), int64_t(kTile)));
+    const int hi = static_cast<int>(min(max(t_end - t0, int64_t(0)), int64_t(kTile)));
+    if (lo >= hi) return;
+    const int64_t row = (b * p.n_heads + h) * p.cache_len + at + t0;  // of the tile's first token; used from `lo` on
+    src += h * R.s_head + (t0 + grp) * R.s_tok;
+    codes += (row + grp) * kRowBytes;
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    const int64_t x = t0 + i * kGroups + grp;
-    const bool in = x < limit;
-    int64_t t = in ? x : 0;
-    uint32_t h = h0;
-    if (!p.by_head) {  // fewer than kGroups tokens: 32 bits hold a row's index
-      const uint32_t xr = static_cast<uint32_t>(t);
-      t = xr / p.n_heads;
-      h = xr - static_cast<uint32_t>(t) * p.n_heads;
+    for (int i = 0; i < kRows; ++i) {
+      const int x = i * kGroups + grp;
+      raw[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (x >= lo && x < hi) raw[i] = ldg_cg_128(src + i * kGroups * R.s_tok);
     }
-    const bool fits = at >= -t && at < p.cache_len - t;  // 0 <= at + t < cache_len, without the sum (at may be any)
-    lost |= in && !fits;
-    dst[i] = in && fits ? row0 + h * p.cache_len + t : -1;
-    raw[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (dst[i] >= 0) raw[i] = ldg_cg_128(src + t * R.s_tok + h * R.s_head);
-  }
-  if (lost && sub == 0) atomicOr(&g_device_error, static_cast<unsigned>(ERR_ARG));
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    if constexpr (kFmt == RB_KV_PLAIN) {
-      if (dst[i] >= 0) reinterpret_cast<uint4*>(R.c)[dst[i] * kLanes + sub] = raw[i];
-    } else {
-      const uint32_t r4[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-      float x[8], m = 0.f, s;
-      raw_to_f32(raw[i], kBf16, x);
-      uint32_t word = 0u;
-      if constexpr (kFmt == RB_KV_INT8) {
-        // the order of the magnitudes' bits is the order of the magnitudes, with infinity and NaN above the others
-        uint32_t top = 0u;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) top = __vmaxu2(top, r4[e] & 0x7fff7fffu);
-        top = row_all<kLanes>(max(top & 0xffffu, top >> 16), [](uint32_t a, uint32_t c) { return max(a, c); });
-        // no 11-bit value is 127 times a 9-bit one: top / 127 is never near a tie of bf16, and the product rounds as it does
-        s = bf16_round(act_of(top, kBf16) * (1.f / 127.f));
-        if (top >= (kBf16 ? 0x7f80u : 0x7c00u)) s = __int_as_float(0x7fc00000);
-      } else {
-        uint32_t hi2 = r4[0], lo2 = r4[0];
-#pragma unroll
-        for (int e = 1; e < 4; ++e) hi2 = pick2<kBf16, true>(hi2, r4[e]), lo2 = pick2<kBf16, false>(lo2, r4[e]);
-        hi2 = row_all<kLanes>(hi2, [](uint32_t a, uint32_t c) { return pick2<kBf16, true>(a, c); });
-        lo2 = row_all<kLanes>(lo2, [](uint32_t a, uint32_t c) { return pick2<kBf16, false>(a, c); });
-        const uint32_t lo = pick2<kBf16, false>(lo2, lo2 >> 16) & 0xffffu;
-        m = act_of(lo, kBf16);
-        const float range = act_of(pick2<kBf16, true>(hi2, hi2 >> 16) & 0xffffu, kBf16) - m;
-        s = range <= 3.402823466e38f ? bf16_round(__fdiv_rn(range, 15.f)) : __int_as_float(0x7fc00000);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] -= m;
-        word = lo << 16;
-      }
-      word |= __bfloat16_as_ushort(__float2bfloat16_rn(s));
-      uint32_t q[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
-      if (s > 0.f) quantise8(x, s, kFmt == RB_KV_INT8 ? -127 : 0, kFmt == RB_KV_INT8 ? 127 : 15, q);
-      if constexpr (kFmt == RB_KV_INT8) {  // + 128 of a signed byte: its top bit turned over
-        if (dst[i] >= 0)
-          reinterpret_cast<uint2*>(R.c)[dst[i] * kLanes + sub] =
-              make_uint2(low_bytes(q[0], q[1], q[2], q[3]) ^ 0x80808080u, low_bytes(q[4], q[5], q[6], q[7]) ^ 0x80808080u);
-      } else {
-        const uint32_t even = low_bytes(q[0], q[2], q[4], q[6]), odd = low_bytes(q[1], q[3], q[5], q[7]);
-        if (dst[i] >= 0) reinterpret_cast<uint32_t*>(R.c)[dst[i] * kLanes + sub] = even | (odd << 4);
-      }
-      if (p.by_head) {
-        if (sub == 0) par[i * kGroups + grp] = word;
-      } else if (sub == 0 && dst[i] >= 0) {
-        if constexpr (kFmt == RB_KV_INT8) reinterpret_cast<uint16_t*>(R.par)[dst[i]] = static_cast<uint16_t>(word);
-        else reinterpret_cast<uint32_t*>(R.par)[dst[i]] = word;
+    for (int i = 0; i < kRows; ++i) {
+      const int x = i * kGroups + grp;
+      quantise_row<kLanes, kFmt, kBf16>(raw[i], x >= lo && x < hi, codes + i * kGroups * kRowBytes, [&](uint32_t word) {
+        if (sub == 0) par[x] = word;
+      });
+    }
+    if constexpr (kFmt != RB_KV_PLAIN) {
+      __syncthreads();
+      uint8_t* dst = static_cast<uint8_t*>(R.par) + row * kParBytes;
+      for (int x = threadIdx.x; x < hi; x += kThreads) {
+        if (x < lo) continue;
+        if constexpr (kFmt == RB_KV_INT8) reinterpret_cast<uint16_t*>(dst)[x] = static_cast<uint16_t>(par[x]);
+        else reinterpret_cast<uint32_t*>(dst)[x] = par[x];
       }
     }
-  }
-  if constexpr (kFmt != RB_KV_PLAIN) {
-    if (!p.by_head) return;
-    __syncthreads();
-    for (int i = threadIdx.x; i < kTile; i += kThreads) {
-      const int64_t t = t0 + i;
-      if (t >= limit || !(at >= -t && at < p.cache_len - t)) continue;
-      const int64_t row = (b * p.n_heads + h0) * p.cache_len + at + t;
-      if constexpr (kFmt == RB_KV_INT8) reinterpret_cast<uint16_t*>(R.par)[row] = static_cast<uint16_t>(par[i]);
-      else reinterpret_cast<uint32_t*>(R.par)[row] = par[i];
+  } else {
+    int64_t dst[kRows];  // the row in the cache; -1: nothing to store
+    const uint32_t rows = static_cast<uint32_t>(p.n_tokens) * p.n_heads;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const uint32_t x = tile * kTile + i * kGroups + grp;
+      const uint32_t t = x / p.n_heads, h = x - t * p.n_heads;
+      const bool on = x < rows && t >= t_lo && t < t_end;
+      dst[i] = on ? (b * p.n_heads + h) * p.cache_len + at + t : -1;
+      raw[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (on) raw[i] = ldg_cg_128(src + t * R.s_tok + h * R.s_head);
+    }
+#pragma unroll 1
+    for (int i = 0; i < kRows; ++i) {
+      const int64_t d = i < 2 ? (i ? dst[1] : dst[0]) : (i == 2 ? dst[2] : dst[3]);
+      const uint4 v = i < 2 ? (i ? raw[1] : raw[0]) : (i == 2 ? raw[2] : raw[3]);
+      if (__all_sync(0xffffffffu, d < 0)) continue;  // a step of one token leaves most of the tile empty
+      quantise_row<kLanes, kFmt, kBf16>(v, d >= 0, codes + d * kRowBytes, [&](uint32_t word) {
+        if (sub != 0 || d < 0) return;
+        if constexpr (kFmt == RB_KV_INT8) reinterpret_cast<uint16_t*>(R.par)[d] = static_cast<uint16_t>(word);
+        else reinterpret_cast<uint32_t*>(R.par)[d] = word;
+      });
     }
   }
 }
@@ -301,6 +344,16 @@ int launch(void (*kern)(P), const P& p, int64_t blocks, int flags, cudaStream_t 
   return cudaLaunchKernelEx(&cfg, kern, p) == cudaSuccess ? RB_OK : RB_ERR_LAUNCH;
 }
 
+template <bool kByHead>
+auto write_kernel(int fmt, bool wide, bool bf) -> void (*)(WriteParams) {
+  if (fmt == RB_KV_PLAIN) return wide ? kv_write_kernel<128, RB_KV_PLAIN, false, kByHead> : kv_write_kernel<64, RB_KV_PLAIN, false, kByHead>;
+  if (fmt == RB_KV_INT8)
+    return wide ? (bf ? kv_write_kernel<128, RB_KV_INT8, true, kByHead> : kv_write_kernel<128, RB_KV_INT8, false, kByHead>)
+                : (bf ? kv_write_kernel<64, RB_KV_INT8, true, kByHead> : kv_write_kernel<64, RB_KV_INT8, false, kByHead>);
+  return wide ? (bf ? kv_write_kernel<128, RB_KV_INT4, true, kByHead> : kv_write_kernel<128, RB_KV_INT4, false, kByHead>)
+              : (bf ? kv_write_kernel<64, RB_KV_INT4, true, kByHead> : kv_write_kernel<64, RB_KV_INT4, false, kByHead>);
+}
+
 }  // namespace kvc
 
 int launch_kv_write(const rb_kv_cache* c, const void* k, const void* v, const int64_t* ks, const int64_t* vs,
@@ -321,15 +374,7 @@ int launch_kv_write(const rb_kv_cache* c, const void* k, const void* v, const in
   if (blocks > (int64_t(1) << 31) - 1) return RB_ERR_SHAPE;
   p.tiles = static_cast<uint32_t>(tiles);
   const bool bf = c->dtype == RB_BF16, wide = c->head_dim == 128;
-  void (*kern)(WriteParams);
-  if (c->fmt == RB_KV_PLAIN)
-    kern = wide ? kv_write_kernel<128, RB_KV_PLAIN, false> : kv_write_kernel<64, RB_KV_PLAIN, false>;
-  else if (c->fmt == RB_KV_INT8)
-    kern = wide ? (bf ? kv_write_kernel<128, RB_KV_INT8, true> : kv_write_kernel<128, RB_KV_INT8, false>)
-                : (bf ? kv_write_kernel<64, RB_KV_INT8, true> : kv_write_kernel<64, RB_KV_INT8, false>);
-  else
-    kern = wide ? (bf ? kv_write_kernel<128, RB_KV_INT4, true> : kv_write_kernel<128, RB_KV_INT4, false>)
-                : (bf ? kv_write_kernel<64, RB_KV_INT4, true> : kv_write_kernel<64, RB_KV_INT4, false>);
+  void (*kern)(WriteParams) = p.by_head ? write_kernel<true>(c->fmt, wide, bf) : write_kernel<false>(c->fmt, wide, bf);
   return launch(kern, p, blocks, flags, stream);
 }
 

@@ -100,6 +100,7 @@ class BeamTensor(ctypes.Structure):
 EPI_STORE, EPI_ROPE_KV, EPI_SWIGLU = 0, 1, 2
 # device error word bits (rb_get_device_error): a wait that ran out, or an out-of-range device-side argument
 DEVERR_TC_WAIT, DEVERR_TP_WAIT, DEVERR_ARG, DEVERR_ATT_WAIT, DEVERR_STEP_WAIT = 1 << 7, 1 << 8, 1 << 9, 1 << 10, 1 << 11
+DEVERR_PFX_WAIT = 1 << 12
 
 SIGNATURES = {
     "rb_gemv_int4": (_int, [_vp, _int, _i64, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _int, _vp]),

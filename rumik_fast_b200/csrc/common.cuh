@@ -32,6 +32,7 @@ enum : unsigned int {
   ERR_ARG = 1u << 9,          // a device-side argument (a decode position) was out of range; nothing stored
   ERR_ATT_WAIT = 1u << 10,    // a fused-attention launch timed out waiting for the attention outputs
   ERR_STEP_WAIT = 1u << 11,   // the whole-step kernel gave up a wait (and aborted the launch)
+  ERR_PFX_WAIT = 1u << 12,    // the prefix attention timed out on an mbarrier
 };
 
 // Upper bound on the wall time of one wait (an mbarrier phase, a peer's flag, a completion counter). Healthy
@@ -344,6 +345,30 @@ __device__ __forceinline__ void dq_scales8_f16x2(uint32_t words, float s_row, ui
 
 __device__ __forceinline__ float round_act(float v, bool is_bf16) {
   return is_bf16 ? __bfloat162float(__float2bfloat16_rn(v)) : __half2float(__float2half_rn(v));
+}
+
+// Two fp32 operations in one instruction (sm_100a): a b + c on both halves.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)),
+        "l"(*reinterpret_cast<unsigned long long*>(&c)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
 }
 
 // One element of a bf16 or fp16 array, to fp32.

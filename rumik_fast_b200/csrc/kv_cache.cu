@@ -72,23 +72,6 @@ __device__ __forceinline__ float act_of(uint32_t bits16, bool bf16) {
   return bf16 ? __uint_as_float(bits16 << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(bits16)));
 }
 
-// Two fp32 operations in one instruction (sm_100a): a b + c on both halves.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  unsigned long long d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(d)
-      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)),
-        "l"(*reinterpret_cast<unsigned long long*>(&c)));
-  return *reinterpret_cast<float2*>(&d);
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  unsigned long long d;
-  asm("add.rn.f32x2 %0, %1, %2;"
-      : "=l"(d)
-      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
-  return *reinterpret_cast<float2*>(&d);
-}
-
 // The 16-bit pair as fp32.
 template <bool kBf16>
 __device__ __forceinline__ float2 pair_of(uint32_t w) {

@@ -48,6 +48,7 @@ struct Params {
   float scale;
   int wm, tiles_m;   // warps along the rows of a tile, row tiles of the prefix's M = n_seqs rep rows
   int max_np;        // most splits of the prefix
+  int parts;         // partials a prefix split leaves: 1, or 2 (prefix_attn_tc.cu)
   int max_ns;        // most splits of a sequence's own rows
   float* o;          // partials: prefix items [n_kv][tiles_m][max_np][rows][hd], then own [n_seqs][n_kv][max_ns][rep][hd]
   float2* rl;        // the same without hd: (R, l)
@@ -781,12 +782,17 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_merge(const __grid_const
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int b = blockIdx.x / p.n_q, h = blockIdx.x % p.n_q, kv = h / p.rep, j = h % p.rep;
   const int64_t n_pre = p.pre.k ? __ldcg(p.pre.len) : 0, n_own = p.own.k ? __ldcg(p.own.len + b) : 0;
-  const int np = __ldcg(p.plan), ot = __ldcg(p.plan + 3);
+  const int ot = __ldcg(p.plan + 3);
+  int np = __ldcg(p.plan);
   if (n_pre < 0 || n_pre > p.pre.cache_len || n_own < 0 || n_own > p.own.cache_len) return;
+  if (p.parts == 2) {  // the tcgen05 kernel's splits: the tiles dealt evenly, two partials each
+    const int tiles = static_cast<int>((n_pre + 127) / 128), per = max(1, (tiles + p.max_np - 1) / p.max_np);
+    np = 2 * ((tiles + per - 1) / per);
+  }
   const int ns = n_own ? static_cast<int>(((n_own + stage - 1) / stage + ot - 1) / ot) : 0;
   const int r = b * p.rep + j, rt = r / tile_rows;
   // partial i: row x0 + i xs of the prefix's, then own row y0 + (i - np) rep
-  const int64_t x0 = (static_cast<int64_t>(kv) * p.tiles_m + rt) * p.max_np * tile_rows + r % tile_rows;
+  const int64_t x0 = (static_cast<int64_t>(kv) * p.tiles_m + rt) * p.max_np * p.parts * tile_rows + r % tile_rows;
   const int64_t y0 = p.own_rl + (static_cast<int64_t>(b) * p.n_kv + kv) * p.max_ns * p.rep + j;
   auto at = [&](int i) { return i < np ? x0 + static_cast<int64_t>(i) * tile_rows : y0 + static_cast<int64_t>(i - np) * p.rep; };
   const int n = np + ns;
@@ -820,7 +826,8 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_merge(const __grid_const
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const float f = v[k].x == -INFINITY ? 0.f : ex2(v[k].x - hi);
+      if (v[k].x == -INFINITY) continue;  // nothing there: its sums may not have been written
+      const float f = ex2(v[k].x - hi);
       l = fmaf(v[k].y, f, l);
 #pragma unroll
       for (int e = 0; e < kE; ++e) acc[e] = fmaf(x[k][e], f, acc[e]);
@@ -843,107 +850,6 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_merge(const __grid_const
   }
 }
 
-// Warps along the rows: the fewest whose 16-row tiles hold the batch's rows, at most four.
-inline int warps_m(int64_t rows) { return rows <= 16 ? 1 : (rows <= 32 ? 2 : 4); }
-
-struct Layout {
-  int grid, wm, tile_rows, tiles_m, max_np, max_ns;
-  int64_t pre_slots, own_slots, rl_bytes, o_bytes, total;
-};
-inline Layout layout_of(const rb_prefix_attn_args* a, int num_sms) {
-  const rb_kv_cache* c = a->prefix ? a->prefix : a->own;
-  const int rep = a->n_q_heads / c->n_kv_heads;
-  const int64_t rows = a->n_seqs * rep;
-  Layout L = {};
-  L.grid = kCtasPerSm * num_sms;
-  L.wm = warps_m(rows);
-  L.tile_rows = 16 * L.wm;
-  L.tiles_m = static_cast<int>((rows + L.tile_rows - 1) / L.tile_rows);
-  const int64_t lanes = static_cast<int64_t>(c->n_kv_heads) * L.tiles_m, heads = a->n_seqs * c->n_kv_heads;
-  L.max_np = a->prefix ? static_cast<int>(std::max<int64_t>(1, L.grid / std::max<int64_t>(lanes, 1))) : 0;
-  L.max_ns = a->own ? static_cast<int>(std::max<int64_t>(1, L.grid / std::max<int64_t>(heads, 1))) : 0;
-  L.pre_slots = lanes * L.max_np * L.tile_rows;
-  L.own_slots = heads * L.max_ns * rep;
-  L.rl_bytes = ((L.pre_slots + L.own_slots) * 8 + 255) / 256 * 256;
-  L.o_bytes = (L.pre_slots + L.own_slots) * c->head_dim * 4;
-  L.total = 256 + L.rl_bytes + L.o_bytes;
-  return L;
-}
-
-inline cudaLaunchConfig_t launch_config(int grid, int smem, int flags, cudaStream_t stream, cudaLaunchAttribute* attr) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = (flags & RB_FLAG_PDL) ? 1 : 0;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cfg;
-}
-
-template <typename F>
-int launch_format(const Params& p, const Layout& L, int flags, cudaStream_t stream) {
-  constexpr int smem = Tile<F>::kSmem;
-  static_assert((smem + 1024) * kCtasPerSm <= 227 * 1024, "CTAs an SM");
-  cudaLaunchAttribute attr[1];
-  if (ensure_smem_limit(reinterpret_cast<const void*>(prefix_attn_kernel<F>), smem) != cudaSuccess) return RB_ERR_LAUNCH;
-  cudaLaunchConfig_t cfg = launch_config(L.grid, smem, flags, stream, attr);
-  if (cudaLaunchKernelEx(&cfg, prefix_attn_kernel<F>, p) != cudaSuccess) return RB_ERR_LAUNCH;
-  cfg = launch_config(p.n_seqs * p.n_q, 0, flags, stream, attr);
-  return cudaLaunchKernelEx(&cfg, prefix_attn_merge<F::kHd>, p, L.tile_rows, F::kTile) == cudaSuccess ? RB_OK : RB_ERR_LAUNCH;
-}
-
 }  // namespace pfx
-
-int64_t prefix_attn_workspace(const rb_prefix_attn_args* a, int num_sms) { return pfx::layout_of(a, num_sms).total; }
-
-int launch_prefix_attn(const rb_prefix_attn_args* a, int num_sms, int flags, cudaStream_t stream) {
-  using namespace pfx;
-  const rb_kv_cache* c = a->prefix ? a->prefix : a->own;
-  const Layout L = layout_of(a, num_sms);
-  Params p = {};
-  p.q = a->q;
-  p.out = a->out;
-  p.ldq = a->ldq;
-  p.ldo = a->ldo;
-  auto side = [](const rb_kv_cache* s, const int64_t* len) {
-    return Side{static_cast<const uint8_t*>(s->k), static_cast<const uint8_t*>(s->v), s->k_par, s->v_par, len, s->cache_len};
-  };
-  if (a->prefix) p.pre = side(a->prefix, a->prefix_len);
-  if (a->own) p.own = side(a->own, a->own_len);
-  p.n_seqs = static_cast<int>(a->n_seqs);
-  p.n_q = a->n_q_heads;
-  p.n_kv = c->n_kv_heads;
-  p.rep = p.n_q / p.n_kv;
-  p.bf16 = c->dtype == RB_BF16;
-  p.scale = a->scale;
-  p.tiles_m = L.tiles_m;
-  p.max_np = L.max_np;
-  p.max_ns = L.max_ns;
-  uint8_t* w = static_cast<uint8_t*>(a->ws);
-  p.plan = reinterpret_cast<int*>(w);
-  p.rl = reinterpret_cast<float2*>(w + 256);
-  p.o = reinterpret_cast<float*>(w + 256 + L.rl_bytes);
-  p.own_rl = L.pre_slots;
-  p.own_o = L.pre_slots * c->head_dim;
-  p.wm = L.wm;
-  const bool wide = c->head_dim == 128;
-  switch (c->fmt) {
-    case RB_KV_INT8:
-      return wide ? launch_format<Fmt<128, RB_KV_INT8, false>>(p, L, flags, stream)
-                  : launch_format<Fmt<64, RB_KV_INT8, false>>(p, L, flags, stream);
-    case RB_KV_INT4:
-      return wide ? launch_format<Fmt<128, RB_KV_INT4, false>>(p, L, flags, stream)
-                  : launch_format<Fmt<64, RB_KV_INT4, false>>(p, L, flags, stream);
-    default:
-      if (p.bf16)
-        return wide ? launch_format<Fmt<128, RB_KV_PLAIN, true>>(p, L, flags, stream)
-                    : launch_format<Fmt<64, RB_KV_PLAIN, true>>(p, L, flags, stream);
-      return wide ? launch_format<Fmt<128, RB_KV_PLAIN, false>>(p, L, flags, stream)
-                  : launch_format<Fmt<64, RB_KV_PLAIN, false>>(p, L, flags, stream);
-  }
-}
 
 }  // namespace rb

@@ -20,9 +20,12 @@ from .cuda_gemv import _on_device, _require
 
 
 class PrefixAttention:
-    """Owns its workspace; calls sharing one object must be issued on one stream. scale: head_dim ** -0.5 by default."""
+    """Owns its workspace; calls sharing one object must be issued on one stream. scale: head_dim ** -0.5 by default.
+    kernel: which kernel streams the prefix, "tc" (tcgen05, 128 query rows a key-value head at a time) or "mma" (warp
+    level); None: by the number of rows and the prefix's capacity."""
 
-    def __init__(self, q, out, prefix=None, prefix_len=None, own=None, own_len=None, scale=None):
+    def __init__(self, q, out, prefix=None, prefix_len=None, own=None, own_len=None, scale=None, kernel=None):
+        _require(kernel in _lib.KERNEL_FLAGS, f"kernel must be None, 'tc' or 'mma', got {kernel!r}")
         _require(prefix is not None or own is not None, "a prefix or own rows are needed")
         c = prefix if prefix is not None else own
         B, nq, hd = q.shape if q.dim() == 3 else (0, 0, 0)
@@ -58,9 +61,9 @@ class PrefixAttention:
             _lib.check("rb_prefix_attn_workspace", -need)
         self.ws = torch.zeros(need, dtype=torch.uint8, device=self.device)
         a.ws, a.ws_bytes = self.ws.data_ptr(), need
-        self._args, self._ref = a, ctypes.byref(a)
+        self._args, self._ref, self._flags = a, ctypes.byref(a), _lib.KERNEL_FLAGS[kernel]
 
     def __call__(self):
         with _on_device(self.device):
-            st = _lib.lib().rb_prefix_attn(self._ref, config.flags(), _lib.stream_ptr(self.device))
+            st = _lib.lib().rb_prefix_attn(self._ref, config.flags() | self._flags, _lib.stream_ptr(self.device))
         _lib.check("rb_prefix_attn", st)

@@ -33,7 +33,7 @@ def rows(shape, dtype, seed, spread=1.0):
 class Setup:
     """Caches of a random prefix and random own rows (with NaN rows beyond every length), and the attention over them."""
 
-    def __init__(self, B, nq, nkv, hd, P, lens, fmt, dtype, seed=0, spread=1.0, slack=3):
+    def __init__(self, B, nq, nkv, hd, P, lens, fmt, dtype, seed=0, spread=1.0, slack=3, kernel=None):
         dt = DTYPES[dtype]
         self.B, self.fmt, self.dt, self.lens, self.scale = B, fmt, dt, lens, hd ** -0.5
         self.q = rows((B, nq, hd), dt, seed, spread)
@@ -59,7 +59,7 @@ class Setup:
             self.own_vals = tuple(ref.values(x, fmt).transpose(1, 2) for x in (k, v))
             self.own_len = torch.tensor(lens, device=DEV)
             kw.update(own=self.own, own_len=self.own_len)
-        self.attn = PrefixAttention(self.q.to(DEV), self.out, **kw)
+        self.attn = PrefixAttention(self.q.to(DEV), self.out, kernel=kernel, **kw)
 
     @staticmethod
     def fill(cache, value):
@@ -189,6 +189,85 @@ def test_a_nan_in_a_visible_row_shows(fmt):
     s.own.write(x.to(DEV), bad.to(DEV), torch.tensor([2, 5, 0], device=DEV))   # 1 and 2: beyond their lengths
     s.attn()
     assert torch.isnan(s.out[0, 2:]).any() and torch.isfinite(s.out[0, :2]).all() and torch.isfinite(s.out[1:]).all()
+
+
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("fmt", ["plain", "int8", "int4"])
+@pytest.mark.parametrize("B,nq,nkv,hd,P,lens", [
+    (1, 1, 1, 64, 1, None),
+    (1, 2, 2, 128, 127, [3]),
+    (5, 16, 4, 128, 128, [0, 1, 2, 3, 4]),
+    (11, 12, 4, 64, 129, None),
+    (16, 48, 8, 128, 300, [i * 5 % 23 for i in range(16)]),
+    (43, 6, 2, 128, 1000, None),
+    (64, 16, 2, 64, 2500, [i % 3 for i in range(64)]),
+    (150, 2, 1, 128, 6000, None),
+])
+def test_tcgen05_kernel_against_64_bits(B, nq, nkv, hd, P, lens, fmt, dtype):
+    """The tcgen05 kernel at sizes that the choice by rows would leave to the warp-level one as well: single rows and
+    tiles, tiles that end inside, several row tiles, one and many splits."""
+    s = Setup(B, nq, nkv, hd, P, lens, fmt, dtype, seed=B + P, kernel="tc")
+    s.attn()
+    assert rb.device_error() == 0
+    s.check()
+    first = s.out.clone()
+    s.attn()
+    assert torch.equal(first, s.out)
+
+
+@pytest.mark.parametrize("fmt", ["plain", "int8", "int4"])
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+def test_tcgen05_kernel_peaked_flat_and_rising_scores(fmt, dtype):
+    """Scores spread over hundreds, all equal, and rising along the prefix (the references are raised again and again)."""
+    s = Setup(20, 6, 2, 128, 1500, [i % 5 for i in range(20)], fmt, dtype, seed=8, spread=6.0, kernel="tc")
+    s.attn()
+    s.check()
+    s.q.zero_()
+    s.attn._keep[0].zero_()
+    s.attn()
+    s.check()
+    k = rows((1, 1500, 2, 128), s.dt, 1)
+    k = (k.float() * torch.linspace(0, 12, 1500)[None, :, None, None]).to(s.dt)
+    v = rows((1, 1500, 2, 128), s.dt, 2)
+    s.pre.write(k.to(DEV), v.to(DEV), torch.zeros(1, dtype=torch.int64, device=DEV))
+    s.pre_vals = tuple(ref.values(x[0], fmt).transpose(0, 1) for x in (k, v))
+    s.q = rows((20, 6, 128), s.dt, 3)
+    s.attn._keep[0].copy_(s.q)
+    s.attn()
+    s.check()
+
+
+def test_tcgen05_kernel_lengths_and_nan():
+    """Lengths that change under one object, none, out of range, and a NaN among the prefix's values."""
+    for fmt in ("plain", "int8", "int4"):
+        s = Setup(12, 8, 2, 128, 700, [i for i in range(12)], fmt, "fp16", seed=20, kernel="tc")
+        for P in (700, 1, 300, 0):
+            s.prefix_len.fill_(P)
+            s.attn()
+            s.check(P=P)
+        s.out.fill_(7)
+        s.prefix_len.fill_(704)
+        s.attn()
+        assert rb.device_error() == rb._lib.DEVERR_ARG and (s.out == 7).all()
+        s.prefix_len.fill_(700)
+        bad = torch.full((1, 1, 2, 128), float("nan"), dtype=torch.float16, device=DEV)
+        s.pre.write(bad, bad, torch.tensor([650], device=DEV))
+        s.attn()
+        assert torch.isnan(s.out).all()
+        s.prefix_len.fill_(650)
+        s.attn()
+        s.check(P=650)
+
+
+def test_tcgen05_kernel_negative_and_zero_scale():
+    for scale in (-0.1, 0.0):
+        for fmt in ("plain", "int8", "int4"):
+            for kernel in ("tc", "mma"):
+                s = Setup(12, 8, 2, 64, 300, [i for i in range(12)], fmt, "bf16", seed=21)
+                s.scale = scale
+                PrefixAttention(s.attn._keep[0], s.out, prefix=s.pre, prefix_len=s.prefix_len, own=s.own, own_len=s.own_len,
+                                scale=scale, kernel=kernel)()
+                s.check()
 
 
 def test_strided_queries_and_outputs():

@@ -37,7 +37,7 @@ def build(force=False, verbose=False):
     """Compile the library if any source is newer than it. Returns the path of the .so."""
     if not force and up_to_date():
         return OUT
-    cmd = [_nvcc(), *ARCH, "-lineinfo", "-O3", "-std=c++17", "--split-compile=0", "-Xcompiler", "-fPIC", "-shared",
+    cmd = [_nvcc(), *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-shared",
            "-o", OUT + ".tmp", SRC]
     if verbose:
         print(" ".join(cmd), flush=True)

@@ -6,12 +6,16 @@
 //   S = Q K^T    Q and K in shared memory (K-major, 128-byte swizzle), S in tensor memory
 //   O += P V     P in tensor memory as 16-bit values over the columns of S it came from, V in shared memory as its rows
 //                lie (MN-major), O in tensor memory
-// Two groups of four softmax warps (thread = row = tensor-memory lane) take the tiles in turn, each with its own S, its
-// own O and its own references: 4 x 128 columns fill the tensor memory, and a group only waits for the tensor core. They
-// leave two partials. One thread issues every MMA, in the order QK(0) QK(1) PV(0) QK(2) PV(1) ...: MMAs of one thread
-// complete in order, so QK(t + 2) may overwrite the columns that PV(t) read. Eight loader warps fill rings of two key
-// and three value tiles: 16-bit rows by asynchronous copies, codes through registers, converted to 16-bit integers on
-// the way (a tile ahead, so that a whole tile of codes is always in flight).
+// Two groups of four softmax warps take the tiles in turn, each with its own S, its own O and its own references: 4 x 128
+// columns fill the tensor memory, and a group only waits for the tensor core. They leave two partials. A warp reads its
+// 32 lanes of S as 16 x 256-bit fragments: a thread then holds every fourth pair of columns of four rows, and needs a
+// quarter of the tile's scales - delivering all of them to every thread took longer than the exponentials. Rows lie on
+// lanes 32 (r % 4) + r / 4, so that a batch of up to 64 rows uses half of each warp's lanes, not two of the four warps.
+// A group's first warp issues its MMAs, PV(t) and then QK(t + 2): MMAs of one thread complete in order, so QK(t + 2) may
+// overwrite the columns that PV(t) reads. Four warps fill a ring of key tiles and four a ring of value tiles: 16-bit rows
+// by asynchronous copies, two tiles ahead; codes through registers, converted to 16-bit integers on the way, the next
+// tile's already in flight. (One warp for all MMAs made 17 warps, which leaves 96 registers a thread and spills; four
+// loader warps for both rings paced the whole kernel at 4,100 cycles a tile.)
 #include "common.cuh"
 #include "tc.cuh"
 #include "kernels.h"
@@ -25,13 +29,14 @@ using pfx::Item;
 using pfx::Params;
 
 constexpr int kTile = 128;        // slots of a tile, and query rows of a CTA
-constexpr int kSoftWarps = 8;
-constexpr int kMmaWarp = 8;
-constexpr int kFirstLoad = 9;
-constexpr int kLoadWarps = 8;
+constexpr int kFirstK = 8, kFirstV = 12;  // warps 0 .. 7: two softmax groups; 8 .. 11 and 12 .. 15: loaders
+constexpr int kLoadWarps = 4;
 constexpr int kLoadThreads = kLoadWarps * 32;
-constexpr int kThreads = (kFirstLoad + kLoadWarps) * 32;
-constexpr int kKRing = 2, kVRing = 3;
+constexpr int kThreads = 512;
+// The softmax warps hold a tile's scores in registers, 128 a thread; the loaders give them up.
+constexpr int kSoftRegs = 184, kLoadRegs = 72;
+static_assert(2 * kSoftRegs + 2 * kLoadRegs <= 4 * (65536 / kThreads), "registers of the launch, by warpgroup");
+constexpr int kVRing = 3, kKParRing = 4;
 constexpr uint32_t kTmemCols = 512;
 
 template <int kHd_, int kFmt_, bool kBf16_>
@@ -41,10 +46,16 @@ struct Fmt {
   static constexpr int kRow = kPlain ? 2 * kHd : (kFmt == RB_KV_INT8 ? kHd : kHd / 2);
   static constexpr int kAtom = kTile * 128;              // 64 columns of 128 rows
   static constexpr int kTileBytes = kTile * kHd * 2;     // a tile of 16-bit values
-  static constexpr int kPar = kTile * 4 * 4;             // fp32 s of keys, s of values, m of keys, m of values
+  static constexpr int kKRing = kPlain ? 3 : 2;          // copies two tiles ahead need three
+  // fp32 s and m of a tile's keys (values), in the order in which the fragments need them: slot 8 u + 2 c + e at
+  // c kParC + 2 u + e, so that a lane reads its columns in sixteen-byte pieces and the four c fall on different banks
+  static constexpr int kParC = kTile / 4 + 4, kParN = 4 * kParC;
+  static constexpr int kPar = kPlain ? 0 : kParN * 4 * 2;
   static constexpr int kOffK = kTileBytes, kOffV = kOffK + kKRing * kTileBytes, kOffPar = kOffV + kVRing * kTileBytes;
-  static constexpr int kOffBar = kOffPar + kVRing * kPar;
-  static constexpr int kBars = 2 * kKRing + 2 * kVRing + 3 * 2 + 1;
+  static constexpr int kOffVPar = kOffPar + kKParRing * kPar;
+  static constexpr int kOffRow = kOffVPar + kVRing * kPar;  // factor and sum of the rows' queries
+  static constexpr int kOffBar = kOffRow + kTile * 8;
+  static constexpr int kBars = 2 * kKRing + 2 * kVRing + 2 * 2;
   static constexpr int kSmem = 1024 + kOffBar + kBars * 8 + 16;
   static constexpr int kRaw = kPlain ? 1 : kTile * kRow / 16 / kLoadThreads;  // 16-byte pieces of a thread in a tile of codes
   static constexpr uint32_t kType = kBf16 ? 1u : 0u;
@@ -74,27 +85,6 @@ __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint
       : "memory");
 }
 
-__device__ __forceinline__ void tmem_ld32(uint32_t a, float (&f)[32]) {
-  uint32_t v[32];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
-      "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
-        "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]),
-        "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
-        "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-      : "r"(a)
-      : "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
-}
-__device__ __forceinline__ void tmem_st16(uint32_t a, const uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(a),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
-      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-      : "memory");
-}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
@@ -106,8 +96,300 @@ __device__ __forceinline__ float4 lds128f(uint32_t a) {
   return v;
 }
 
+// One lane of a converged warp; the compiler keeps what is computed for it in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t on;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(on));
+  return on != 0;
+}
+
 // Byte offset of the 16-byte piece `ch` (eight 16-bit columns) of row r in a swizzled tile.
 __device__ __forceinline__ uint32_t piece_at(int r, int ch) { return (ch >> 3) * (kTile * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4); }
+
+constexpr int kBarSoft = 1, kBarGroup = 2;  // named barriers: all softmax warps; a group (2, 3)
+
+// 16 lanes x 128 columns as fragments: x[4 u + e] is column 8 u + 2 c + (e & 1) of lane l + 8 (e >> 1), with l = lane / 4 and
+// c = lane % 4. Valid after tmem_wait_ld.
+__device__ __forceinline__ void tmem_ld_frag(uint32_t a, float (&x)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];"
+      : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7]), "=f"(x[8]), "=f"(x[9]), "=f"(x[10]), "=f"(x[11]), "=f"(x[12]), "=f"(x[13]), "=f"(x[14]), "=f"(x[15]), "=f"(x[16]), "=f"(x[17]), "=f"(x[18]), "=f"(x[19]), "=f"(x[20]), "=f"(x[21]), "=f"(x[22]), "=f"(x[23]), "=f"(x[24]), "=f"(x[25]), "=f"(x[26]), "=f"(x[27]), "=f"(x[28]), "=f"(x[29]), "=f"(x[30]), "=f"(x[31]), "=f"(x[32]), "=f"(x[33]), "=f"(x[34]), "=f"(x[35]), "=f"(x[36]), "=f"(x[37]), "=f"(x[38]), "=f"(x[39]), "=f"(x[40]), "=f"(x[41]), "=f"(x[42]), "=f"(x[43]), "=f"(x[44]), "=f"(x[45]), "=f"(x[46]), "=f"(x[47]), "=f"(x[48]), "=f"(x[49]), "=f"(x[50]), "=f"(x[51]), "=f"(x[52]), "=f"(x[53]), "=f"(x[54]), "=f"(x[55]), "=f"(x[56]), "=f"(x[57]), "=f"(x[58]), "=f"(x[59]), "=f"(x[60]), "=f"(x[61]), "=f"(x[62]), "=f"(x[63])
+      : "r"(a));
+}
+// The same of 16 columns.
+__device__ __forceinline__ void tmem_ld_frag16(uint32_t a, float (&x)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7])
+               : "r"(a));
+}
+__device__ __forceinline__ void tmem_st_frag16(uint32_t a, const float (&x)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.16x256b.x2.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(a), "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
+               : "memory");
+}
+// 16 lanes x 16 columns of packed pairs: v[2 i + h] is column 4 i + c of lane l + 8 h.
+__device__ __forceinline__ void tmem_st_pairs(uint32_t a, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+template <int N>
+__device__ __forceinline__ void tmem_wait_ld(float (&x)[N]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+f"(x[i]));
+}
+
+// The softmax warps' work on the CTA's tiles. kH: 16-lane halves of a warp that hold rows of the batch.
+template <typename F, int kH>
+__device__ __forceinline__ void run_softmax(const Params& p, uint32_t s0, uint8_t* smem, uint32_t tmem, int g, int quad, int lane, int nt,
+                                            int64_t n, int rows, int64_t split) {
+  uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + F::kOffBar);
+  uint64_t* kempty = kfull + F::kKRing;
+  uint64_t* vfull = kempty + F::kKRing;
+  uint64_t* vempty = vfull + kVRing;
+  uint64_t* sfull = vempty + kVRing + g;
+  uint64_t* pvdone = sfull + 2;
+  const float* rowf = reinterpret_cast<const float*>(smem + F::kOffRow);
+  const int l0 = lane >> 2, c = lane & 3;
+  const uint32_t tq = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+  const uint32_t ts = tq + g * kTile, to = tq + (2 + g) * kTile, half = 16u << 16;  // the second half's lanes
+  const bool busy = quad < rows;
+  float fr[2 * kH], qs[2 * kH], ref[2 * kH], ve = F::kPlain ? 0.f : pfx::kLowestE;  // row y of the thread: lane 16 (y / 2) + 8 (y % 2) + l0
+  float l[2 * kH], w[2 * kH];
+#pragma unroll
+  for (int y = 0; y < 2 * kH; ++y) {
+    const int at = quad * 32 + 8 * y + l0;
+    fr[y] = rowf[at];
+    qs[y] = F::kFmt == RB_KV_INT4 ? rowf[kTile + at] : 0.f;
+    ref[y] = -INFINITY;
+    l[y] = w[y] = 0.f;
+  }
+  bool ok = true;
+  // The group's first warp: S = Q K^T of tile t, once its keys are there.
+  auto issue_qk = [&](int t) {
+    const int ks = t % F::kKRing;
+    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(kfull + ks, (t / F::kKRing) & 1, ERR_PFX_WAIT));
+    mm4::tc_fence_after();
+    if (ok && elect_one()) {
+      const uint64_t qd = mm4::sw128_desc(s0), kd = mm4::sw128_desc(s0 + F::kOffK + ks * F::kTileBytes);
+#pragma unroll
+      for (int i = 0; i < F::kHd / 16; ++i) {
+        const uint32_t at = ((i >> 2) * F::kAtom + (i & 3) * 32) >> 4;
+        umma_ss(tmem + g * kTile, qd + at, kd + at, F::kIdescQk, i != 0);
+      }
+      mm4::umma_commit(sfull);
+      mm4::umma_commit(kempty + ks);
+    }
+    __syncwarp();
+  };
+  if (quad == 0 && g < nt) issue_qk(g);
+  // Every warp goes through every tile, also after a wait that ran out, so that the group's barrier is complete.
+#pragma unroll 1
+  for (int t = g; t < nt; t += 2) {
+    if (ok) ok = mbar_wait(sfull, (t >> 1) & 1, ERR_PFX_WAIT);
+    if (ok) ok = mbar_wait(vfull + t % kVRing, (t / kVRing) & 1, ERR_PFX_WAIT);  // its parameters; the PV below needs them
+    ok = __all_sync(0xffffffffu, ok);
+    mm4::tc_fence_after();
+    if (busy && ok) {
+      const uint32_t kpar = s0 + F::kOffPar + (t % kKParRing) * F::kPar + c * (F::kParC * 4);
+      const uint32_t vpar = s0 + F::kOffVPar + (t % kVRing) * F::kPar + c * (F::kParC * 4);
+      // A lane's row parameters of the columns 8 u + 2 c, two u at a time, loaded kAhead steps before they are used: a load
+      // from shared memory takes long while the tensor core reads its operands there.
+      constexpr int kAhead = F::kFmt == RB_KV_INT4 ? 1 : 2;
+      float4 ps[kAhead], pm[F::kFmt == RB_KV_INT4 ? kAhead : 1];
+      auto ahead = [&](uint32_t base, int i) {
+        if constexpr (!F::kPlain) {
+          ps[i % kAhead] = lds128f(base + 16 * i);
+          if constexpr (F::kFmt == RB_KV_INT4) pm[i % kAhead] = lds128f(base + F::kParN * 4 + 16 * i);
+        }
+      };
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) ahead(kpar, i);
+      const int left = static_cast<int>(min(n - static_cast<int64_t>(t) * kTile, int64_t(kTile)));
+      float ven = ve;
+      if constexpr (!F::kPlain) {
+        // the tile's largest value scale: its exponent is part of every row's reference
+        const float4 s = lds128f(vpar + ((lane >> 3) - c) * (F::kParC * 4) + 16 * (lane & 7));
+        auto bits = [](float f) { return f == f ? __float_as_uint(f) : 0u; };  // a NaN shows by itself
+        const uint32_t hi = __reduce_max_sync(0xffffffffu, max(max(bits(s.x), bits(s.y)), max(bits(s.z), bits(s.w))));
+        ven = fmaxf(ve, fminf(fmaxf(static_cast<float>(static_cast<int>(hi >> 23) - 127), pfx::kLowestE), pfx::kHighestE));
+      }
+      // the rows' scores, scaled by the keys' scales, -inf beyond the prefix
+      float x[kH][64];
+#pragma unroll
+      for (int h = 0; h < kH; ++h) tmem_ld_frag(ts + h * half, x[h]);
+#pragma unroll
+      for (int h = 0; h < kH; ++h) tmem_wait_ld(x[h]);
+      if constexpr (!F::kPlain) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float4 k4 = ps[i % kAhead], m4 = F::kFmt == RB_KV_INT4 ? pm[i % (F::kFmt == RB_KV_INT4 ? kAhead : 1)] : k4;
+          if (i + kAhead < 8) ahead(kpar, i + kAhead);
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const int u = 2 * i + q;
+            const float2 ks = q ? make_float2(k4.z, k4.w) : make_float2(k4.x, k4.y), km = q ? make_float2(m4.z, m4.w) : make_float2(m4.x, m4.y);
+#pragma unroll
+            for (int y = 0; y < 2 * kH; ++y) {
+              float& a = x[y >> 1][4 * u + 2 * (y & 1)];
+              float& b = x[y >> 1][4 * u + 2 * (y & 1) + 1];
+              float2 v = make_float2(a, b);
+              if constexpr (F::kFmt == RB_KV_INT8) v = mul2(v, ks);
+              else v = fma2(v, ks, mul2(km, make_float2(qs[y], qs[y])));
+              a = v.x, b = v.y;
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) ahead(vpar, i);
+      }
+      if (left < kTile) {
+#pragma unroll
+        for (int h = 0; h < kH; ++h)
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (8 * (i >> 2) + 2 * c + (i & 1) >= left) x[h][i] = -INFINITY;
+      }
+      float top[2 * kH];
+      bool raise = ven > ve;
+#pragma unroll
+      for (int y = 0; y < 2 * kH; ++y) {
+        top[y] = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 16; ++u) top[y] = fmaxf(top[y], fmaxf(x[y >> 1][4 * u + 2 * (y & 1)], x[y >> 1][4 * u + 2 * (y & 1) + 1]));
+        raise |= top[y] * fr[y] > ref[y] + pfx::kSlack;
+      }
+      if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+        for (int y = 0; y < 2 * kH; ++y) {
+          float v = top[y];
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+          const float nr = fmaxf(ref[y], v * fr[y]);
+          top[y] = ref[y] == -INFINITY ? 0.f : ex2((ref[y] - nr) + (ve - ven));  // the rows' factor from here on
+          ref[y] = nr;
+          l[y] *= top[y];
+          w[y] *= top[y];
+        }
+        if (t >= 2) {  // the group's O holds something: all of it is there, and the next PV waits for this tile's P
+          ok = __all_sync(0xffffffffu, mbar_wait(pvdone, ((t >> 1) - 1) & 1, ERR_PFX_WAIT));
+          mm4::tc_fence_after();
+#pragma unroll 1
+          for (int c0 = 0; c0 < F::kHd && ok; c0 += 16) {
+#pragma unroll
+            for (int h = 0; h < kH; ++h) {
+              float v[8];
+              tmem_ld_frag16(to + h * half + c0, v);
+              tmem_wait_ld(v);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[i] *= top[2 * h + ((i >> 1) & 1)];
+              tmem_st_frag16(to + h * half + c0, v);
+            }
+          }
+        }
+      }
+      // P = 2^(t - R), over the columns that S came from
+      float base[2 * kH];
+#pragma unroll
+      for (int y = 0; y < 2 * kH; ++y) base[y] = ref[y] == -INFINITY ? 0.f : -(ref[y] + ven);
+#pragma unroll
+      for (int u0 = 0; u0 < 16; u0 += 4) {  // 32 columns: sixteen of packed pairs, and sixteen for their remainders
+        uint32_t hi[kH][8], lo[F::kFmt == RB_KV_INT4 ? kH : 1][8];
+#pragma unroll
+        for (int u = u0; u < u0 + 4; ++u) {
+          float2 vs = make_float2(1.f, 1.f), vm = make_float2(0.f, 0.f);
+          if constexpr (!F::kPlain) {
+            const int i = u >> 1;
+            const float4 s4 = ps[i % kAhead];
+            vs = (u & 1) ? make_float2(s4.z, s4.w) : make_float2(s4.x, s4.y);
+            if constexpr (F::kFmt == RB_KV_INT4) {
+              const float4 m4 = pm[i % kAhead];
+              vm = (u & 1) ? make_float2(m4.z, m4.w) : make_float2(m4.x, m4.y);
+            }
+            if ((u & 1) && i + kAhead < 8) ahead(vpar, i + kAhead);
+          }
+#pragma unroll
+          for (int y = 0; y < 2 * kH; ++y) {
+            float2 v = make_float2(x[y >> 1][4 * u + 2 * (y & 1)], x[y >> 1][4 * u + 2 * (y & 1) + 1]);
+            v = fma2(v, make_float2(fr[y], fr[y]), make_float2(base[y], base[y]));
+            v.x = ex2(v.x);
+            v.y = ex2(v.y);
+            l[y] += v.x + v.y;
+            if constexpr (F::kFmt == RB_KV_INT4) w[y] = fmaf(v.x, vm.x, fmaf(v.y, vm.y, w[y]));
+            if constexpr (!F::kPlain) v = mul2(v, vs);
+            uint32_t& out = hi[y >> 1][2 * (u - u0) + (y & 1)];
+            out = pfx::pack2<F::kBf16>(v.x, v.y);
+            if constexpr (F::kFmt == RB_KV_INT4) {  // what the rounding of p s left, as a second term
+              const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&out));
+              lo[y >> 1][2 * (u - u0) + (y & 1)] = pfx::pack2<false>(v.x - r.x, v.y - r.y);
+            }
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < kH; ++h) {
+          tmem_st_pairs(ts + h * half + 8 * u0, hi[h]);
+          if constexpr (F::kFmt == RB_KV_INT4) tmem_st_pairs(ts + h * half + 8 * u0 + 16, lo[h]);
+        }
+      }
+      ve = ven;
+      tmem_wait_st();
+    }
+    mm4::tc_fence_before();
+    named_bar_sync(kBarGroup + g, 128);  // the group's P is complete
+    if (quad == 0) {
+      mm4::tc_fence_after();
+      const int vs = t % kVRing;
+      if (ok && elect_one()) {
+        const uint64_t vd = v_desc(s0 + F::kOffV + vs * F::kTileBytes, F::kAtom);
+        const uint32_t s = tmem + g * kTile, o = tmem + (2 + g) * kTile;
+#pragma unroll
+        for (int i = 0; i < kTile / 16; ++i)
+          umma_ts(o, s + 32 * (i >> 1) + 8 * (i & 1), vd + i * (2048 >> 4), F::kIdescPv, t >= 2 || i != 0);
+        if constexpr (F::kFmt == RB_KV_INT4) {
+#pragma unroll
+          for (int i = 0; i < kTile / 16; ++i)
+            umma_ts(o, s + 32 * (i >> 1) + 16 + 8 * (i & 1), vd + i * (2048 >> 4), F::kIdescPv, 1);
+        }
+        mm4::umma_commit(vempty + vs);
+        mm4::umma_commit(pvdone);
+      }
+      __syncwarp();
+      if (t + 2 < nt) issue_qk(t + 2);
+    }
+  }
+  // ---- the group's partial ----
+  const int mine = nt > g ? (nt - g + 1) / 2 : 0;  // tiles of this group
+  if (mine && ok) ok = __all_sync(0xffffffffu, mbar_wait(pvdone, (mine - 1) & 1, ERR_PFX_WAIT));
+  mm4::tc_fence_after();
+  const int64_t first = (split * 2 + g) * kTile;
+#pragma unroll
+  for (int y = 0; y < 2 * kH; ++y) {
+    l[y] += __shfl_xor_sync(0xffffffffu, l[y], 1);
+    l[y] += __shfl_xor_sync(0xffffffffu, l[y], 2);
+    w[y] += __shfl_xor_sync(0xffffffffu, w[y], 1);
+    w[y] += __shfl_xor_sync(0xffffffffu, w[y], 2);
+    const int r = (8 * y + l0) * 4 + quad;
+    if (c == 0 && r < rows)
+      p.rl[first + r] = make_float2(!mine || (ref[y] == -INFINITY && l[y] == 0.f) ? -INFINITY : (ref[y] == -INFINITY ? 0.f : ref[y] + ve), l[y]);
+  }
+  if (mine && busy && ok) {
+#pragma unroll 2
+    for (int c0 = 0; c0 < F::kHd; c0 += 16) {
+#pragma unroll
+      for (int h = 0; h < kH; ++h) {
+        float v[8];
+        tmem_ld_frag16(to + h * half + c0, v);
+        tmem_wait_ld(v);
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          const int y = 2 * h + ((i >> 1) & 1), r = (8 * y + l0) * 4 + quad;
+          if (r < rows)
+            *reinterpret_cast<float2*>(p.o + (first + r) * F::kHd + c0 + 8 * (i >> 2) + 2 * c) = make_float2(v[i] + w[y], v[i + 1] + w[y]);
+        }
+      }
+    }
+  }
+  mm4::tc_fence_before();
+}
 
 template <typename F>
 __global__ void __launch_bounds__(kThreads, 1) prefix_attn_tc_kernel(const __grid_constant__ Params p) {
@@ -116,14 +398,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attn_tc_kernel(const __gri
   const uint32_t s0 = smem_u32(smem);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + F::kOffBar);
-  uint64_t* kempty = kfull + kKRing;
-  uint64_t* vfull = kempty + kKRing;
+  uint64_t* kempty = kfull + F::kKRing;
+  uint64_t* vfull = kempty + F::kKRing;
   uint64_t* vempty = vfull + kVRing;
   uint64_t* sfull = vempty + kVRing;  // [2] S of the group's tile is there
-  uint64_t* pfull = sfull + 2;        // [2] the group has written P (four warps)
-  uint64_t* pvdone = pfull + 2;       // [2] the group's last PV is complete
-  uint64_t* qfull = pvdone + 2;       // Q is in shared memory (four warps)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(qfull + 1);
+  uint64_t* pvdone = sfull + 2;       // [2] the group's last PV is complete
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pvdone + 2);
 
   griddep_wait();
   griddep_launch_dependents();
@@ -140,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attn_tc_kernel(const __gri
   if (nt <= 0) return;  // the merge knows which splits there are
 
   if (tid == 0) {
-    for (int i = 0; i < kKRing; ++i) {
+    for (int i = 0; i < F::kKRing; ++i) {
       mbar_init(kfull + i, kLoadWarps);
       mbar_init(kempty + i, 1);
     }
@@ -150,13 +430,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attn_tc_kernel(const __gri
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(sfull + i, 1);
-      mbar_init(pfull + i, 4);
       mbar_init(pvdone + i, 1);
     }
-    mbar_init(qfull, 4);
     fence_mbar_init();
   }
-  if (warp == kMmaWarp) {
+  if (warp == kFirstK) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kTmemCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -167,109 +445,113 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attn_tc_kernel(const __gri
   const uint32_t tmem = *tmem_slot;  // S of group 0, S of group 1, O of group 0, O of group 1: 128 columns each
   const int64_t head = static_cast<int64_t>(kv) * p.pre.cache_len;  // the head's first row
 
-  if (warp == kMmaWarp) {
-    // ---------------- MMA issuer ----------------
-    if (lane == 0) {
-      bool ok = mbar_wait(qfull, 0, ERR_PFX_WAIT);
-      mm4::tc_fence_after();
-      for (int t = 0; t <= nt && ok; ++t) {
-        if (t < nt) {
-          const int ks = t % kKRing;
-          ok = mbar_wait(kfull + ks, (t / kKRing) & 1, ERR_PFX_WAIT);
-          if (!ok) break;
-          mm4::tc_fence_after();
-          const uint32_t kt = s0 + F::kOffK + ks * F::kTileBytes;
-#pragma unroll
-          for (int i = 0; i < F::kHd / 16; ++i)
-            umma_ss(tmem + (t & 1) * kTile, mm4::sw128_desc(s0 + (i >> 2) * F::kAtom + (i & 3) * 32),
-                    mm4::sw128_desc(kt + (i >> 2) * F::kAtom + (i & 3) * 32), F::kIdescQk, i != 0);
-          mm4::umma_commit(sfull + (t & 1));
-          mm4::umma_commit(kempty + ks);
-        }
-        if (t > 0) {
-          const int u = t - 1, vs = u % kVRing, g = u & 1;
-          ok = mbar_wait(vfull + vs, (u / kVRing) & 1, ERR_PFX_WAIT) && mbar_wait(pfull + g, (u >> 1) & 1, ERR_PFX_WAIT);
-          if (!ok) break;
-          mm4::tc_fence_after();
-          const uint32_t vt = s0 + F::kOffV + vs * F::kTileBytes, s = tmem + g * kTile, o = tmem + (2 + g) * kTile;
-#pragma unroll
-          for (int i = 0; i < kTile / 16; ++i)
-            umma_ts(o, s + 32 * (i >> 1) + 8 * (i & 1), v_desc(vt + i * 2048, F::kAtom), F::kIdescPv, u >= 2 || i != 0);
-          if constexpr (F::kFmt == RB_KV_INT4) {
-#pragma unroll
-            for (int i = 0; i < kTile / 16; ++i)
-              umma_ts(o, s + 32 * (i >> 1) + 16 + 8 * (i & 1), v_desc(vt + i * 2048, F::kAtom), F::kIdescPv, 1);
-          }
-          mm4::umma_commit(vempty + vs);
-          mm4::umma_commit(pvdone + g);
-        }
-      }
-    }
-  } else if (warp >= kFirstLoad) {
-    // ---------------- loaders ----------------
-    const int lt = tid - kFirstLoad * 32;
+  if (warp >= kFirstK) {
+    // ---------------- loaders: four warps of keys, four of values ----------------
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
+    const bool keys = warp < kFirstV;
+    const int lw = warp - (keys ? kFirstK : kFirstV), lt = lw * 32 + lane;
+    const int ring = keys ? F::kKRing : kVRing;
+    uint64_t* full = keys ? kfull : vfull;
+    uint64_t* empty = keys ? kempty : vempty;
+    const uint8_t* src = (keys ? p.pre.k : p.pre.v) + head * F::kRow;
+    const uint32_t base = s0 + (keys ? F::kOffK : F::kOffV);
     bool ok = true;
-    auto arrive = [&](uint64_t* bar) {
+    auto arrive = [&](int slot) {
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar);
+      if (lane == 0) mbar_arrive(full + slot);
     };
-    const uint8_t* k = p.pre.k + head * F::kRow;
-    const uint8_t* v = p.pre.v + head * F::kRow;
+    int slot = 0, phase = 1;  // of the tile to fill: its slot, and the parity of the release that it waits for
+    auto free_slot = [&](int t) {
+      if (t >= ring && ok) ok = mbar_wait(empty + slot, phase, ERR_PFX_WAIT);
+      ok = __all_sync(0xffffffffu, ok);
+      return ok;
+    };
+    auto next_slot = [&] {
+      if (++slot == ring) slot = 0, phase ^= 1;
+    };
     if constexpr (F::kPlain) {
       constexpr int kPieces = F::kRow / 16, kEach = kTile * kPieces / kLoadThreads;
-      auto load = [&](const uint8_t* src, uint32_t dst, int t) {
-        const int64_t first = static_cast<int64_t>(t0 + t) * kTile;
+      int landed = 0;  // slot of the tile to release
+      for (int t = 0; t < nt + 2; ++t) {
+        if (t < nt) {
+          if (!free_slot(t)) break;
+          const int64_t first = static_cast<int64_t>(t0 + t) * kTile;
+          const uint32_t dst = base + slot * F::kTileBytes;
+          const uint8_t* from = src + first * F::kRow + lt * 16;
+          if (first + kTile <= n) {
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-          const int x = i * kLoadThreads + lt, r = x / kPieces, ch = x % kPieces;
-          const bool on = first + r < n;
-          pfx::cp_async16(dst + piece_at(r, ch), on ? src + (first + r) * F::kRow + ch * 16 : src, on);
+            for (int i = 0; i < kEach; ++i) {
+              const int x = i * kLoadThreads + lt;
+              pfx::cp_async16(dst + piece_at(x / kPieces, x % kPieces), from + i * kLoadThreads * 16, true);
+            }
+          } else {
+#pragma unroll 1
+            for (int i = 0; i < kEach; ++i) {
+              const int x = i * kLoadThreads + lt;
+              const bool on = first + x / kPieces < n;
+              pfx::cp_async16(dst + piece_at(x / kPieces, x % kPieces), on ? from + i * kLoadThreads * 16 : src, on);
+            }
+          }
+          next_slot();
         }
         pfx::cp_commit();
-      };
-      for (int t = 0; t <= nt; ++t) {
-        if (t < nt) {
-          if (t >= kKRing && ok) ok = mbar_wait(kempty + t % kKRing, (t / kKRing - 1) & 1, ERR_PFX_WAIT);
-          if (ok) load(k, s0 + F::kOffK + (t % kKRing) * F::kTileBytes, t);
-          if (t >= kVRing && ok) ok = mbar_wait(vempty + t % kVRing, (t / kVRing - 1) & 1, ERR_PFX_WAIT);
-          if (ok) load(v, s0 + F::kOffV + (t % kVRing) * F::kTileBytes, t);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-        }
-        if (t > 0) {  // the tile before has landed
-          if (t < nt) pfx::cp_wait<2>();
-          else pfx::cp_wait<0>();
-          arrive(kfull + (t - 1) % kKRing);
-          arrive(vfull + (t - 1) % kVRing);
+        if (t > 1) {  // two tiles may still be under way: tile t - 2 has landed
+          pfx::cp_wait<2>();
+          arrive(landed);
+          landed = landed + 1 == ring ? 0 : landed + 1;
         }
       }
       pfx::cp_wait<0>();
     } else {
       constexpr int kPieces = F::kRow / 16;
-      uint4 kr[F::kRaw], vr[F::kRaw];
+      // A thread's pieces: two neighbouring ones (a 32-byte sector) by a lane pair, and the rows of eight lanes chosen so
+      // that the pieces they store, 2 (4) columns of sixteen bytes apart, fall on eight different bank groups.
+      constexpr int kPairs = kPieces / 2;
+      static_assert(F::kRaw == 2 * kPairs, "two row blocks of sixteen a warp");
+      const int lr = F::kFmt == RB_KV_INT8 ? ((lane >> 1) & 1) | (((lane >> 3) & 1) << 1) | (((lane >> 2) & 1) << 2) | ((lane >> 4) << 3) : lane >> 1;
+      auto row_of = [&](int i) { return ((i / kPairs) * kLoadWarps + lw) * 16 + lr; };
+      auto piece_of = [&](int i) { return 2 * (i % kPairs) + (lane & 1); };
+      const void* par_src = keys ? p.pre.k_par : p.pre.v_par;
+      constexpr int kParBytes = F::kFmt == RB_KV_INT8 ? 2 : 4;
+      uint4 raw[F::kRaw];
       uint32_t par = 0u;
-      auto fetch = [&](const uint8_t* src, int t, uint4 (&raw)[F::kRaw]) {
-        const int64_t first = static_cast<int64_t>(t0 + t) * kTile;
-#pragma unroll
-        for (int i = 0; i < F::kRaw; ++i) {
-          const int x = i * kLoadThreads + lt;
-          raw[i] = make_uint4(0u, 0u, 0u, 0u);
-          if (first + x / kPieces < n) raw[i] = ldg_cg_128(src + first * F::kRow + x * 16);
+      const uint8_t* from = src + static_cast<int64_t>(t0) * kTile * F::kRow + lr * F::kRow + (lane & 1) * 16 + lw * 16 * F::kRow;
+      int64_t seen = n - static_cast<int64_t>(t0) * kTile;  // slots from the tile to fetch on
+      auto fetch = [&](int i) {  // piece i of a thread: row block i / kPairs of its warp, pieces 2 (i % kPairs) and the next
+        raw[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (row_of(i) < seen) raw[i] = ldg_cg_128(from + (i / kPairs) * (kLoadWarps * 16 * F::kRow) + (i % kPairs) * 32);
+      };
+      auto fetch_par = [&](int t) {  // thread: slot
+        const int64_t at = head + static_cast<int64_t>(t0 + t) * kTile + lt;
+        par = 0u;
+        if (lt < seen)
+          par = F::kFmt == RB_KV_INT8 ? static_cast<uint32_t>(__ldcg(reinterpret_cast<const unsigned short*>(par_src) + at))
+                                      : __ldcg(reinterpret_cast<const unsigned int*>(par_src) + at);
+        // registers hold one tile ahead, less than the way from HBM takes: the tiles behind it are called to L2
+        constexpr int kFar = 4;
+        const int64_t far = static_cast<int64_t>(t0 + t + kFar) * kTile;
+        if (t + kFar < nt && lt < 2) {
+          const int rows = static_cast<int>(min(n - far, int64_t(kTile)));
+          const uint8_t* what = lt == 0 ? src + far * F::kRow
+                                        : reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(static_cast<const uint8_t*>(par_src) + (head + far) * kParBytes) & ~uintptr_t(15));
+          const uint32_t bytes = lt == 0 ? rows * F::kRow : rows * kParBytes & ~15;
+          if (bytes) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(what), "r"(bytes) : "memory");
         }
       };
-      auto fetch_par = [&](int t) {  // threads 0..127: a key's, 128..255: a value's
-        const int64_t r = static_cast<int64_t>(t0 + t) * kTile + (lt & (kTile - 1));
-        const void* src = lt < kTile ? p.pre.k_par : p.pre.v_par;
-        par = 0u;
-        if (r < n)
-          par = F::kFmt == RB_KV_INT8 ? static_cast<uint32_t>(__ldcg(reinterpret_cast<const unsigned short*>(src) + head + r))
-                                      : __ldcg(reinterpret_cast<const unsigned int*>(src) + head + r);
-      };
-      auto store = [&](uint32_t dst, const uint4 (&raw)[F::kRaw]) {
+#pragma unroll
+      for (int i = 0; i < F::kRaw; ++i) fetch(i);
+      fetch_par(0);
+      for (int t = 0; t < nt; ++t) {
+        // The keys' parameters lie in a ring of four: tile t - 4's are free once QK(t - 2), which its group issued behind
+        // PV(t - 4), has released the keys' slot.
+        if (!free_slot(t)) break;
+        const uint32_t dst = base + slot * F::kTileBytes;
+        from += kTile * F::kRow;
+        seen = t + 1 < nt ? seen - kTile : 0;  // no fetch behind the last tile
 #pragma unroll
         for (int i = 0; i < F::kRaw; ++i) {
-          const int x = i * kLoadThreads + lt, r = x / kPieces, ch = x % kPieces;
+          const int r = row_of(i), ch = piece_of(i);
           const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
           if constexpr (F::kFmt == RB_KV_INT8) {
             uint32_t h[8];
@@ -291,242 +573,78 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attn_tc_kernel(const __gri
             }
           }
         }
-      };
-      auto store_par = [&](int t) {
-        float* dst = reinterpret_cast<float*>(smem + F::kOffPar + (t % kVRing) * F::kPar);
+        float* pd = reinterpret_cast<float*>(smem + (keys ? F::kOffPar + (t % kKParRing) * F::kPar : F::kOffVPar + slot * F::kPar));
         const float s = __uint_as_float(par << 16);
-        dst[lt] = s;
+        const int at = ((lt >> 1) & 3) * F::kParC + 2 * (lt >> 3) + (lt & 1);
+        pd[at] = s;
         if constexpr (F::kFmt == RB_KV_INT4)
-          dst[2 * kTile + lt] =
-              fmaf(8.f, s, p.bf16 ? __uint_as_float(par & 0xffff0000u) : __half2float(__ushort_as_half(static_cast<unsigned short>(par >> 16))));
-      };
-      fetch(k, 0, kr);
-      fetch(v, 0, vr);
-      fetch_par(0);
-      for (int t = 0; t < nt; ++t) {
-        if (t >= kKRing && ok) ok = mbar_wait(kempty + t % kKRing, (t / kKRing - 1) & 1, ERR_PFX_WAIT);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        store(s0 + F::kOffK + (t % kKRing) * F::kTileBytes, kr);
-        if (t + 1 < nt) fetch(k, t + 1, kr);
-        arrive(kfull + t % kKRing);
-        if (t >= kVRing && ok) ok = mbar_wait(vempty + t % kVRing, (t / kVRing - 1) & 1, ERR_PFX_WAIT);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        store_par(t);
-        store(s0 + F::kOffV + (t % kVRing) * F::kTileBytes, vr);
-        if (t + 1 < nt) {
-          fetch(v, t + 1, vr);
-          fetch_par(t + 1);
-        }
-        arrive(vfull + t % kVRing);
+          pd[F::kParN + at] = fmaf(8.f, s, p.bf16 ? __uint_as_float(par & 0xffff0000u) : __half2float(__ushort_as_half(static_cast<unsigned short>(par >> 16))));
+        // The fence in arrive waits for a thread's outstanding loads too: the next tile's are issued behind it.
+        arrive(slot);
+#pragma unroll
+        for (int i = 0; i < F::kRaw; ++i) fetch(i);
+        fetch_par(t + 1);
+        next_slot();
       }
     }
   } else {
-    // ---------------- softmax: group g takes the tiles t % 2 == g; thread = row ----------------
-    const int g = warp >> 2, quad = warp & 3, r = quad * 32 + lane, row = row0 + r;
+    // ---------------- softmax: group g takes the tiles t % 2 == g ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
+    const int g = warp >> 2, quad = warp & 3;
     const int rows = min(kTile, p.n_seqs * p.rep - row0);
-    const bool on = r < rows, busy = quad * 32 < rows;  // busy: the warp has a row of the batch
-    const uint32_t tq = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-    const uint32_t ts = tq + g * kTile, to = tq + (2 + g) * kTile;
-    float fr = fmaxf(fabsf(p.scale) * pfx::kLog2e, 1e-30f), qs = 0.f;
-    {
-      // the row of Q: group 0 writes it to shared memory, both keep its factor and sum
+    float* rowf = reinterpret_cast<float*>(smem + F::kOffRow);
+    float* qsum = rowf + kTile;
+    if (g == 0) {
+      // group 0 brings the queries: thread = lane, its row's loads all at once
+      const int r = lane * 4 + quad, lane_row = quad * 32 + lane, row = row0 + r;
+      const bool on = r < rows;
       const int b = on ? row / p.rep : 0, j = on ? row % p.rep : 0;
       const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.q) + b * p.ldq + static_cast<int64_t>(kv * p.rep + j) * F::kHd);
+      uint4 q[F::kHd / 8];
+#pragma unroll
+      for (int i = 0; i < F::kHd / 8; ++i) q[i] = on ? ldg_cg_128(src + i) : make_uint4(0u, 0u, 0u, 0u);
       const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
-      float down = 1.f;
+      float f = fmaxf(fabsf(p.scale) * pfx::kLog2e, 1e-30f), sum = 0.f, down = 1.f;
       if constexpr (!F::kPlain) {
         uint32_t top = 0u;
-#pragma unroll 4
-        for (int i = 0; i < F::kHd / 8; ++i) {
-          const uint4 x = on ? __ldcg(src + i) : make_uint4(0u, 0u, 0u, 0u);
-          top = __vmaxu2(top, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
-        }
+#pragma unroll
+        for (int i = 0; i < F::kHd / 8; ++i)
+          top = __vmaxu2(top, __vmaxu2(__vmaxu2(q[i].x & 0x7fff7fffu, q[i].y & 0x7fff7fffu), __vmaxu2(q[i].z & 0x7fff7fffu, q[i].w & 0x7fff7fffu)));
         const uint32_t t16 = max(top & 0xffffu, top >> 16);
         const uint32_t ex = __float_as_uint(p.bf16 ? __uint_as_float(t16 << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(t16)))) >> 23;
         const uint32_t exc = ex < 30u ? 30u : (ex > 220u ? 220u : ex);
         down = __uint_as_float((254u - exc) << 23);
-        fr *= __uint_as_float(exc << 23);
+        f *= __uint_as_float(exc << 23);
       }
-#pragma unroll 4
+#pragma unroll
       for (int i = 0; i < F::kHd / 8; ++i) {
-        const uint4 x = on ? __ldcg(src + i) : make_uint4(0u, 0u, 0u, 0u);
-        uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if constexpr (!F::kPlain) {
-            float2 f;
-            if (p.bf16) f = make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u));
-            else f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-            w[e] = pfx::pack2<false>(f.x * down, f.y * down);
+            float2 v;
+            if (p.bf16) v = make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u));
+            else v = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+            w[e] = pfx::pack2<false>(v.x * down, v.y * down);
             if constexpr (F::kFmt == RB_KV_INT4) {
-              f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-              qs += f.x + f.y;
+              v = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+              sum += v.x + v.y;
             }
           }
           w[e] ^= flip;
         }
-        if (g == 0) sts128(s0 + piece_at(r, i), w[0], w[1], w[2], w[3]);
+        sts128(s0 + piece_at(lane_row, i), w[0], w[1], w[2], w[3]);
       }
-      if (flip) qs = -qs;
-      if (g == 0) {
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(qfull);
-      }
+      rowf[lane_row] = f;
+      qsum[lane_row] = flip ? -sum : sum;
+      fence_proxy_async_smem();
     }
-    float ref = -INFINITY, ve = F::kPlain ? 0.f : pfx::kLowestE;
-    float2 l2 = make_float2(0.f, 0.f), w2 = make_float2(0.f, 0.f);
-    bool ok = true;
-    for (int t = g; t < nt && ok; t += 2) {
-      ok = mbar_wait(sfull + g, (t >> 1) & 1, ERR_PFX_WAIT);
-      if (!F::kPlain && ok) ok = mbar_wait(vfull + t % kVRing, (t / kVRing) & 1, ERR_PFX_WAIT);  // its parameters
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      mm4::tc_fence_after();
-      const uint32_t par = s0 + F::kOffPar + (t % kVRing) * F::kPar;
-      const int left = static_cast<int>(min(n - static_cast<int64_t>(t0 + t) * kTile, int64_t(kTile)));
-      if (busy) {
-        // 32 columns of the row's scores from column c0: scaled by the keys' scales, -inf beyond the prefix
-        auto scores = [&](int c0, float2 (&x)[16]) {
-          float f[32];
-          tmem_ld32(ts + c0, f);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) x[i] = make_float2(f[2 * i], f[2 * i + 1]);
-          if constexpr (!F::kPlain) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float4 s = lds128f(par + (c0 + 4 * i) * 4);
-              if constexpr (F::kFmt == RB_KV_INT4) {
-                const float4 m = lds128f(par + (2 * kTile + c0 + 4 * i) * 4);
-                const float2 q2 = make_float2(qs, qs);
-                x[2 * i] = fma2(x[2 * i], make_float2(s.x, s.y), mul2(make_float2(m.x, m.y), q2));
-                x[2 * i + 1] = fma2(x[2 * i + 1], make_float2(s.z, s.w), mul2(make_float2(m.z, m.w), q2));
-              } else {
-                x[2 * i] = mul2(x[2 * i], make_float2(s.x, s.y));
-                x[2 * i + 1] = mul2(x[2 * i + 1], make_float2(s.z, s.w));
-              }
-            }
-          }
-          if (c0 + 32 > left) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              if (c0 + 2 * i >= left) x[i].x = -INFINITY;
-              if (c0 + 2 * i + 1 >= left) x[i].y = -INFINITY;
-            }
-          }
-        };
-        float top = -INFINITY;
-#pragma unroll 1
-        for (int c0 = 0; c0 < kTile; c0 += 32) {
-          float2 x[16];
-          scores(c0, x);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) top = fmaxf(top, fmaxf(x[i].x, x[i].y));
-        }
-        float ven = ve;
-        if constexpr (!F::kPlain) {
-          const float4 s = lds128f(par + (kTile + 4 * lane) * 4);
-          auto bits = [](float f) { return f == f ? __float_as_uint(f) : 0u; };  // a NaN shows by itself
-          const uint32_t hi = __reduce_max_sync(0xffffffffu, max(max(bits(s.x), bits(s.y)), max(bits(s.z), bits(s.w))));
-          ven = fmaxf(ve, fminf(fmaxf(static_cast<float>(static_cast<int>(hi >> 23) - 127), pfx::kLowestE), pfx::kHighestE));
-        }
-        if (__any_sync(0xffffffffu, top * fr > ref + pfx::kSlack || ven > ve)) {
-          const float nr = fmaxf(ref, top * fr);
-          const float f = ref == -INFINITY ? 0.f : ex2((ref - nr) + (ve - ven));
-          ref = nr;
-          ve = ven;
-          l2 = mul2(l2, make_float2(f, f));
-          w2 = mul2(w2, make_float2(f, f));
-          if (t >= 2) {  // the group's O holds something: all of it is there, and the next PV waits for this tile's P
-            ok = __all_sync(0xffffffffu, mbar_wait(pvdone + g, ((t >> 1) - 1) & 1, ERR_PFX_WAIT));
-            mm4::tc_fence_after();
-#pragma unroll 1
-            for (int c0 = 0; c0 < F::kHd && ok; c0 += 16) {
-              uint32_t v[16];
-              asm volatile(
-                  "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
-                  "[%16];\n\ttcgen05.wait::ld.sync.aligned;"
-                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-                    "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-                  : "r"(to + c0)
-                  : "memory");
-#pragma unroll
-              for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-              tmem_st16(to + c0, v);
-            }
-          }
-        }
-        const float base = ref == -INFINITY ? 0.f : -(ref + ve);
-        const float2 f2 = make_float2(fr, fr), b2 = make_float2(base, base);
-#pragma unroll 1
-        for (int c0 = 0; c0 < kTile && ok; c0 += 32) {
-          float2 x[16];
-          scores(c0, x);
-          uint32_t hi[16], lo[F::kFmt == RB_KV_INT4 ? 16 : 1];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float2 pr = fma2(x[i], f2, b2);
-            pr.x = ex2(pr.x);
-            pr.y = ex2(pr.y);
-            l2 = add2(l2, pr);
-            x[i] = pr;
-          }
-          if constexpr (!F::kPlain) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float4 s = lds128f(par + (kTile + c0 + 4 * i) * 4);
-              if constexpr (F::kFmt == RB_KV_INT4) {
-                const float4 m = lds128f(par + (3 * kTile + c0 + 4 * i) * 4);
-                w2 = fma2(x[2 * i], make_float2(m.x, m.y), w2);
-                w2 = fma2(x[2 * i + 1], make_float2(m.z, m.w), w2);
-              }
-              x[2 * i] = mul2(x[2 * i], make_float2(s.x, s.y));
-              x[2 * i + 1] = mul2(x[2 * i + 1], make_float2(s.z, s.w));
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            hi[i] = pfx::pack2<F::kBf16>(x[i].x, x[i].y);
-            if constexpr (F::kFmt == RB_KV_INT4) {  // what the rounding of p s left, as a second term
-              const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
-              lo[i] = pfx::pack2<false>(x[i].x - h.x, x[i].y - h.y);
-            }
-          }
-          tmem_st16(ts + c0, hi);
-          if constexpr (F::kFmt == RB_KV_INT4) tmem_st16(ts + c0 + 16, lo);
-        }
-        tmem_wait_st();
-      }
-      if (!ok) break;
-      mm4::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(pfull + g);
-    }
-    // ---- the group's partial ----
-    const int mine = nt > g ? (nt - g + 1) / 2 : 0;  // tiles of this group
-    if (mine && ok) ok = __all_sync(0xffffffffu, mbar_wait(pvdone + g, (mine - 1) & 1, ERR_PFX_WAIT));
-    mm4::tc_fence_after();
-    const int64_t slot = (static_cast<int64_t>(lane_i) * p.max_np + sp) * 2 + g;
-    const float l = l2.x + l2.y, w = w2.x + w2.y;
-    if (on) p.rl[slot * kTile + r] = make_float2(!mine || (ref == -INFINITY && l == 0.f) ? -INFINITY : (ref == -INFINITY ? 0.f : ref + ve), l);
-    if (mine && busy && ok) {
-      float4* dst = reinterpret_cast<float4*>(p.o + (slot * kTile + r) * F::kHd);
-#pragma unroll 1
-      for (int c0 = 0; c0 < F::kHd; c0 += 32) {
-        float f[32];
-        tmem_ld32(to + c0, f);
-        if (on) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) dst[c0 / 4 + i] = make_float4(f[4 * i] + w, f[4 * i + 1] + w, f[4 * i + 2] + w, f[4 * i + 3] + w);
-        }
-      }
-    }
-    mm4::tc_fence_before();
+    named_bar_sync(kBarSoft, 256);
+    if (rows <= kTile / 2) run_softmax<F, 1>(p, s0, smem, tmem, g, quad, lane, nt, n - static_cast<int64_t>(t0) * kTile, rows, lane_i * p.max_np + sp);
+    else run_softmax<F, 2>(p, s0, smem, tmem, g, quad, lane, nt, n - static_cast<int64_t>(t0) * kTile, rows, lane_i * p.max_np + sp);
   }
   __syncthreads();
-  if (warp == kMmaWarp) {
+  if (warp == kFirstK) {
     mm4::tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
   }

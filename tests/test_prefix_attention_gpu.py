@@ -202,6 +202,7 @@ def test_a_nan_in_a_visible_row_shows(fmt):
     (43, 6, 2, 128, 1000, None),
     (64, 16, 2, 64, 2500, [i % 3 for i in range(64)]),
     (150, 2, 1, 128, 6000, None),
+    (100, 12, 4, 64, 12000, None),      # three row tiles of four heads: splits of many tiles
 ])
 def test_tcgen05_kernel_against_64_bits(B, nq, nkv, hd, P, lens, fmt, dtype):
     """The tcgen05 kernel at sizes that the choice by rows would leave to the warp-level one as well: single rows and

@@ -293,7 +293,7 @@ struct Item {
 // slots of a stage. Three CTAs an SM: one's loads and barriers hide behind the others' products.
 template <typename F>
 struct Tile {
-  static constexpr int kBlock = F::kPlain ? 16 : 32;          // slots of one softmax step
+  static constexpr int kBlock = 16;                           // slots of one softmax step
   static constexpr int kNt = kBlock / 8;
   static constexpr int kMergeRow = (F::kNv * 33) * 16;        // a warp's 16-row accumulator tile, padded
   static constexpr int kStages = F::kStage <= 20 * 1024 ? 3 : 2;
@@ -370,16 +370,9 @@ __device__ __forceinline__ void run_item(const Params& p, const Item it, const i
   static_assert(F::kPlain || F::kTile == kThreads, "one thread a slot's parameters");
 
   __syncthreads();  // the previous item's merge has been read
-#pragma unroll 1
-  for (int i = 0; i < T::kStages - 1; ++i) {
-    if (it.t0 + i < it.t1) {
-      load_rows(it.t0 + i);
-      load_par(it.t0 + i);
-      store_par();
-      ld_slot = next(ld_slot);
-    }
-    cp_commit();
-  }
+  load_rows(it.t0);
+  cp_commit();
+  load_par(it.t0);
 
   // ---- the warp's queries (rows g, g + 8 of its 16) as A fragments, straight from global memory ----
   uint32_t qa[F::kKs][4];
@@ -442,6 +435,18 @@ __device__ __forceinline__ void run_item(const Params& p, const Item it, const i
     }
     fr[x] = f;
     qs[x] = sum;
+  }
+  store_par();
+  ld_slot = next(ld_slot);
+#pragma unroll 1
+  for (int i = 1; i < T::kStages - 1; ++i) {
+    if (it.t0 + i < it.t1) {
+      load_rows(it.t0 + i);
+      load_par(it.t0 + i);
+      store_par();
+      ld_slot = next(ld_slot);
+    }
+    cp_commit();
   }
 
   float o[F::kNv][4], l[2], w[2], ref[2];
@@ -523,7 +528,7 @@ __device__ __forceinline__ void run_item(const Params& p, const Item it, const i
       if constexpr (!F::kPlain) {
         // the block's largest value scale (NaN left out: it shows by itself): its exponent goes into the reference,
         // so that the 16-bit p s stay within fp16's range whatever the size of the values
-        const float vs = __uint_as_float(lds32(pt + (F::kTile + b0 + lane) * 4));
+        const float vs = __uint_as_float(lds32(pt + (F::kTile + b0 + (lane & (T::kBlock - 1))) * 4));
         const uint32_t hi = __reduce_max_sync(0xffffffffu, vs == vs ? __float_as_uint(vs) : 0u);
         ven = fmaxf(ve, fminf(fmaxf(static_cast<float>(static_cast<int>(hi >> 23) - 127), kLowestE), kHighestE));
         raise |= ven > ve;
@@ -661,38 +666,36 @@ struct Plan {
 
 template <int kTile>
 __device__ __forceinline__ Plan make_plan(const Params& p, int grid) {
-  __shared__ unsigned long long sum_s;
-  __shared__ int most_s;
-  if (threadIdx.x == 0) sum_s = 0, most_s = 0;
-  const int64_t np_raw = p.pre.k ? *p.pre.len : 0;
-  __syncthreads();
+  // every warp by itself: no barrier, and the loads of all lengths go out together
+  const int lane = threadIdx.x & 31;
+  const int64_t np_raw = p.pre.k ? __ldg(p.pre.len) : 0;
+  int sum = 0, most = 0;
   if (p.own.k) {
-    unsigned long long sum = 0;
-    int most = 0;
-    for (int b = threadIdx.x; b < p.n_seqs; b += blockDim.x) {
-      const int64_t n = p.own.len[b];
+#pragma unroll 2
+    for (int b = lane; b < p.n_seqs; b += 32) {
+      const int64_t n = __ldg(p.own.len + b);
       if (n <= 0 || n > p.own.cache_len) continue;
       const int t = static_cast<int>((n + kTile - 1) / kTile);
-      sum += t + 2;  // an item's start and end cost about two stages
-      most = most > t ? most : t;
+      sum += min(t + 2, 1 << 20);  // an item's start and end cost about two stages
+      most = max(most, t);
     }
-    if (sum) atomicAdd(&sum_s, sum), atomicMax(&most_s, most);
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    most = __reduce_max_sync(0xffffffffu, most);
   }
-  __syncthreads();
   Plan pl;
   pl.prefix_ok = np_raw >= 0 && np_raw <= p.pre.cache_len;
   const int64_t n = pl.prefix_ok ? np_raw : 0;
   const int tiles = static_cast<int>((n + kTile - 1) / kTile), lanes = p.n_kv * p.tiles_m;
-  const double own = static_cast<double>(sum_s) * p.n_kv, pre = static_cast<double>(tiles) * lanes;
-  int g_own = own > 0 ? static_cast<int>(grid * (own / (own + pre)) + 0.5) : 0;
-  if (own > 0 && g_own < 1) g_own = 1;
+  const float own = static_cast<float>(sum) * static_cast<float>(p.n_kv), pre = static_cast<float>(tiles) * static_cast<float>(lanes);
+  int g_own = sum > 0 ? static_cast<int>(__fdividef(own, own + pre) * static_cast<float>(grid) + 0.5f) : 0;
+  if (sum > 0 && g_own < 1) g_own = 1;
   if (tiles > 0 && g_own >= grid) g_own = grid - 1;
   pl.np = tiles ? max(1, min(min((grid - g_own) / lanes, tiles), p.max_np)) : 0;
   pl.pt = pl.np ? (tiles + pl.np - 1) / pl.np : 0;
   pl.np = pl.pt ? (tiles + pl.pt - 1) / pl.pt : 0;
-  pl.ns = most_s ? min(p.max_ns, (most_s + 3) / 4) : 0;  // at least four stages a split
-  pl.ot = pl.ns ? (most_s + pl.ns - 1) / pl.ns : 0;
-  pl.ns = pl.ot ? (most_s + pl.ot - 1) / pl.ot : 0;
+  pl.ns = most ? min(p.max_ns, (most + 3) / 4) : 0;  // at least four stages a split
+  pl.ot = pl.ns ? (most + pl.ns - 1) / pl.ns : 0;
+  pl.ns = pl.ot ? (most + pl.ot - 1) / pl.ot : 0;
   pl.prefix_items = lanes * pl.np;
   pl.own_items = p.n_seqs * p.n_kv * pl.ns;
   return pl;

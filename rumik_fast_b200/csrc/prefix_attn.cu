@@ -133,7 +133,7 @@ struct Fmt {
   static constexpr int kNv = kHd / 8;            // n8 tiles of p v
   static constexpr int kRow = kPlain ? 2 * kHd : (kFmt == RB_KV_INT8 ? kHd : kHd / 2);  // bytes of a row
   static constexpr int kChunks = kRow / 16;
-  static constexpr int kTile = kPlain ? 64 : 128;  // slots of a stage
+  static constexpr int kTile = 64;                 // slots of a stage
   static constexpr int kSide = kTile * kRow;       // bytes of a stage's keys (or values)
   static constexpr int kPar = kPlain ? 0 : kTile * 4 * (kFmt == RB_KV_INT4 ? 4 : 2);  // fp32 s (and m) of keys, values
   static constexpr int kStage = 2 * kSide + kPar;
@@ -296,7 +296,7 @@ struct Tile {
   static constexpr int kBlock = 16;                           // slots of one softmax step
   static constexpr int kNt = kBlock / 8;
   static constexpr int kMergeRow = (F::kNv * 33) * 16;        // a warp's 16-row accumulator tile, padded
-  static constexpr int kStages = F::kStage <= 20 * 1024 ? 3 : 2;
+  static constexpr int kStages = F::kStage <= 11 * 1024 ? 5 : (F::kStage <= 20 * 1024 ? 3 : 2);
   static constexpr int kRing = kStages * F::kStage;
   static constexpr int kMerge = kWarps * kMergeRow;
   static constexpr int kOffRl = kRing > kMerge ? kRing : kMerge;  // the merge reuses the ring; (R, l) [4][16]
@@ -339,35 +339,28 @@ __device__ __forceinline__ void run_item(const Params& p, const Item it, const i
   };
   // A stage's row parameters: loaded into registers ahead, stored as fp32 behind its rows (2-byte scales of an odd
   // cache length have no alignment that an asynchronous copy takes).
-  uint32_t par[2] = {0u, 0u};
+  uint32_t par = 0u;  // threads 0 .. 63: a key's, the others: a value's
   auto load_par = [&](int t) {
     if constexpr (!F::kPlain) {
-      const int64_t r = static_cast<int64_t>(t) * F::kTile + tid;
-      const bool on = r < it.n;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const void* src = s ? it.v_par : it.k_par;
-        par[s] = 0u;
-        if (on) par[s] = F::kFmt == RB_KV_INT8 ? static_cast<uint32_t>(__ldcg(reinterpret_cast<const unsigned short*>(src) + it.par0 + r))
-                                               : __ldcg(reinterpret_cast<const unsigned int*>(src) + it.par0 + r);
-      }
+      const int64_t r = static_cast<int64_t>(t) * F::kTile + (tid & (F::kTile - 1));
+      const void* src = tid < F::kTile ? it.k_par : it.v_par;
+      par = 0u;
+      if (r < it.n) par = F::kFmt == RB_KV_INT8 ? static_cast<uint32_t>(__ldcg(reinterpret_cast<const unsigned short*>(src) + it.par0 + r))
+                                                : __ldcg(reinterpret_cast<const unsigned int*>(src) + it.par0 + r);
     }
   };
   auto store_par = [&]() {  // behind the rows of the stage last loaded
     if constexpr (!F::kPlain) {
       float* dst = reinterpret_cast<float*>(smem + ld_slot + 2 * F::kSide);
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const float sc = __uint_as_float(par[s] << 16);
-        dst[s * F::kTile + tid] = sc;
-        if constexpr (F::kFmt == RB_KV_INT4)  // codes enter as c - 8: m + 8 s stands for the middle of the row's range
-          dst[(2 + s) * F::kTile + tid] = fmaf(
-              8.f, sc, p.bf16 ? __uint_as_float(par[s] & 0xffff0000u) : __half2float(__ushort_as_half(static_cast<unsigned short>(par[s] >> 16))));
-      }
+      const float sc = __uint_as_float(par << 16);
+      dst[tid] = sc;
+      if constexpr (F::kFmt == RB_KV_INT4)  // codes enter as c - 8: m + 8 s stands for the middle of the row's range
+        dst[2 * F::kTile + tid] =
+            fmaf(8.f, sc, p.bf16 ? __uint_as_float(par & 0xffff0000u) : __half2float(__ushort_as_half(static_cast<unsigned short>(par >> 16))));
     }
   };
   auto next = [](uint32_t slot) { return slot + F::kStage == T::kRing ? 0u : slot + F::kStage; };
-  static_assert(F::kPlain || F::kTile == kThreads, "one thread a slot's parameters");
+  static_assert(2 * F::kTile == kThreads, "a thread for each slot's parameters of keys and of values");
 
   __syncthreads();  // the previous item's merge has been read
   load_rows(it.t0);
@@ -687,17 +680,18 @@ __device__ __forceinline__ Plan make_plan(const Params& p, int grid) {
   const int64_t n = pl.prefix_ok ? np_raw : 0;
   const int tiles = static_cast<int>((n + kTile - 1) / kTile), lanes = p.n_kv * p.tiles_m;
   const float own = static_cast<float>(sum) * static_cast<float>(p.n_kv), pre = static_cast<float>(tiles) * static_cast<float>(lanes);
+  pl.ns = most ? min(p.max_ns, (most + 3) / 4) : 0;  // at least four stages a split
+  pl.ot = pl.ns ? (most + pl.ns - 1) / pl.ns : 0;
+  pl.ns = pl.ot ? (most + pl.ot - 1) / pl.ot : 0;
+  pl.own_items = p.n_seqs * p.n_kv * pl.ns;
+  // the own items' share of the CTAs, at most one each; the rest for the prefix
   int g_own = sum > 0 ? static_cast<int>(__fdividef(own, own + pre) * static_cast<float>(grid) + 0.5f) : 0;
-  if (sum > 0 && g_own < 1) g_own = 1;
+  g_own = min(max(g_own, sum > 0 ? 1 : 0), pl.own_items);
   if (tiles > 0 && g_own >= grid) g_own = grid - 1;
   pl.np = tiles ? max(1, min(min((grid - g_own) / lanes, tiles), p.max_np)) : 0;
   pl.pt = pl.np ? (tiles + pl.np - 1) / pl.np : 0;
   pl.np = pl.pt ? (tiles + pl.pt - 1) / pl.pt : 0;
-  pl.ns = most ? min(p.max_ns, (most + 3) / 4) : 0;  // at least four stages a split
-  pl.ot = pl.ns ? (most + pl.ns - 1) / pl.ns : 0;
-  pl.ns = pl.ot ? (most + pl.ot - 1) / pl.ot : 0;
   pl.prefix_items = lanes * pl.np;
-  pl.own_items = p.n_seqs * p.n_kv * pl.ns;
   return pl;
 }
 

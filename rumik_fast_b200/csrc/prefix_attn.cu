@@ -24,7 +24,11 @@ namespace pfx {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kCtasPerSm = 3;
+// CTAs of an SM, by registers: codes of 128 columns run two, with stages of 128 slots and steps of 32; everything else
+// three, with 64 and 16. (int8, 16 sequences of 4,096 slots: 44 us so, 48 with three CTAs of 64-slot stages; 64 sequences
+// of 700: 20 against 26.)
+constexpr bool wide_steps(int fmt, int hd) { return fmt != RB_KV_PLAIN && hd == 128; }
+constexpr int ctas_per_sm(int fmt, int hd) { return wide_steps(fmt, hd) ? 2 : 3; }
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.f;     // a row's reference is raised when a score exceeds it by this (log2)
 constexpr float kLowestE = -90.f; // exponent range of the value scales folded into the reference
@@ -133,7 +137,8 @@ struct Fmt {
   static constexpr int kNv = kHd / 8;            // n8 tiles of p v
   static constexpr int kRow = kPlain ? 2 * kHd : (kFmt == RB_KV_INT8 ? kHd : kHd / 2);  // bytes of a row
   static constexpr int kChunks = kRow / 16;
-  static constexpr int kTile = 64;                 // slots of a stage
+  static constexpr int kCtas = ctas_per_sm(kFmt, kHd);
+  static constexpr int kTile = wide_steps(kFmt, kHd) ? 128 : 64;  // slots of a stage
   static constexpr int kSide = kTile * kRow;       // bytes of a stage's keys (or values)
   static constexpr int kPar = kPlain ? 0 : kTile * 4 * (kFmt == RB_KV_INT4 ? 4 : 2);  // fp32 s (and m) of keys, values
   static constexpr int kStage = 2 * kSide + kPar;
@@ -290,13 +295,15 @@ struct Item {
 };
 
 // A CTA's four warps: each takes 16 query rows; wm of them stand along the rows (1, 2 or 4), the other 4 / wm along the
-// slots of a stage. Three CTAs an SM: one's loads and barriers hide behind the others' products.
+// slots of a stage. Two or three CTAs an SM: one's loads and barriers hide behind the others' products.
 template <typename F>
 struct Tile {
-  static constexpr int kBlock = 16;                           // slots of one softmax step
+  static constexpr int kBlock = wide_steps(F::kFmt, F::kHd) ? 32 : 16;  // slots of one softmax step
   static constexpr int kNt = kBlock / 8;
+  static_assert(F::kTile / kWarps % kBlock == 0, "a warp's slots of a stage are whole steps");
   static constexpr int kMergeRow = (F::kNv * 33) * 16;        // a warp's 16-row accumulator tile, padded
-  static constexpr int kStages = F::kStage <= 11 * 1024 ? 5 : (F::kStage <= 20 * 1024 ? 3 : 2);
+  static constexpr int kFit = (227 * 1024 / F::kCtas - 2048) / F::kStage;  // of a CTA's share of the shared memory
+  static constexpr int kStages = kFit < 2 ? 2 : (kFit > 5 ? 5 : kFit);
   static constexpr int kRing = kStages * F::kStage;
   static constexpr int kMerge = kWarps * kMergeRow;
   static constexpr int kOffRl = kRing > kMerge ? kRing : kMerge;  // the merge reuses the ring; (R, l) [4][16]
@@ -339,28 +346,36 @@ __device__ __forceinline__ void run_item(const Params& p, const Item it, const i
   };
   // A stage's row parameters: loaded into registers ahead, stored as fp32 behind its rows (2-byte scales of an odd
   // cache length have no alignment that an asynchronous copy takes).
-  uint32_t par = 0u;  // threads 0 .. 63: a key's, the others: a value's
+  constexpr int kWords = 2 * F::kTile / kThreads;  // a thread's: the keys' parameters first, then the values'
+  uint32_t par[kWords];
   auto load_par = [&](int t) {
     if constexpr (!F::kPlain) {
-      const int64_t r = static_cast<int64_t>(t) * F::kTile + (tid & (F::kTile - 1));
-      const void* src = tid < F::kTile ? it.k_par : it.v_par;
-      par = 0u;
-      if (r < it.n) par = F::kFmt == RB_KV_INT8 ? static_cast<uint32_t>(__ldcg(reinterpret_cast<const unsigned short*>(src) + it.par0 + r))
-                                                : __ldcg(reinterpret_cast<const unsigned int*>(src) + it.par0 + r);
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) {
+        const int x = i * kThreads + tid;
+        const int64_t r = static_cast<int64_t>(t) * F::kTile + (x & (F::kTile - 1));
+        const void* src = x < F::kTile ? it.k_par : it.v_par;
+        par[i] = 0u;
+        if (r < it.n) par[i] = F::kFmt == RB_KV_INT8 ? static_cast<uint32_t>(__ldcg(reinterpret_cast<const unsigned short*>(src) + it.par0 + r))
+                                                     : __ldcg(reinterpret_cast<const unsigned int*>(src) + it.par0 + r);
+      }
     }
   };
   auto store_par = [&]() {  // behind the rows of the stage last loaded
     if constexpr (!F::kPlain) {
       float* dst = reinterpret_cast<float*>(smem + ld_slot + 2 * F::kSide);
-      const float sc = __uint_as_float(par << 16);
-      dst[tid] = sc;
-      if constexpr (F::kFmt == RB_KV_INT4)  // codes enter as c - 8: m + 8 s stands for the middle of the row's range
-        dst[2 * F::kTile + tid] =
-            fmaf(8.f, sc, p.bf16 ? __uint_as_float(par & 0xffff0000u) : __half2float(__ushort_as_half(static_cast<unsigned short>(par >> 16))));
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) {
+        const int x = i * kThreads + tid;
+        const float sc = __uint_as_float(par[i] << 16);
+        dst[x] = sc;
+        if constexpr (F::kFmt == RB_KV_INT4)  // codes enter as c - 8: m + 8 s stands for the middle of the row's range
+          dst[2 * F::kTile + x] =
+              fmaf(8.f, sc, p.bf16 ? __uint_as_float(par[i] & 0xffff0000u) : __half2float(__ushort_as_half(static_cast<unsigned short>(par[i] >> 16))));
+      }
     }
   };
   auto next = [](uint32_t slot) { return slot + F::kStage == T::kRing ? 0u : slot + F::kStage; };
-  static_assert(2 * F::kTile == kThreads, "a thread for each slot's parameters of keys and of values");
 
   __syncthreads();  // the previous item's merge has been read
   load_rows(it.t0);
@@ -387,7 +402,7 @@ __device__ __forceinline__ void run_item(const Params& p, const Item it, const i
     const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
     float f = fmaxf(fabsf(p.scale) * kLog2e, 1e-30f);
     float sum = 0.f;
-    if constexpr (!F::kPlain) {
+    if (!F::kPlain && p.bf16) {
       // fp16 queries for the codes' product: scaled by a power of two so that the row's largest is in [1, 2) - exact
       // but for elements 2^-24 below it
       uint32_t top = 0u;
@@ -398,7 +413,7 @@ __device__ __forceinline__ void run_item(const Params& p, const Item it, const i
       top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const uint32_t t16 = max(top & 0xffffu, top >> 16);
-      const uint32_t ex = __float_as_uint(p.bf16 ? __uint_as_float(t16 << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(t16)))) >> 23;
+      const uint32_t ex = t16 >> 7;  // the exponent of a bf16
       const uint32_t exc = ex < 30u ? 30u : (ex > 220u ? 220u : ex);
       const float down = __uint_as_float((254u - exc) << 23);
       f *= __uint_as_float(exc << 23);
@@ -407,24 +422,23 @@ __device__ __forceinline__ void run_item(const Params& p, const Item it, const i
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
           const uint32_t u = qa[ks][2 * q + x];
-          float2 v;
-          if (p.bf16) v = make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
-          else v = __half22float2(*reinterpret_cast<const __half2*>(&u));
-          const uint32_t h = pack2<false>(v.x * down, v.y * down);
-          if constexpr (F::kFmt == RB_KV_INT4) {
-            const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&h));
-            sum += w.x + w.y;
-          }
-          qa[ks][2 * q + x] = h ^ flip;
+          qa[ks][2 * q + x] = pack2<false>(__uint_as_float(u << 16) * down, __uint_as_float(u & 0xffff0000u) * down);
         }
-      if constexpr (F::kFmt == RB_KV_INT4) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        if (flip) sum = -sum;
-      }
-    } else {
+    }
+    if (flip) {
 #pragma unroll
       for (int ks = 0; ks < F::kKs; ++ks) qa[ks][x] ^= flip, qa[ks][2 + x] ^= flip;
+    }
+    if constexpr (F::kFmt == RB_KV_INT4) {
+#pragma unroll
+      for (int ks = 0; ks < F::kKs; ++ks)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&qa[ks][2 * q + x]));
+          sum += v.x + v.y;
+        }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
     }
     fr[x] = f;
     qs[x] = sum;
@@ -536,7 +550,7 @@ __device__ __forceinline__ void run_item(const Params& p, const Item it, const i
           const float f = ref[x] == -INFINITY ? 0.f : ex2((ref[x] - nr) + (ve - ven));
           ref[x] = nr;
           l[x] *= f;
-          w[x] *= f;
+          if constexpr (F::kFmt == RB_KV_INT4) w[x] *= f;
 #pragma unroll
           for (int u = 0; u < F::kNv; ++u) o[u][2 * x] *= f, o[u][2 * x + 1] *= f;
         }
@@ -617,7 +631,8 @@ __device__ __forceinline__ void run_item(const Params& p, const Item it, const i
 #pragma unroll
     for (int u = 0; u < F::kNv; ++u)
       *reinterpret_cast<float4*>(dst + (u * 33 + lane) * 16) =
-          make_float4((o[u][0] + w[0]) * f[0], (o[u][1] + w[0]) * f[0], (o[u][2] + w[1]) * f[1], (o[u][3] + w[1]) * f[1]);
+          F::kFmt == RB_KV_INT4 ? make_float4((o[u][0] + w[0]) * f[0], (o[u][1] + w[0]) * f[0], (o[u][2] + w[1]) * f[1], (o[u][3] + w[1]) * f[1])
+                                : make_float4(o[u][0] * f[0], o[u][1] * f[0], o[u][2] * f[1], o[u][3] * f[1]);
   }
   __syncthreads();
 #pragma unroll 2
@@ -696,7 +711,7 @@ __device__ __forceinline__ Plan make_plan(const Params& p, int grid) {
 }
 
 template <typename F>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) prefix_attn_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, F::kCtas) prefix_attn_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
   griddep_wait();
   griddep_launch_dependents();

@@ -673,13 +673,13 @@ inline Layout layout_of(const rb_prefix_attn_args* a, int num_sms, bool tc) {
   const int rep = a->n_q_heads / c->n_kv_heads;
   const int64_t rows = a->n_seqs * rep;
   Layout L = {};
-  L.grid = kCtasPerSm * num_sms;
+  L.grid = ctas_per_sm(c->fmt, c->head_dim) * num_sms;
   L.wm = warps_m(rows);
   L.parts = tc ? 2 : 1;
   L.tile_rows = tc ? pfxt::kTile : 16 * L.wm;
   L.tiles_m = static_cast<int>((rows + L.tile_rows - 1) / L.tile_rows);
   const int64_t lanes = static_cast<int64_t>(c->n_kv_heads) * L.tiles_m, heads = a->n_seqs * c->n_kv_heads;
-  // the warp-level kernel deals its items to kCtasPerSm CTAs an SM, the tcgen05 kernel has one CTA an item and SM
+  // the warp-level kernel deals its items to two or three CTAs an SM, the tcgen05 kernel has one CTA an item and SM
   L.max_np = a->prefix ? static_cast<int>(std::max<int64_t>(1, (tc ? num_sms : L.grid) / std::max<int64_t>(lanes, 1))) : 0;
   L.max_ns = a->own ? static_cast<int>(std::max<int64_t>(1, L.grid / std::max<int64_t>(heads, 1))) : 0;
   L.pre_slots = lanes * L.max_np * L.parts * L.tile_rows;
@@ -707,7 +707,7 @@ int launch_format(const Params& p, const Layout& L, bool tc, int flags, cudaStre
   using F = Fmt<kHd, kFmt, kBf16>;
   using T = pfxt::Fmt<kHd, kFmt, kBf16>;
   constexpr int smem = Tile<F>::kSmem;
-  static_assert((smem + 1024) * kCtasPerSm <= 227 * 1024, "CTAs an SM");
+  static_assert((smem + 1024) * F::kCtas <= 227 * 1024, "CTAs an SM");
   static_assert(T::kSmem <= 227 * 1024, "the tcgen05 kernel's shared memory");
   cudaLaunchAttribute attr[1];
   cudaLaunchConfig_t cfg;

@@ -279,6 +279,9 @@ struct Fmt {
   }
 };
 
+// Tiles of a split in the tcgen05 kernel: at least two, one for each of its groups.
+__device__ __forceinline__ int tiles_of_split(int tiles, int max_np) { return max(2, (tiles + max_np - 1) / max_np); }
+
 // What one item reads and where its partial goes.
 struct Item {
   const uint8_t* k;  // the head's first row
@@ -713,7 +716,11 @@ __device__ __forceinline__ Plan make_plan(const Params& p, int grid) {
 template <typename F>
 __global__ void __launch_bounds__(kThreads, F::kCtas) prefix_attn_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
-  griddep_wait();
+  // Behind the tcgen05 kernel (parts == 2) the own rows need not wait for it: it let this launch start only after its own
+  // wait, so what comes before both is complete. They start on the SMs that it leaves, and wait for it at their end, so
+  // that the merge, which waits for this launch, finds both kernels' partials.
+  const bool beside = p.parts == 2;
+  if (!beside) griddep_wait();
   griddep_launch_dependents();
   const int grid = gridDim.x, cta = blockIdx.x;
   const Plan pl = make_plan<F::kTile>(p, grid);
@@ -777,6 +784,7 @@ __global__ void __launch_bounds__(kThreads, F::kCtas) prefix_attn_kernel(const _
     it.v_par = S.v_par;
     run_item<F>(p, it, wm, smem);
   }
+  if (beside) griddep_wait();
   // an own length outside its cache with no item of its own (no split at all) is reported here
   if (cta == 0 && pl.ns == 0 && p.own.k)
     for (int b = threadIdx.x; b < p.n_seqs; b += kThreads)
@@ -798,7 +806,7 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_merge(const __grid_const
   int np = __ldcg(p.plan);
   if (n_pre < 0 || n_pre > p.pre.cache_len || n_own < 0 || n_own > p.own.cache_len) return;
   if (p.parts == 2) {  // the tcgen05 kernel's splits: the tiles dealt evenly, two partials each
-    const int tiles = static_cast<int>((n_pre + 127) / 128), per = max(1, (tiles + p.max_np - 1) / p.max_np);
+    const int tiles = static_cast<int>((n_pre + 127) / 128), per = tiles_of_split(tiles, p.max_np);
     np = 2 * ((tiles + per - 1) / per);
   }
   const int ns = n_own ? static_cast<int>(((n_own + stage - 1) / stage + ot - 1) / ot) : 0;

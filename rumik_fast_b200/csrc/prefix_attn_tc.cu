@@ -33,9 +33,13 @@ constexpr int kFirstK = 8, kFirstV = 12;  // warps 0 .. 7: two softmax groups; 8
 constexpr int kLoadWarps = 4;
 constexpr int kLoadThreads = kLoadWarps * 32;
 constexpr int kThreads = 512;
-// The softmax warps hold a tile's scores in registers, 128 a thread; the loaders give them up.
-constexpr int kSoftRegs = 184, kLoadRegs = 72;
-static_assert(2 * kSoftRegs + 2 * kLoadRegs <= 4 * (65536 / kThreads), "registers of the launch, by warpgroup");
+// Registers by warpgroup, and the tiles of codes that a loader holds ahead. kH 16-lane halves of a warp hold rows: the
+// softmax warps keep a tile's scores, 64 kH a thread; what they leave goes to the loaders.
+template <int kFmt, int kH>
+struct Regs {
+  static constexpr int kSoft = kH == 1 ? 144 : (kFmt == RB_KV_INT4 ? 200 : 192), kLoad = 256 - kSoft, kAhead = kH == 1 ? 2 : 1;
+  static_assert(2 * kSoft + 2 * kLoad <= 4 * (65536 / kThreads), "the launch's registers");
+};
 constexpr int kVRing = 3, kKParRing = 4;
 constexpr uint32_t kTmemCols = 512;
 
@@ -391,7 +395,7 @@ __device__ __forceinline__ void run_softmax(const Params& p, uint32_t s0, uint8_
   mm4::tc_fence_before();
 }
 
-template <typename F>
+template <typename F, int kH>
 __global__ void __launch_bounds__(kThreads, 1) prefix_attn_tc_kernel(const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -415,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attn_tc_kernel(const __gri
     return;
   }
   const int tiles = static_cast<int>((n + kTile - 1) / kTile);
-  const int per = (tiles + p.max_np - 1) / p.max_np;
+  const int per = pfx::tiles_of_split(tiles, p.max_np);
   const int t0 = sp * per, t1 = min(tiles, t0 + per), nt = t1 - t0;
   if (nt <= 0) return;  // the merge knows which splits there are
 
@@ -447,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attn_tc_kernel(const __gri
 
   if (warp >= kFirstK) {
     // ---------------- loaders: four warps of keys, four of values ----------------
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Regs<F::kFmt, kH>::kLoad));
     const bool keys = warp < kFirstV;
     const int lw = warp - (keys ? kFirstK : kFirstV), lt = lw * 32 + lane;
     const int ring = keys ? F::kKRing : kVRing;
@@ -512,43 +516,46 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attn_tc_kernel(const __gri
       const int lr = F::kFmt == RB_KV_INT8 ? ((lane >> 1) & 1) | (((lane >> 3) & 1) << 1) | (((lane >> 2) & 1) << 2) | ((lane >> 4) << 3) : lane >> 1;
       auto row_of = [&](int i) { return ((i / kPairs) * kLoadWarps + lw) * 16 + lr; };
       auto piece_of = [&](int i) { return 2 * (i % kPairs) + (lane & 1); };
-      const void* par_src = keys ? p.pre.k_par : p.pre.v_par;
       constexpr int kParBytes = F::kFmt == RB_KV_INT8 ? 2 : 4;
-      uint4 raw[F::kRaw];
-      uint32_t par = 0u;
+      constexpr int kAhead = Regs<F::kFmt, kH>::kAhead;
+      uint4 raws[kAhead][F::kRaw];
+      uint32_t pars[kAhead];
       const uint8_t* from = src + static_cast<int64_t>(t0) * kTile * F::kRow + lr * F::kRow + (lane & 1) * 16 + lw * 16 * F::kRow;
-      int64_t seen = n - static_cast<int64_t>(t0) * kTile;  // slots from the tile to fetch on
-      auto fetch = [&](int i) {  // piece i of a thread: row block i / kPairs of its warp, pieces 2 (i % kPairs) and the next
-        raw[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (row_of(i) < seen) raw[i] = ldg_cg_128(from + (i / kPairs) * (kLoadWarps * 16 * F::kRow) + (i % kPairs) * 32);
-      };
-      auto fetch_par = [&](int t) {  // thread: slot
-        const int64_t at = head + static_cast<int64_t>(t0 + t) * kTile + lt;
+      const uint8_t* par_from = static_cast<const uint8_t*>(keys ? p.pre.k_par : p.pre.v_par) + (head + static_cast<int64_t>(t0) * kTile + lt) * kParBytes;
+      int seen = static_cast<int>(n - static_cast<int64_t>(t0) * kTile);  // slots from the tile to fetch on
+      // Tile t (in order, none left out): piece i of a thread is of row block i / kPairs of its warp, pieces
+      // 2 (i % kPairs) and the next; its parameters' word is of slot lt.
+      auto fetch = [&](int t, uint4 (&raw)[F::kRaw], uint32_t& par) {
+        if (t >= nt) return;
+#pragma unroll
+        for (int i = 0; i < F::kRaw; ++i) {
+          raw[i] = make_uint4(0u, 0u, 0u, 0u);
+          if (row_of(i) < seen) raw[i] = ldg_cg_128(from + (i / kPairs) * (kLoadWarps * 16 * F::kRow) + (i % kPairs) * 32);
+        }
         par = 0u;
         if (lt < seen)
-          par = F::kFmt == RB_KV_INT8 ? static_cast<uint32_t>(__ldcg(reinterpret_cast<const unsigned short*>(par_src) + at))
-                                      : __ldcg(reinterpret_cast<const unsigned int*>(par_src) + at);
-        // registers hold one tile ahead, less than the way from HBM takes: the tiles behind it are called to L2
+          par = F::kFmt == RB_KV_INT8 ? static_cast<uint32_t>(__ldcg(reinterpret_cast<const unsigned short*>(par_from)))
+                                      : __ldcg(reinterpret_cast<const unsigned int*>(par_from));
+        // registers hold less than is on the way from HBM: the tiles behind are called to L2, by the two threads whose
+        // addresses start a tile
         constexpr int kFar = 4;
-        const int64_t far = static_cast<int64_t>(t0 + t + kFar) * kTile;
-        if (t + kFar < nt && lt < 2) {
-          const int rows = static_cast<int>(min(n - far, int64_t(kTile)));
-          const uint8_t* what = lt == 0 ? src + far * F::kRow
-                                        : reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(static_cast<const uint8_t*>(par_src) + (head + far) * kParBytes) & ~uintptr_t(15));
-          const uint32_t bytes = lt == 0 ? rows * F::kRow : rows * kParBytes & ~15;
-          if (bytes) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(what), "r"(bytes) : "memory");
+        if (t + kFar < nt && lt == 0) {
+          const int rows = min(seen - kFar * kTile, kTile);
+          asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from + kFar * kTile * F::kRow), "r"(rows * F::kRow) : "memory");
+          const uint8_t* what = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(par_from + kFar * kTile * kParBytes) & ~uintptr_t(15));
+          if (rows * kParBytes >= 16) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(what), "r"(rows * kParBytes & ~15) : "memory");
         }
+        from += kTile * F::kRow;
+        par_from += kTile * kParBytes;
+        seen -= kTile;
       };
 #pragma unroll
-      for (int i = 0; i < F::kRaw; ++i) fetch(i);
-      fetch_par(0);
-      for (int t = 0; t < nt; ++t) {
+      for (int i = 0; i < kAhead; ++i) fetch(i, raws[i], pars[i]);
+      auto convert = [&](int t, uint4 (&raw)[F::kRaw], uint32_t& par) {
         // The keys' parameters lie in a ring of four: tile t - 4's are free once QK(t - 2), which its group issued behind
         // PV(t - 4), has released the keys' slot.
-        if (!free_slot(t)) break;
+        if (!free_slot(t)) return;
         const uint32_t dst = base + slot * F::kTileBytes;
-        from += kTile * F::kRow;
-        seen = t + 1 < nt ? seen - kTile : 0;  // no fetch behind the last tile
 #pragma unroll
         for (int i = 0; i < F::kRaw; ++i) {
           const int r = row_of(i), ch = piece_of(i);
@@ -579,17 +586,19 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attn_tc_kernel(const __gri
         pd[at] = s;
         if constexpr (F::kFmt == RB_KV_INT4)
           pd[F::kParN + at] = fmaf(8.f, s, p.bf16 ? __uint_as_float(par & 0xffff0000u) : __half2float(__ushort_as_half(static_cast<unsigned short>(par >> 16))));
-        // The fence in arrive waits for a thread's outstanding loads too: the next tile's are issued behind it.
         arrive(slot);
-#pragma unroll
-        for (int i = 0; i < F::kRaw; ++i) fetch(i);
-        fetch_par(t + 1);
         next_slot();
+        fetch(t + kAhead, raw, par);
+      };
+      for (int t = 0; t < nt && ok; t += kAhead) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+          if (t + i < nt && ok) convert(t + i, raws[i], pars[i]);
       }
     }
   } else {
     // ---------------- softmax: group g takes the tiles t % 2 == g ----------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Regs<F::kFmt, kH>::kSoft));
     const int g = warp >> 2, quad = warp & 3;
     const int rows = min(kTile, p.n_seqs * p.rep - row0);
     float* rowf = reinterpret_cast<float*>(smem + F::kOffRow);
@@ -640,8 +649,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attn_tc_kernel(const __gri
       fence_proxy_async_smem();
     }
     named_bar_sync(kBarSoft, 256);
-    if (rows <= kTile / 2) run_softmax<F, 1>(p, s0, smem, tmem, g, quad, lane, nt, n - static_cast<int64_t>(t0) * kTile, rows, lane_i * p.max_np + sp);
-    else run_softmax<F, 2>(p, s0, smem, tmem, g, quad, lane, nt, n - static_cast<int64_t>(t0) * kTile, rows, lane_i * p.max_np + sp);
+    run_softmax<F, kH>(p, s0, smem, tmem, g, quad, lane, nt, n - static_cast<int64_t>(t0) * kTile, rows, lane_i * p.max_np + sp);
   }
   __syncthreads();
   if (warp == kFirstK) {
@@ -657,11 +665,18 @@ namespace pfx {
 // Warps along the rows: the fewest whose 16-row tiles hold the batch's rows, at most four.
 inline int warps_m(int64_t rows) { return rows <= 16 ? 1 : (rows <= 32 ? 2 : 4); }
 
-// Which kernel streams the prefix, when the flags do not say.
+// Which kernel streams the prefix, when the flags do not say: by its capacity, the lengths being on the device. The
+// tcgen05 kernel's start costs about what one to two thousand slots cost the warp-level one (8 heads of 128, 16 bits, 20
+// own slots, 24 rows: 1,000 slots 11 us against 13, 3,000 12 against 18, 40,000 42 against 44; 256 rows: 27 against 32, 32
+// against 40, 103 against 179). Only for up to 16 rows of 8-bit codes of 128 columns is the warp-level kernel's conversion,
+// which uses no shared memory on the way, the faster one (8 rows: 10,000 slots 18 us against 16, 40,000 44 against 33; 24
+// rows: 22 against 21, 47 against 47; 48 rows: 48 against 67).
 inline bool use_tc(const rb_prefix_attn_args* a, int rep, int flags) {
   if (!a->prefix || (flags & RB_FLAG_KERNEL_MMA)) return false;
   if (flags & RB_FLAG_KERNEL_TC) return true;
-  return a->n_seqs * rep > 32 && a->prefix->cache_len >= 2048;
+  const int64_t rows = a->n_seqs * rep;
+  if (a->prefix->fmt == RB_KV_INT8 && a->prefix->head_dim == 128 && rows <= 16) return false;
+  return a->prefix->cache_len >= (rows > 32 ? 1024 : 2048);
 }
 
 struct Layout {
@@ -713,7 +728,7 @@ int launch_format(const Params& p, const Layout& L, bool tc, int flags, cudaStre
   cudaLaunchConfig_t cfg;
   Params rest = p;
   if (tc) {
-    auto* kern = pfxt::prefix_attn_tc_kernel<T>;
+    auto* kern = p.n_seqs * p.rep <= pfxt::kTile / 2 ? pfxt::prefix_attn_tc_kernel<T, 1> : pfxt::prefix_attn_tc_kernel<T, 2>;
     if (ensure_smem_limit(reinterpret_cast<const void*>(kern), T::kSmem) != cudaSuccess) return RB_ERR_LAUNCH;
     cfg = launch_config(p.n_kv * p.tiles_m * p.max_np, pfxt::kThreads, T::kSmem, flags, stream, attr);
     if (cudaLaunchKernelEx(&cfg, kern, p) != cudaSuccess) return RB_ERR_LAUNCH;

@@ -9,6 +9,7 @@ The search's state stays on the device, so a step can be captured in a CUDA grap
 with a sampler (engine/sample.py; here sample.FusedSampler) and has no beam search.
 """
 import ctypes
+import math
 
 import torch
 
@@ -85,7 +86,7 @@ class BeamReorder:
         for i, t in enumerate(tensors):
             _require(t.is_cuda and t.device == dev and t.is_contiguous() and t.dim() >= 3 and t.shape[0] == R * nb
                      and t.shape[2] == S, f"tensor {i} must be a contiguous [{R * nb}, n_heads, {S}, ...] tensor on {dev}")
-            row = t.element_size() * (t[0, 0, 0].numel() if t.numel() else 1)
+            row = t.element_size() * math.prod(t.shape[3:])
             _require(row % 2 == 0, f"tensor {i}: rows of {row} bytes (an even number is needed)")
             arr[i] = _lib.BeamTensor(t.data_ptr(), t.shape[1], row)
         self.device, self._keep = dev, (list(tensors), parents, slots)

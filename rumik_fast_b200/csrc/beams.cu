@@ -5,8 +5,10 @@
 //   cand[b, v] = (x[b, v] - lse_b) + score_b,  lse_b = log sum_v exp(x[b, v])        (a live beam)
 //   cand[b, end] = score_b and nothing else                                           (a finished beam)
 // and the nb best of the nb V candidates. Within a beam the order of the candidates is the order of the logits, so no
-// normaliser is needed to find a beam's nb best rows: one pass over the logits yields each 4096-row chunk's maximum,
-// sum of exponentials and nb best (value, row) keys. The last chunk of a beam to finish merges them, and the last beam
+// normaliser is needed to find a beam's nb best rows: one pass over the logits yields each chunk's maximum, sum of
+// exponentials and nb best (value, row) keys. A CTA takes its chunk in batches of 4096 rows, the next one's loads in
+// flight; the first batch gives a bound that nb keys reach, and of later ones only the keys above it are looked at: two
+// barriers a batch instead of a selection. The last chunk of a beam to finish merges them, and the last beam
 // of a request picks the winners: one launch, every logit read once.
 // A key is the logit's order-preserving 32 bits above the row's complement, so the largest key is the largest logit,
 // the lower row among equals, and no two keys are equal: the result does not depend on the order of arrival.
@@ -20,11 +22,13 @@ namespace bm {
 using Key = unsigned long long;
 constexpr int kThreads = 256;
 constexpr int kPer = 16;                       // logits of a thread, held in registers
-constexpr int kChunk = kThreads * kPer;        // 4096 rows a CTA
+constexpr int kChunk = kThreads * kPer;        // 4096 rows a batch
+constexpr int kSelectCtas = 4;                 // of an SM, by registers and shared memory
+constexpr int kFew = 64;                       // threads whose keys a CTA's list takes before it is cut back to the nb best
 constexpr int kMaxBeams = 32;
 constexpr int kMaxChunks = 256;                // V <= 2^20
 constexpr int kCap = kThreads / 32 * kMaxBeams * kPer;                // keys that may pass a bound: 4096
-static_assert(kCap >= kMaxBeams * (kMaxChunks * kMaxBeams / kThreads), "those of a beam's merged lists as well");
+static_assert(kCap >= kChunk && kCap >= kFew * kPer && kCap >= kMaxBeams * (kMaxChunks * kMaxBeams / kThreads), "those of a beam's merged lists as well");
 
 struct SelectParams {
   const void* logits;
@@ -43,11 +47,11 @@ struct SelectParams {
   float* row_cand;         // [R nb][nb] a beam's best candidates, best first
   int* row_idx;            // [R nb][nb] their rows (-1: none)
   int64_t end_idx, min_new;
-  int nb, V, chunks, dtype;
+  int nb, V, chunks, per;  // per: batches of kChunk logits a CTA takes
 };
 
 __device__ __forceinline__ Key make_key(float x, uint32_t row) {
-  const uint32_t b = __float_as_uint(x);
+  const uint32_t b = __float_as_uint(x + 0.f);  // -0 -> +0
   const uint32_t k = (b & 0x80000000u) ? ~b : b | 0x80000000u;
   return (static_cast<Key>(k) << 32) | (0xffffffffu - row);
 }
@@ -58,7 +62,7 @@ __device__ __forceinline__ float key_value(Key key) {
 __device__ __forceinline__ uint32_t key_row(Key key) { return 0xffffffffu - static_cast<uint32_t>(key); }
 
 struct Shared {
-  Key cand[kCap];
+  Key cand[kCap + kMaxBeams];  // a batch's keys and those that were kept of the ones before
   Key top[kThreads];
   Key bound[kThreads / 32], each[kThreads / 32];
   float2 red[kThreads / 32];
@@ -76,7 +80,6 @@ __device__ __forceinline__ Key cta_bound(Shared& sh, int k, Key best) {
   constexpr int kN = kWide ? kThreads : 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   sh.top[threadIdx.x] = best;
-  if (threadIdx.x == 0) sh.n = 0;
   if (lane == 0) sh.bound[warp] = 1, sh.each[warp] = 0;
   if (kWide) __syncthreads();
   else __syncwarp();
@@ -127,6 +130,7 @@ __device__ __forceinline__ void cta_top(Shared& sh, int k, int n, Get get, Out o
     if (v) sh.cand[atomicAdd(&sh.n, 1)] = v;
   } else {
     Key best = 0;
+    if (threadIdx.x == 0) sh.n = 0;
 #pragma unroll 1
     for (int i = threadIdx.x; i < n; i += kThreads) {
       const Key v = get(i);
@@ -159,10 +163,16 @@ __device__ __forceinline__ bool last_to_arrive(Shared& sh, unsigned int* ticket,
   return sh.last != 0;
 }
 
-// exp(x), x <= 0: the hardware's 2^x (relative error 2^-22)
-__device__ __forceinline__ float exp_of(float x) {
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float ex2(float x) {  // the hardware's 2^x (relative error 2^-22)
   float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float exp_of(float x) { return ex2(x * kLog2e); }
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
 }
 
@@ -174,7 +184,7 @@ __device__ __forceinline__ float2 merge_sums(float2 a, float2 b) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) beam_select_kernel(const __grid_constant__ SelectParams p) {
+__global__ void __launch_bounds__(kThreads, kSelectCtas) beam_select_kernel(const __grid_constant__ SelectParams p) {
   __shared__ Shared sh;
   griddep_wait();
   griddep_launch_dependents();
@@ -186,57 +196,104 @@ __global__ void __launch_bounds__(kThreads) beam_select_kernel(const __grid_cons
   const bool done = p.done[row] != 0;
   const bool dead = !(score > -INFINITY && score < INFINITY);  // no candidate of this beam counts
   if (!done && !dead) {
-    const int first = chunk * kChunk + tid;
-    const T* x = reinterpret_cast<const T*>(p.logits) + row * p.ld + first;
-    float v[kPer];
-    if (chunk * kChunk + kChunk <= p.V) {
+    const int begin = chunk * p.per * kChunk, end = min(p.V, begin + p.per * kChunk);
+    const T* x = reinterpret_cast<const T*>(p.logits) + row * p.ld;
+    T raw[kPer];
+    auto load = [&](int from) {
+      if (from + kChunk <= end) {
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) v[i] = static_cast<float>(x[i * kThreads]) + 0.f;  // -0 -> +0
-    } else {
+        for (int i = 0; i < kPer; ++i) raw[i] = x[from + tid + i * kThreads];
+      } else {
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) v[i] = first + i * kThreads < p.V ? static_cast<float>(x[i * kThreads]) + 0.f : -INFINITY;
+        for (int i = 0; i < kPer; ++i) raw[i] = from + tid + i * kThreads < end ? x[from + tid + i * kThreads] : T(-INFINITY);
+      }
+    };
+    load(begin);
+    float2 ms = make_float2(-INFINITY, 0.f);
+    bool odd = false;
+    Key lim = 1;         // at least nb keys so far reach it (1: fewer keys than that)
+    float least = 0.f;   // its logit (NaN for 1)
+    int held = 0;        // threads whose keys are in sh.cand, about the keys there
+    if (tid == 0) sh.n = 0;
+#pragma unroll 1
+    for (int from = begin; from < end; from += kChunk) {
+      const int first = from + tid;
+      float v[kPer];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) v[i] = static_cast<float>(raw[i]);
+      if (from + kChunk < end) load(from + kChunk);
+      if (early) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          if (first + i * kThreads == p.end_idx) v[i] = -INFINITY;
+      }
+      float top = v[0];
+#pragma unroll
+      for (int i = 1; i < kPer; ++i) top = max_nan(top, v[i]);
+      odd |= !(top < INFINITY);  // NaN or +inf: the row has no distribution
+      if (!odd && top > -INFINITY) {
+        const float m = fmaxf(ms.x, top);
+        float2 sum = make_float2(ms.y * exp_of(ms.x - m), 0.f);
+        const float2 off = make_float2(-m, -m), unit = make_float2(kLog2e, kLog2e);
+#pragma unroll
+        for (int i = 0; i < kPer; i += 2) {
+          const float2 t = mul2(add2(make_float2(v[i], v[i + 1]), off), unit);
+          sum = add2(sum, make_float2(ex2(t.x), ex2(t.y)));
+        }
+        ms = make_float2(m, sum.x + sum.y);
+      }
+      auto best = [&] {  // this thread's largest key: the lowest row among equals
+        int at = 0;
+#pragma unroll
+        for (int i = kPer - 1; i > 0; --i)
+          if (v[i] == top) at = i;
+        if (v[0] == top) at = 0;
+        return first < end ? make_key(top, first + at * kThreads) : Key(0);
+      };
+      // rows past the vocabulary hold -inf like masked ones, but no key
+      auto reaches = [&] { return first < end && !(top < least); };
+      if (from == begin) {
+        lim = cta_bound<false>(sh, nb, best());
+        least = key_value(lim);
+      }
+      int many = __syncthreads_count(reaches());
+      if (from > begin && held + many > kFew) {
+        // the list's nb best stay, and the last of them is the new bound
+        cta_rank(sh, nb, [&](int r, Key key) { sh.top[r] = key; });
+        if (tid < nb) sh.cand[tid] = sh.top[tid];
+        if (tid == 0) sh.n = min(sh.n, nb);
+        lim = max(lim, sh.top[nb - 1]);
+        least = key_value(lim);
+        held = nb;
+        many = __syncthreads_count(reaches());
+        if (many > kFew) {  // rising logits, for one: this batch's own bound is closer
+          lim = max(lim, cta_bound<false>(sh, nb, best()));
+          least = key_value(lim);
+          many = __syncthreads_count(reaches());
+        }
+      }
+      held += many;
+      if (reaches()) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          if (!(v[i] < least)) {
+            const Key key = make_key(v[i], first + i * kThreads);
+            if (key >= lim && first + i * kThreads < end) sh.cand[atomicAdd(&sh.n, 1)] = key;
+          }
+      }
     }
-    if (early) {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (first + i * kThreads == p.end_idx) v[i] = -INFINITY;
-    }
-    float top = v[0];
-    int at = 0;
-    bool odd = !(v[0] < INFINITY);  // NaN or +inf: the row has no distribution
-#pragma unroll
-    for (int i = 1; i < kPer; ++i) {
-      odd |= !(v[i] < INFINITY);
-      if (v[i] > top) top = v[i], at = i;  // the lowest row among equals
-    }
-    float2 ms = make_float2(odd ? INFINITY : top, 0.f);
-    if (!odd && top > -INFINITY) {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) ms.y += exp_of(v[i] - top);
-    }
+    if (odd) ms = make_float2(INFINITY, 0.f);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
       ms = merge_sums(ms, make_float2(__shfl_xor_sync(0xffffffffu, ms.x, o), __shfl_xor_sync(0xffffffffu, ms.y, o)));
     if (lane == 0) sh.red[warp] = ms;
-    // rows past the vocabulary hold -inf like masked ones, but no key
-    const Key best = first < p.V ? make_key(top, first + at * kThreads) : Key(0);
-    const Key lim = cta_bound<false>(sh, nb, best);
+    Key* dst = p.keys + (static_cast<int64_t>(row) * p.chunks + chunk) * nb;
+    cta_rank(sh, nb, [&](int r, Key key) { dst[r] = key; });
     if (tid == 0) {
 #pragma unroll 1
       for (int w = 1; w < kThreads / 32; ++w) ms = merge_sums(ms, sh.red[w]);
       p.part[static_cast<int64_t>(row) * p.chunks + chunk] = ms;
     }
-    if (best >= lim) {
-      const float least = key_value(lim);
-#pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if ((!(v[i] < least) || lim == 1) && first + i * kThreads < p.V) {
-          const Key key = make_key(v[i], first + i * kThreads);
-          if (key >= lim) sh.cand[atomicAdd(&sh.n, 1)] = key;
-        }
-    }
-    Key* dst = p.keys + (static_cast<int64_t>(row) * p.chunks + chunk) * nb;
-    cta_rank(sh, nb, [&](int r, Key key) { dst[r] = key; });
   }
   if (!last_to_arrive(sh, p.tickets + row, p.chunks)) return;
 
@@ -389,7 +446,7 @@ int64_t beam_select_workspace(int64_t requests, int nb, int64_t V) {
   return beam_select_tickets(requests, nb) + align16(rows * ch * 8) + align16(rows * ch * nb * 8) + 2 * align16(rows * nb * 4);
 }
 
-int launch_beam_select(const rb_beam_select_args* a, int flags, cudaStream_t stream) {
+int launch_beam_select(const rb_beam_select_args* a, int num_sms, int flags, cudaStream_t stream) {
   using namespace bm;
   const int64_t rows = a->requests * a->n_beams;
   SelectParams p = {};
@@ -407,8 +464,12 @@ int launch_beam_select(const rb_beam_select_args* a, int flags, cudaStream_t str
   p.min_new = a->min_new;
   p.nb = a->n_beams;
   p.V = static_cast<int>(a->n_vocab);
-  p.chunks = static_cast<int>(select_chunks(a->n_vocab));
-  p.dtype = a->logits_dtype;
+  // one batch a CTA while the CTAs fit on the SMs at once, else the fewest that make them fit
+  const int64_t batches = select_chunks(a->n_vocab);
+  int64_t per = 1;
+  while (per < batches && rows * ((batches + per - 1) / per) > kSelectCtas * static_cast<int64_t>(num_sms)) ++per;
+  p.per = static_cast<int>(per);
+  p.chunks = static_cast<int>((batches + per - 1) / per);
   uint8_t* w = static_cast<uint8_t*>(a->ws);
   p.tickets = reinterpret_cast<unsigned int*>(w);
   w += beam_select_tickets(a->requests, a->n_beams);

@@ -680,7 +680,7 @@ int rb_beam_select(const rb_beam_select_args* a, int flags, void* stream) {
   if (a->ws_bytes < rb::beam_select_workspace(a->requests, a->n_beams, a->n_vocab)) return RB_ERR_SHAPE;
   int sms = 0, st = device_sms(&sms);
   if (st != RB_OK) return st;
-  st = rb::launch_beam_select(a, flags, static_cast<cudaStream_t>(stream));
+  st = rb::launch_beam_select(a, sms, flags, static_cast<cudaStream_t>(stream));
   if (st == RB_OK && cudaGetLastError() != cudaSuccess) st = RB_ERR_LAUNCH;
   return st;
 }

@@ -74,7 +74,7 @@ int launch_kv_read(const rb_kv_cache* c, void* k_out, void* v_out, int64_t start
 int64_t prefix_attn_workspace(const rb_prefix_attn_args* a, int num_sms);
 int launch_prefix_attn(const rb_prefix_attn_args* a, int num_sms, int flags, cudaStream_t stream);
 int64_t beam_select_workspace(int64_t requests, int nb, int64_t V);
-int launch_beam_select(const rb_beam_select_args* a, int flags, cudaStream_t stream);
+int launch_beam_select(const rb_beam_select_args* a, int num_sms, int flags, cudaStream_t stream);
 int launch_beam_reorder(const rb_beam_tensor* t, int count, int64_t requests, int nb, int64_t cache_len,
                         const int64_t* parents, const int64_t* slots, int num_sms, int flags, cudaStream_t stream);
 // The add + LayerNorm of rb_add_layernorm (one CTA), bit-identical to the prologue of rb_gemv_int4_fused.

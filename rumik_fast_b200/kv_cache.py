@@ -82,6 +82,7 @@ class KVCache:
                                  None if v_par is None else v_par.data_ptr(), FORMATS[self.fmt], _lib.dtype_code(dtype),
                                  self.n_seqs, self.n_kv_heads, self.head_dim, self.cache_len)
         self._ref = ctypes.byref(self.desc)
+        self._empty = torch.empty(0, dtype=dtype, device=k.device)
 
     def tensors(self):
         """The cache's tensors, for beams.BeamReorder."""
@@ -120,8 +121,7 @@ class KVCache:
             _require(False, f"slots {start} .. {start + count - 1} are not in a cache of {self.cache_len}")
         shape = (self.n_seqs, self.n_kv_heads, count, self.head_dim)
         if out is None:
-            both = torch.empty((2,) + shape, dtype=self.dtype, device=self.device)
-            out = (both[0], both[1])
+            out = (self._empty.new_empty(shape), self._empty.new_empty(shape))
         else:
             for t in out:
                 _require(t.shape == shape and t.dtype == self.dtype and t.device == self.device and t.is_contiguous(),

@@ -61,6 +61,21 @@ def test_largest_vocabulary():
     check(logits, scores, done, 5, BeamSelect(logits.to(DEV), scores.to(DEV), done.to(DEV), end_idx=5)())
 
 
+@pytest.mark.parametrize("order", ["up", "down", "shuffled"])
+@pytest.mark.parametrize("nb,V", [(16, 9000), (32, 16500)])
+def test_rows_of_several_batches(nb, V, order):
+    """More rows than CTAs at once: a CTA takes several batches of its row, whose logits rise, fall or do neither."""
+    at = torch.arange(V)
+    if order == "down":
+        at = at.flip(0)
+    elif order == "shuffled":
+        at = at[torch.randperm(V, generator=torch.Generator().manual_seed(V))]
+    logits = (at * 0.002).float().expand(40, nb, V).contiguous()
+    scores = (-0.0103 * torch.arange(nb)).float().expand(40, nb).contiguous()
+    done = torch.zeros(40, nb, dtype=torch.bool)
+    check(logits, scores, done, 3, BeamSelect(logits.to(DEV), scores.to(DEV), done.to(DEV), end_idx=3)())
+
+
 def test_ties_go_to_the_lowest_beam_and_row():
     """All logits and scores equal, and a few equal peaks: every order is decided by the index."""
     for V in (7, 4096, 10000):

@@ -60,7 +60,9 @@ enum rb_flags {
   RB_FLAG_PREFETCH_WEIGHTS = 2,
   /* GEMV lists (rb_gemv_int4_multi / _multi_ws / _fused): run on the tcgen05 kernel, or on the warp-MMA kernel,
    * whatever the list's size. Without either, lists whose codes total less than 128 MiB (a decode layer's
-   * projections, latency-bound) run on the warp-MMA kernel and longer lists on the tcgen05 kernel. */
+   * projections, latency-bound) run on the warp-MMA kernel and longer lists on the tcgen05 kernel.
+   * rb_prefix_attn: stream the prefix with the tcgen05 kernel, or with the warp-MMA kernel, whatever the number of
+   * query rows and the prefix's capacity. */
   RB_FLAG_KERNEL_TC = 4,
   RB_FLAG_KERNEL_MMA = 8,
   /* rb_attn_decode: merge the splits through global partials and a per-head ticket (the form that needs no
@@ -528,10 +530,10 @@ int rb_kv_read(const rb_kv_cache* cache, void* k_out, void* v_out, int64_t start
  * slots j < own_len[b] of sequence b in `own` (n_seqs as the call's). The prefix is read once for the whole batch, not
  * once a sequence. A sequence without any slot gets zeros. Either cache may be NULL; both have one format, dtype, head
  * count and head_dim. 1 <= n_q_heads / n_kv_heads <= 16. Lengths are int64 on the device; a *prefix_len or own_len[b]
- * outside its cache stores nothing for the sequences it concerns and sets RB_DEVERR_ARG. Rows at or beyond a length are
- * not looked at. Scores, softmax and sums are fp32; a quantised row enters the products as its codes.
- * ws: rb_prefix_attn_workspace(...) bytes, 16-byte aligned, zero before the first call; every call leaves its counters
- * zero. Calls that share a workspace must not overlap in time.
+ * outside its cache stores nothing for the sequences it concerns and sets RB_DEVERR_ARG. Scores, softmax and sums are
+ * fp32; a quantised row enters the products as its codes. Rows at or beyond a length may hold anything. A wait that runs out sets bit 12 (0x1000) of the device error word.
+ * ws: rb_prefix_attn_workspace(...) bytes, 16-byte aligned, whatever they hold. Calls that share a workspace must not
+ * overlap in time.
  */
 typedef struct rb_prefix_attn_args {
   const void* q;              /* [n_seqs, n_q_heads, head_dim], sequence stride ldq elements (multiple of 8) */

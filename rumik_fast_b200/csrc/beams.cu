@@ -12,6 +12,9 @@
 // of a request picks the winners: one launch, every logit read once.
 // A key is the logit's order-preserving 32 bits above the row's complement, so the largest key is the largest logit,
 // the lower row among equals, and no two keys are equal: the result does not depend on the order of arrival.
+// Bound: 8 requests of 16 beams over 130,001 fp32 logits take 30 us, 0.34 of the measured copy bandwidth: half of the time
+// in barriers of the batches, the rest in the 17 instructions a warp spends on 32 logits (45 us with one batch a CTA and
+// its selection for each). Four beams over 16,385 rows: 10 us, three dependent steps of latency (chunk, beam, request).
 #include "common.cuh"
 #include "kernels.h"
 
@@ -24,7 +27,7 @@ constexpr int kThreads = 256;
 constexpr int kPer = 16;                       // logits of a thread, held in registers
 constexpr int kChunk = kThreads * kPer;        // 4096 rows a batch
 constexpr int kSelectCtas = 4;                 // of an SM, by registers and shared memory
-constexpr int kFew = 64;                       // threads whose keys a CTA's list takes before it is cut back to the nb best
+constexpr int kFew = 64;                        // threads whose keys a list takes before it is cut back to the nb best (144: 32 us, not 30)
 constexpr int kMaxBeams = 32;
 constexpr int kMaxChunks = 256;                // V <= 2^20
 constexpr int kCap = kThreads / 32 * kMaxBeams * kPer;                // keys that may pass a bound: 4096
@@ -354,6 +357,10 @@ __global__ void __launch_bounds__(kThreads, kSelectCtas) beam_select_kernel(cons
 
 // ---- reordering ----
 
+// Of every (tensor, beam head) line the columns are independent: a thread holds one column of all beams, so any permutation
+// or copying of beams is done in place and each row is read once, however many beams take it over. HBM-bound: 72 tensors
+// of 8 beams with 701 slots, 0.72 GB, 130 us (0.85 of the measured copy bandwidth). One launch for up to kMaxTensors
+// tensors, which is what counts for small states: 8 tensors of 61 slots 3 us.
 constexpr int kReorderThreads = 128;
 
 struct Tensor {

@@ -11,6 +11,9 @@
 // depend on how wide the quotient is computed.
 // A row with a NaN or an infinity gets s = NaN and codes of zero: all of it reads back as NaN, in this kernel and in
 // the attention. s == 0 (a row of equal values, or of zeros) gives codes of zero.
+// Bound: HBM for prompts, each byte moved once. 65,536 tokens of 8 heads of 128 in int8, written and read back: 159 us
+// for 0.81 GB, 0.78 of the measured copy bandwidth; 4,099 tokens in int4 16 us for 42 MB (0.40: a few waves of CTAs). One
+// token of 16 sequences is two launches of 2 us, all latency.
 #include "common.cuh"
 #include "kernels.h"
 
@@ -158,9 +161,11 @@ __device__ __forceinline__ void quantise_row(const uint4 raw, bool store, void* 
   }
 }
 
-// A CTA takes kGroups x kRows rows of one (key or value, sequence); all of a thread's loads go out first. kByHead:
-// consecutive tokens of one head - addresses a constant apart, the parameters one contiguous store. Otherwise (fewer
-// than kGroups tokens, a decode step) rows in (token, head) order.
+// A CTA takes kGroups x kRows rows of one (key or value, sequence); all of a thread's loads go out first, four of 16 bytes,
+// which keep HBM busy while other rows' codes are computed (in int8 the arithmetic of a row, some 60 instructions for eight
+// values with packed pairs, takes about as long as its bytes). kByHead: consecutive tokens of one head - addresses a
+// constant apart, the parameters one contiguous store. Otherwise (fewer than kGroups tokens, a decode step) rows in
+// (token, head) order, so that a step of one token is not one row a CTA.
 constexpr int kRows = 4;
 
 template <int kHd, int kFmt, bool kBf16, bool kByHead>
@@ -257,6 +262,7 @@ __device__ __forceinline__ uint32_t pack_act2(float a, float b, bool bf16) {
 }
 
 // A CTA reads kThreads x kUnits pieces of eight values of one (key or value, sequence, head); its loads go out first.
+// HBM-bound: the values that it writes are two to four times the codes it reads.
 constexpr int kUnits = 4;
 
 template <int kHd, int kFmt>

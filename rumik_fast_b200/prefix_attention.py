@@ -59,7 +59,7 @@ class PrefixAttention:
             need = _lib.lib().rb_prefix_attn_workspace(ctypes.byref(a))
         if need < 0:
             _lib.check("rb_prefix_attn_workspace", -need)
-        self.ws = torch.zeros(need, dtype=torch.uint8, device=self.device)
+        self.ws = torch.empty(need, dtype=torch.uint8, device=self.device)
         a.ws, a.ws_bytes = self.ws.data_ptr(), need
         self._args, self._ref, self._flags = a, ctypes.byref(a), _lib.KERNEL_FLAGS[kernel]
 

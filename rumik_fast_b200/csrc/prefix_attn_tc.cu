@@ -18,8 +18,9 @@
 // loader warps for both rings paced the whole kernel at 4,100 cycles a tile.)
 //
 // Bound: 16-bit rows by HBM (32,768 slots of 8 heads with 48 rows in 46 us, of which 38 are this kernel: 3.5 TB/s, the rest
-// start and merge); codes by the loaders, which convert a tile of 128 x 128 in about 2,600 cycles where the tensor core
-// needs 600 and the softmax of 128 rows 1,700 (100,001 slots of 4 heads with 256 rows, int8: 135 us, 390 TFLOP/s).
+// start and merge). 8-bit codes of up to 64 rows by the loaders, 2,100 cycles a tile of keys or values: conversion, the
+// proxy fence and the loads' latency in turn. More rows by a group's chain of QK, softmax and PV, 6,000 cycles for each of
+// two tiles under way, in any format (100,001 slots of 4 heads with 256 rows, int8: 115 us, 99 of them here, 530 TFLOP/s).
 #include "common.cuh"
 #include "tc.cuh"
 #include "kernels.h"
@@ -513,35 +514,38 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attn_tc_kernel(const __gri
       pfx::cp_wait<0>();
     } else {
       constexpr int kPieces = F::kRow / 16;
-      // A thread's pieces: two neighbouring ones (a 32-byte sector) by a lane pair, and the rows of eight lanes chosen so
-      // that the pieces they store, 2 (4) columns of sixteen bytes apart, fall on eight different bank groups.
-      constexpr int kPairs = kPieces / 2;
-      static_assert(F::kRaw == 2 * kPairs, "two row blocks of sixteen a warp");
-      const int lr = F::kFmt == RB_KV_INT8 ? ((lane >> 1) & 1) | (((lane >> 3) & 1) << 1) | (((lane >> 2) & 1) << 2) | ((lane >> 4) << 3) : lane >> 1;
-      auto row_of = [&](int i) { return ((i / kPairs) * kLoadWarps + lw) * 16 + lr; };
-      auto piece_of = [&](int i) { return 2 * (i % kPairs) + (lane & 1); };
+      // A tile's pieces of sixteen bytes lie one after another and are dealt so: a warp's load is 512 bytes in a row, a
+      // thread's pieces are the same columns, ch, of rows kStep apart, and the swizzle of their stores does not change.
+      // Eight lanes that store together hold whole rows; where those span two atoms (128 columns), whose banks are the
+      // same, the lanes of the second one store the halves of their piece in the other order: no two share a bank.
+      constexpr int kStep = kLoadThreads / kPieces, kChunks = F::kFmt == RB_KV_INT8 ? 2 : 4;  // 16-byte chunks of values a piece
+      static_assert(kStep % 8 == 0 && F::kRaw * kStep == kTile, "whole periods of the swizzle");
+      const int lr = lt / kPieces, ch = lt % kPieces;
+      const bool turn = kChunks * ch >= 8;
+      uint32_t at_chunk[kChunks];  // offset of the chunk that is stored e-th, in a tile
+#pragma unroll
+      for (int e = 0; e < kChunks; ++e) at_chunk[e] = piece_at(lr, kChunks * ch + (turn ? e ^ (kChunks / 2) : e));
       constexpr int kParBytes = F::kFmt == RB_KV_INT8 ? 2 : 4;
       constexpr int kAhead = Regs<F::kFmt, kH>::kAhead;
       uint4 raws[kAhead][F::kRaw];
       uint32_t pars[kAhead];
-      const uint8_t* from = src + static_cast<int64_t>(t0) * kTile * F::kRow + lr * F::kRow + (lane & 1) * 16 + lw * 16 * F::kRow;
+      const uint8_t* from = src + static_cast<int64_t>(t0) * kTile * F::kRow + lt * 16;
       const uint8_t* par_from = static_cast<const uint8_t*>(keys ? p.pre.k_par : p.pre.v_par) + (head + static_cast<int64_t>(t0) * kTile + lt) * kParBytes;
       int seen = static_cast<int>(n - static_cast<int64_t>(t0) * kTile);  // slots from the tile to fetch on
-      // Tile t (in order, none left out): piece i of a thread is of row block i / kPairs of its warp, pieces
-      // 2 (i % kPairs) and the next; its parameters' word is of slot lt.
+      // Tile t (in order, none left out): piece i of a thread is of row lr + i kStep, its parameters' word of slot lt.
       auto fetch = [&](int t, uint4 (&raw)[F::kRaw], uint32_t& par) {
         if (t >= nt) return;
 #pragma unroll
         for (int i = 0; i < F::kRaw; ++i) {
           raw[i] = make_uint4(0u, 0u, 0u, 0u);
-          if (row_of(i) < seen) raw[i] = ldg_cg_128(from + (i / kPairs) * (kLoadWarps * 16 * F::kRow) + (i % kPairs) * 32);
+          if (lr + i * kStep < seen) raw[i] = ldg_cg_128(from + i * kLoadThreads * 16);
         }
         par = 0u;
         if (lt < seen)
           par = F::kFmt == RB_KV_INT8 ? static_cast<uint32_t>(__ldcg(reinterpret_cast<const unsigned short*>(par_from)))
                                       : __ldcg(reinterpret_cast<const unsigned int*>(par_from));
-        // registers hold less than is on the way from HBM: the tiles behind are called to L2, by the two threads whose
-        // addresses start a tile
+        // registers hold less than is on the way from HBM: the tiles behind are called to L2 by the thread whose
+        // addresses start a tile (each of them is loaded before the CTA ends). Line by line by all threads it took longer.
         constexpr int kFar = 4;
         if (t + kFar < nt && lt == 0) {
           const int rows = min(seen - kFar * kTile, kTile);
@@ -562,8 +566,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attn_tc_kernel(const __gri
         const uint32_t dst = base + slot * F::kTileBytes;
 #pragma unroll
         for (int i = 0; i < F::kRaw; ++i) {
-          const int r = row_of(i), ch = piece_of(i);
-          const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+          uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+          if (F::kHd == 128 && turn) w[0] = raw[i].z, w[1] = raw[i].w, w[2] = raw[i].x, w[3] = raw[i].y;
+          const uint32_t to = dst + i * (kStep * 128);
           if constexpr (F::kFmt == RB_KV_INT8) {
             uint32_t h[8];
 #pragma unroll
@@ -571,8 +576,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attn_tc_kernel(const __gri
               h[2 * e] = mm4::hsub2_u(__byte_perm(w[e], 0x64646464u, 0x4140), 0x64806480u);  // 1024 + (c + 128) - 1152
               h[2 * e + 1] = mm4::hsub2_u(__byte_perm(w[e], 0x64646464u, 0x4342), 0x64806480u);
             }
-            sts128(dst + piece_at(r, 2 * ch), h[0], h[1], h[2], h[3]);
-            sts128(dst + piece_at(r, 2 * ch + 1), h[4], h[5], h[6], h[7]);
+            sts128(to + at_chunk[0], h[0], h[1], h[2], h[3]);
+            sts128(to + at_chunk[1], h[4], h[5], h[6], h[7]);
           } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {  // a word: eight columns
@@ -580,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attn_tc_kernel(const __gri
 #pragma unroll
               for (int b = 0; b < 4; ++b)  // (1024 + low nibble, 64 + high nibble) - (1032, 72): c - 8
                 h[b] = mm4::hsub2_u(and_or(__byte_perm(w[e], 0u, 0x4040u | (0x0101u * b)), 0x00F0000Fu, 0x54006400u), 0x54806408u);
-              sts128(dst + piece_at(r, 4 * ch + e), h[0], h[1], h[2], h[3]);
+              sts128(to + at_chunk[e], h[0], h[1], h[2], h[3]);
             }
           }
         }
@@ -672,9 +677,10 @@ inline int warps_m(int64_t rows) { return rows <= 16 ? 1 : (rows <= 32 ? 2 : 4);
 // Which kernel streams the prefix, when the flags do not say: by its capacity, the lengths being on the device. The
 // tcgen05 kernel's start costs about what one to two thousand slots cost the warp-level one (8 heads of 128, 16 bits, 20
 // own slots, 24 rows: 1,000 slots 11 us against 13, 3,000 12 against 18, 40,000 42 against 44; 256 rows: 27 against 32, 32
-// against 40, 103 against 179). Only for up to 16 rows of 8-bit codes of 128 columns is the warp-level kernel's conversion,
-// which uses no shared memory on the way, the faster one (8 rows: 10,000 slots 18 us against 16, 40,000 44 against 33; 24
-// rows: 22 against 21, 47 against 47; 48 rows: 48 against 67).
+// against 40, 103 against 179). Only for up to 16 rows of 8-bit codes of 128 columns is the warp-level kernel, which
+// converts in registers what the products read, the faster one on the whole (8 heads, 8 rows: 3,000 slots 12.4 us against
+// 12.0, 10,000 17.7 against 16.8, 40,000 35.9 against 33.2; 2 heads 11.3 against 9.9, 14.7 against 14.7, 20.7 against 22.1;
+// 8 heads, 24 rows: 13.2 against 14.7, 21.6 against 21.0, 39.5 against 46.7).
 inline bool use_tc(const rb_prefix_attn_args* a, int rep, int flags) {
   if (!a->prefix || (flags & RB_FLAG_KERNEL_MMA)) return false;
   if (flags & RB_FLAG_KERNEL_TC) return true;

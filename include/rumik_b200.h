@@ -485,8 +485,9 @@ int rb_decode_layers(const rb_decode_step* st, int dtype, int flags, void* strea
  *   RB_KV_PLAIN  the values themselves
  *   RB_KV_INT8   codes + 128 (uint8, the storage of the int8 head) and s = bf16(max|x| / 127), value = code * s,
  *                code = clamp(rint(x / s), -127, 127)
- *   RB_KV_INT4   codes packed two a byte, low nibble = even column, and the pair s = bf16((max x - m) / 15), m = min x
- *                in `dtype`; value = code * s + m, code = clamp(rint((x - m) / s), 0, 15)
+ *   RB_KV_INT4   codes packed two a byte, low nibble = even column, and the pair s = bf16((max x - m) (1 / 15)), m = min x
+ *                in `dtype`; value = code * s + m, code = clamp(rint((x - m) / s), 0, 15). max x - m, 1 / 15 and their
+ *                product are each rounded to fp32: midway between two bf16 values the larger one is taken
  * s == 0 gives codes of zero. A row that holds a NaN or an infinity (or whose range overflows fp32) has s = NaN and
  * codes of zero, so that all of it reads as NaN. */
 enum rb_kv_format { RB_KV_PLAIN = 0, RB_KV_INT8 = 1, RB_KV_INT4 = 2 };

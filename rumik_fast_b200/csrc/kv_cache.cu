@@ -2,8 +2,10 @@
 // back as the values they stand for (rb_kv_write, rb_kv_read). One row is the head_dim values of one (sequence,
 // slot, key-value head):
 //   RB_KV_INT8   s = bf16(max|x| / 127), c = clamp(rint(x / s), -127, 127); the cache holds c + 128 and s
-//   RB_KV_INT4   m = min x (exact in the activation dtype), s = bf16((max x - m) / 15), c = clamp(rint((x - m) / s),
-//                0, 15); the cache holds two codes a byte (low nibble = even column) and the pair (s, m)
+//   RB_KV_INT4   m = min x (exact in the activation dtype), s = bf16((max x - m) (1 / 15)), the product in fp32,
+//                c = clamp(rint((x - m) / s), 0, 15); the cache holds two codes a byte (low nibble = even column) and the
+//                pair (s, m). One fp16 row in 200 has a range midway between two scales, which are then equally good: by
+//                the product with fp32's 1 / 15, a little above it, the larger one is taken, and no division is needed
 //   RB_KV_PLAIN  the row as it is
 // The scale is rounded to bf16 BEFORE the codes are computed against it, so its 8 bits cost nothing (127 s and 15 s
 // stay within half a step of the largest value) and it keeps fp32's range, which an fp16 scale would not. x (11 bits)
@@ -141,7 +143,7 @@ __device__ __forceinline__ void quantise_row(const uint4 raw, bool store, void* 
       lo2 = row_all<kLanes>(lo2, [](uint32_t a, uint32_t d) { return pick2<kBf16, false>(a, d); });
       const uint32_t lo = pick2<kBf16, false>(lo2, lo2 >> 16) & 0xffffu;
       const float m = act_of(lo, kBf16), range = act_of(pick2<kBf16, true>(hi2, hi2 >> 16) & 0xffffu, kBf16) - m;
-      s = range <= 3.402823466e38f ? bf16_round(__fdiv_rn(range, 15.f)) : __int_as_float(0x7fc00000);
+      s = range <= 3.402823466e38f ? bf16_round(range * (1.f / 15.f)) : __int_as_float(0x7fc00000);
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[e] = add2(x[e], make_float2(-m, -m));
       word = lo << 16;

@@ -17,8 +17,8 @@
 // tile's already in flight. (One warp for all MMAs made 17 warps, which leaves 96 registers a thread and spills; four
 // loader warps for both rings paced the whole kernel at 4,100 cycles a tile.)
 //
-// Bound: 16-bit rows by HBM (32,768 slots of 8 heads with 48 rows in 46 us, of which 38 are this kernel: 3.5 TB/s, the rest
-// start and merge). 8-bit codes of up to 64 rows by the loaders, 2,100 cycles a tile of keys or values: conversion, the
+// Bound: 16-bit rows by HBM in the loop over the tiles (64 KB in 2,950 cycles on every SM: 6.1 TB/s), beside 10 us of start
+// and merge (32,768 slots of 8 heads with 48 rows: 46 us). 8-bit codes of up to 64 rows by the loaders, 2,100 cycles a tile of keys or values: conversion, the
 // proxy fence and the loads' latency in turn. More rows by a group's chain of QK, softmax and PV, 6,000 cycles for each of
 // two tiles under way, in any format (100,001 slots of 4 heads with 256 rows, int8: 115 us, 99 of them here, 530 TFLOP/s).
 #include "common.cuh"
@@ -30,7 +30,6 @@ namespace rb {
 namespace pfxt {
 
 using pfx::ex2;
-using pfx::Item;
 using pfx::Params;
 
 constexpr int kTile = 128;        // slots of a tile, and query rows of a CTA

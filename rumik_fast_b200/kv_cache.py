@@ -10,7 +10,7 @@ head_dim values - the granularity of the library's int4 groups:
 
 prefix_attention.PrefixAttention reads these caches in place, beams.BeamReorder permutes them.
 The formats (include/rumik_b200.h, rb_kv_format): int8 value = code * s with s = bf16(max|x| / 127); int4 value =
-code * s + m with s = bf16((max x - min x) / 15) and m = min x. No reference counterpart (its engine keeps a 16-bit
+code * s + m with s = bf16((max x - min x) (1 / 15)), in fp32, and m = min x. No reference counterpart (its engine keeps a 16-bit
 cache of one sequence, engine/rumik_int4.py:118-130).
 """
 import ctypes

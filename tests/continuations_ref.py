@@ -12,7 +12,8 @@ def bf16_of(x):
 
 def quantise(x, fmt):
     """Rows x [..., hd] (fp16 or bf16, on the CPU) -> (codes [..., hd] int64, s, m): value = code * s + m, in 64 bits.
-    The int4 difference x - m is taken in fp32, as the format says (the quotient of the codes is then exact enough)."""
+    The int4 difference x - m and its product with 1 / 15 are taken in fp32, as the format says (the quotient of the
+    codes is then exact enough)."""
     f = x.to(F64)
     if fmt == "int8":
         top = f.abs().amax(-1)
@@ -22,7 +23,7 @@ def quantise(x, fmt):
         return c.to(torch.int64), s, torch.zeros_like(s)
     lo, hi = f.amin(-1), f.amax(-1)
     rng = (x.float().amax(-1) - x.float().amin(-1))
-    s = bf16_of(rng.to(F64) / 15).to(F64)
+    s = bf16_of(rng * torch.tensor(1 / 15, dtype=torch.float32)).to(F64)
     s = torch.where(torch.isfinite(f).all(-1) & torch.isfinite(rng), s, torch.nan)
     d = (x.float() - x.float().amin(-1, keepdim=True)).to(F64)
     c = torch.where((s > 0)[..., None], torch.round(d / torch.where(s > 0, s, 1.0)[..., None]).clamp(0, 15), 0.0)

@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(kThreads, kSelectCtas) beam_select_kernel(cons
 
 // Of every (tensor, beam head) line the columns are independent: a thread holds one column of all beams, so any permutation
 // or copying of beams is done in place and each row is read once, however many beams take it over. HBM-bound: 72 tensors
-// of 8 beams with 701 slots, 0.72 GB, 130 us (0.85 of the measured copy bandwidth). One launch for up to kMaxTensors
+// of 8 beams with 701 slots, 0.72 GB, 130 to 139 us (0.79 to 0.85 of the measured copy bandwidth). One launch for up to kMaxTensors
 // tensors, which is what counts for small states: 8 tensors of 61 slots 3 us.
 constexpr int kReorderThreads = 128;
 

@@ -152,15 +152,16 @@ __device__ __forceinline__ void cta_top(Shared& sh, int k, int n, Get get, Out o
 }
 
 // Whether this CTA is the last of `of` to arrive at the ticket, which is then zero again. What the others wrote
-// before they arrived is visible to the last one's loads through L2.
+// before they arrived is visible to the last one's loads: the barrier puts a CTA's writes before its one thread's
+// release, and that thread's acquire before the loads.
 __device__ __forceinline__ bool last_to_arrive(Shared& sh, unsigned int* ticket, int of) {
-  __threadfence();
   __syncthreads();
   if (threadIdx.x == 0) {
-    const bool last = atomicAdd(ticket, 1u) + 1u == static_cast<unsigned>(of);
+    unsigned int before;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(ticket) : "memory");
+    const bool last = before + 1u == static_cast<unsigned>(of);
     if (last) *ticket = 0u;
     sh.last = last;
-    __threadfence();
   }
   __syncthreads();
   return sh.last != 0;

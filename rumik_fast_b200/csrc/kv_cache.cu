@@ -15,8 +15,7 @@
 // the attention. s == 0 (a row of equal values, or of zeros) gives codes of zero.
 // Bound: HBM for prompts, each byte moved once. 65,536 tokens of 8 heads of 128 in int8, written and read back: 145 to
 // 160 us for 0.81 GB, 0.77 to 0.85 of the measured copy bandwidth; 4,099 tokens in int4 14 us for 42 MB (0.45: a few waves
-// of CTAs). One
-// token of 16 sequences is two launches of 2 us, all latency.
+// of CTAs). One token of 16 sequences is two launches of 2 us, all latency.
 #include "common.cuh"
 #include "kernels.h"
 

@@ -797,11 +797,12 @@ __global__ void __launch_bounds__(kThreads, F::kCtas) prefix_attn_kernel(const _
 }
 
 // A CTA joins the partials of one (sequence, query head): prefix splits, then own splits. Warp w takes every fourth
-// one, eight loads at a time; their sums are added in warp order.
+// one, eight loads at a time, under a reference of its own (one for all would be another round trip to L2 before the
+// loads); the warps' sums are joined in warp order. Latency-bound: the launch and two dependent loads.
 template <int kHd>
 __global__ void __launch_bounds__(kThreads) prefix_attn_merge(const __grid_constant__ Params p, int tile_rows, int stage) {
   constexpr int kE = kHd / 32;
-  __shared__ float so[kWarps][kHd], sl[kWarps];
+  __shared__ float so[kWarps][kHd], sl[kWarps], sr[kWarps];
   griddep_wait();
   griddep_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -821,11 +822,7 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_merge(const __grid_const
   const int64_t y0 = p.own_rl + (static_cast<int64_t>(b) * p.n_kv + kv) * p.max_ns * p.rep + j;
   auto at = [&](int i) { return i < np ? x0 + static_cast<int64_t>(i) * tile_rows : y0 + static_cast<int64_t>(i - np) * p.rep; };
   const int n = np + ns;
-  float hi = -INFINITY;
-  for (int i = lane; i < n; i += 32) hi = fmaxf(hi, __ldcg(p.rl + at(i)).x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-  float acc[kE], l = 0.f;
+  float acc[kE], l = 0.f, hi = -INFINITY;
 #pragma unroll
   for (int e = 0; e < kE; ++e) acc[e] = 0.f;
   for (int i0 = warp; i0 < n; i0 += 8 * kWarps) {
@@ -849,6 +846,14 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_merge(const __grid_const
         }
       }
     }
+    float top = hi;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) top = fmaxf(top, v[k].x);
+    const float down = hi == -INFINITY ? 0.f : ex2(hi - top);
+    hi = top;
+    l *= down;
+#pragma unroll
+    for (int e = 0; e < kE; ++e) acc[e] *= down;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       if (v[k].x == -INFINITY) continue;  // nothing there: its sums may not have been written
@@ -860,13 +865,18 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_merge(const __grid_const
   }
 #pragma unroll
   for (int e = 0; e < kE; ++e) so[warp][lane * kE + e] = acc[e];
-  if (lane == 0) sl[warp] = l;
+  if (lane == 0) sl[warp] = l, sr[warp] = hi;
   __syncthreads();
   if (threadIdx.x < kHd / 2) {
     const int d = 2 * threadIdx.x;
     float x = 0.f, y = 0.f, lt = 0.f;
+    const float top = fmaxf(fmaxf(sr[0], sr[1]), fmaxf(sr[2], sr[3]));
+    static_assert(kWarps == 4, "the warps' references");
 #pragma unroll
-    for (int k = 0; k < kWarps; ++k) x += so[k][d], y += so[k][d + 1], lt += sl[k];
+    for (int k = 0; k < kWarps; ++k) {
+      const float f = sr[k] == -INFINITY ? 0.f : ex2(sr[k] - top);
+      x = fmaf(so[k][d], f, x), y = fmaf(so[k][d + 1], f, y), lt = fmaf(sl[k], f, lt);
+    }
     const bool none = n_pre + n_own == 0;
     x = none ? 0.f : x / lt;
     y = none ? 0.f : y / lt;

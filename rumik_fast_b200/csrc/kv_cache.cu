@@ -13,9 +13,8 @@
 // depend on how wide the quotient is computed.
 // A row with a NaN or an infinity gets s = NaN and codes of zero: all of it reads back as NaN, in this kernel and in
 // the attention. s == 0 (a row of equal values, or of zeros) gives codes of zero.
-// Bound: HBM for prompts, each byte moved once. 65,536 tokens of 8 heads of 128 in int8, written and read back: 145 to
-// 160 us for 0.81 GB, 0.77 to 0.85 of the measured copy bandwidth; 4,099 tokens in int4 14 us for 42 MB (0.45: a few waves
-// of CTAs). One token of 16 sequences is two launches of 2 us, all latency.
+// Bound: HBM for prompts, each byte moved once. 65,536 tokens of 8 heads of 128 in int8, written and read back: 135 us
+// for 0.81 GB, 0.92 of the measured copy bandwidth; 4,099 tokens in int4 12 us for 42 MB (0.55: a few waves of CTAs). One token of 16 sequences is two launches of 2 us, all latency.
 #include "common.cuh"
 #include "kernels.h"
 
@@ -129,9 +128,11 @@ __device__ __forceinline__ void quantise_row(const uint4 raw, bool store, void* 
     float s;
     uint32_t word = 0u;
     if constexpr (kFmt == RB_KV_INT8) {
-      // the order of the magnitudes' bits is the order of the magnitudes, with infinity and NaN above the others
-      uint32_t top = __vmaxu2(__vmaxu2(r4[0] & 0x7fff7fffu, r4[1] & 0x7fff7fffu), __vmaxu2(r4[2] & 0x7fff7fffu, r4[3] & 0x7fff7fffu));
-      top = row_all<kLanes>(max(top & 0xffffu, top >> 16), [](uint32_t a, uint32_t d) { return max(a, d); });
+      uint32_t top = r4[0] & 0x7fff7fffu;
+#pragma unroll
+      for (int e = 1; e < 4; ++e) top = pick2<kBf16, true>(top, r4[e] & 0x7fff7fffu);
+      top = row_all<kLanes>(top, [](uint32_t a, uint32_t d) { return pick2<kBf16, true>(a, d); });
+      top = pick2<kBf16, true>(top, top >> 16) & 0xffffu;
       // no 11-bit value is 127 times a 9-bit one: top / 127 is never near a tie of bf16, and the product rounds as it does
       s = bf16_round(act_of(top, kBf16) * (1.f / 127.f));
       if (top >= (kBf16 ? 0x7f80u : 0x7c00u)) s = __int_as_float(0x7fc00000);
@@ -251,72 +252,84 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constan
 
 // fp32 -> the activation dtype, clamped to its finite range (15 s + m of a row that reaches fp16's largest value may
 // round past it); NaN stays NaN.
-__device__ __forceinline__ uint32_t pack_act2(float a, float b, bool bf16) {
-  const float top = bf16 ? 3.3895313892515355e38f : 65504.f;
-  a = a > top ? top : (a < -top ? -top : a);
-  b = b > top ? top : (b < -top ? -top : b);
-  if (bf16) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack_act2(float2 v) {
+  uint32_t d;
+  if constexpr (kBf16) asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(v.y), "f"(v.x));
+  else asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(v.y), "f"(v.x));
+  return d;
+}
+
+// The values of eight codes in `raw` (int8: two words; int4: one) under the row's parameters.
+template <int kFmt, bool kBf16>
+__device__ __forceinline__ uint4 values_of(const uint2 raw, uint32_t word) {
+  const float s = __uint_as_float(word << 16);
+  uint32_t o[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (kFmt == RB_KV_INT8) {  // a byte under 2^23's exponent, less 2^23 + 128
+      const uint32_t w = e < 2 ? raw.x : raw.y, at = 2 * (e & 1);
+      const float2 c = make_float2(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440 + at)), __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7441 + at)));
+      o[e] = pack_act2<kBf16>(mul2(add2(c, make_float2(-8388736.f, -8388736.f)), make_float2(s, s)));
+    } else {
+      const float m = act_of(word >> 16, kBf16);
+      const float2 c = make_float2(__uint_as_float(((raw.x >> (8 * e)) & 15u) | 0x4B000000u), __uint_as_float(((raw.x >> (8 * e + 4)) & 15u) | 0x4B000000u));
+      o[e] = pack_act2<kBf16>(fma2(add2(c, make_float2(-8388608.f, -8388608.f)), make_float2(s, s), make_float2(m, m)));
+    }
   }
-  const __half2 v = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&v);
+  return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
 // A CTA reads kThreads x kUnits pieces of eight values of one (key or value, sequence, head); its loads go out first.
-// HBM-bound: the values that it writes are two to four times the codes it reads.
+// HBM-bound: the values that it writes are two to four times the codes it reads. A thread's pieces are kThreads apart, so
+// their addresses and their rows' differ by constants.
 constexpr int kUnits = 4;
 
 template <int kHd, int kFmt>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant__ ReadParams p) {
-  constexpr int kLanes = kHd / 8;
+  constexpr int kLanes = kHd / 8, kRowsApart = kThreads / kLanes;
   griddep_wait();
   griddep_launch_dependents();
   const uint32_t line = blockIdx.x / p.tiles;
   const int64_t u0 = static_cast<int64_t>(blockIdx.x - line * p.tiles) * (kThreads * kUnits) + threadIdx.x, units = p.count * kLanes;
   const int which = line >= p.heads;
   const int64_t bh = which ? line - p.heads : line, src = bh * p.cache_len + p.start;
-  uint4* out = reinterpret_cast<uint4*>(p.out[which]) + bh * units;
-  uint4 raw[kUnits];
-  uint32_t word[kUnits];
+  const int left = static_cast<int>(min(max(units - u0, int64_t(0)), int64_t(kThreads * kUnits)));  // piece i is there: i kThreads < left
+  uint4* out = reinterpret_cast<uint4*>(p.out[which]) + bh * units + u0;
+  const int64_t at = src * kLanes + u0, row = src + u0 / kLanes;
+  if constexpr (kFmt == RB_KV_PLAIN) {
+    const uint4* from = reinterpret_cast<const uint4*>(p.c[which]) + at;
+    uint4 raw[kUnits];
 #pragma unroll
-  for (int i = 0; i < kUnits; ++i) {
-    const int64_t u = u0 + i * kThreads;
-    raw[i] = make_uint4(0u, 0u, 0u, 0u);
-    word[i] = 0u;
-    if (u >= units) continue;
-    const int64_t at = src * kLanes + u;
-    if constexpr (kFmt == RB_KV_PLAIN) {
-      raw[i] = ldg_cg_128(reinterpret_cast<const uint4*>(p.c[which]) + at);
-    } else if constexpr (kFmt == RB_KV_INT8) {
-      const uint2 w = __ldcg(reinterpret_cast<const uint2*>(p.c[which]) + at);
-      raw[i].x = w.x, raw[i].y = w.y;
-      word[i] = __ldcg(reinterpret_cast<const unsigned short*>(p.par[which]) + src + u / kLanes);
-    } else {
-      raw[i].x = __ldcg(reinterpret_cast<const unsigned int*>(p.c[which]) + at);
-      word[i] = __ldcg(reinterpret_cast<const unsigned int*>(p.par[which]) + src + u / kLanes);
-    }
-  }
+    for (int i = 0; i < kUnits; ++i)
+      if (i * kThreads < left) raw[i] = ldg_cg_128(from + i * kThreads);
 #pragma unroll
-  for (int i = 0; i < kUnits; ++i) {
-    const int64_t u = u0 + i * kThreads;
-    if (u >= units) continue;
-    if constexpr (kFmt == RB_KV_PLAIN) {
-      out[u] = raw[i];
-    } else {
-      float v[8];
-      const float s = __uint_as_float(word[i] << 16);
+    for (int i = 0; i < kUnits; ++i)
+      if (i * kThreads < left) out[i * kThreads] = raw[i];
+  } else {
+    uint2 raw[kUnits];
+    uint32_t word[kUnits];
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+      raw[i] = make_uint2(0u, 0u);
+      word[i] = 0u;
+      if (i * kThreads >= left) continue;
       if constexpr (kFmt == RB_KV_INT8) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)  // byte e under 2^23's exponent, less 2^23 + 128
-          v[e] = (__uint_as_float(__byte_perm(e < 4 ? raw[i].x : raw[i].y, 0x4B000000u, 0x7440 + (e & 3))) - 8388736.f) * s;
+        raw[i] = __ldcg(reinterpret_cast<const uint2*>(p.c[which]) + at + i * kThreads);
+        word[i] = __ldcg(reinterpret_cast<const unsigned short*>(p.par[which]) + row + i * kRowsApart);
       } else {
-        const float m = p.bf16 ? __uint_as_float(word[i] & 0xffff0000u) : __half2float(__ushort_as_half(static_cast<unsigned short>(word[i] >> 16)));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = fmaf(__uint_as_float(((raw[i].x >> (4 * e)) & 15u) | 0x4B000000u) - 8388608.f, s, m);
+        raw[i].x = __ldcg(reinterpret_cast<const unsigned int*>(p.c[which]) + at + i * kThreads);
+        word[i] = __ldcg(reinterpret_cast<const unsigned int*>(p.par[which]) + row + i * kRowsApart);
       }
-      out[u] = make_uint4(pack_act2(v[0], v[1], p.bf16), pack_act2(v[2], v[3], p.bf16), pack_act2(v[4], v[5], p.bf16),
-                          pack_act2(v[6], v[7], p.bf16));
+    }
+    if (p.bf16) {
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i)
+        if (i * kThreads < left) out[i * kThreads] = values_of<kFmt, true>(raw[i], word[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i)
+        if (i * kThreads < left) out[i * kThreads] = values_of<kFmt, false>(raw[i], word[i]);
     }
   }
 }

@@ -36,7 +36,6 @@ struct WriteParams {
   const int64_t* pos;
   int64_t n_tokens, cache_len;
   uint32_t n_seqs, n_heads, tiles;  // tiles: CTAs of one (key or value, sequence)
-  int by_head;
 };
 
 struct ReadParams {
@@ -373,13 +372,13 @@ int launch_kv_write(const rb_kv_cache* c, const void* k, const void* v, const in
   p.n_heads = static_cast<uint32_t>(c->n_kv_heads);
   p.n_seqs = static_cast<uint32_t>(c->n_seqs);
   const int64_t groups = kThreads / (c->head_dim / 8), tile = groups * kRows;
-  p.by_head = n_tokens >= groups;
-  const int64_t tiles = p.by_head ? (n_tokens + tile - 1) / tile * c->n_kv_heads : (n_tokens * c->n_kv_heads + tile - 1) / tile;
+  const bool by_head = n_tokens >= groups;
+  const int64_t tiles = by_head ? (n_tokens + tile - 1) / tile * c->n_kv_heads : (n_tokens * c->n_kv_heads + tile - 1) / tile;
   const int64_t blocks = 2 * c->n_seqs * tiles;
   if (blocks > (int64_t(1) << 31) - 1) return RB_ERR_SHAPE;
   p.tiles = static_cast<uint32_t>(tiles);
   const bool bf = c->dtype == RB_BF16, wide = c->head_dim == 128;
-  void (*kern)(WriteParams) = p.by_head ? write_kernel<true>(c->fmt, wide, bf) : write_kernel<false>(c->fmt, wide, bf);
+  void (*kern)(WriteParams) = by_head ? write_kernel<true>(c->fmt, wide, bf) : write_kernel<false>(c->fmt, wide, bf);
   return launch(kern, p, blocks, flags, stream);
 }
 

@@ -807,10 +807,15 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_merge(const __grid_const
   griddep_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int b = blockIdx.x / p.n_q, h = blockIdx.x % p.n_q, kv = h / p.rep, j = h % p.rep;
-  const int64_t n_pre = p.pre.k ? __ldcg(p.pre.len) : 0, n_own = p.own.k ? __ldcg(p.own.len + b) : 0;
-  const int ot = __ldcg(p.plan + 3);
-  int np = __ldcg(p.plan);
-  if (n_pre < 0 || n_pre > p.pre.cache_len || n_own < 0 || n_own > p.own.cache_len) return;
+  const int64_t n_pre = p.pre.len ? __ldcg(p.pre.len) : 0, n_own = p.own.len ? __ldcg(p.own.len + b) : 0;
+  // prefix_attn_kernel leaves the plan, and runs where there are rows for it: a cache without slots has no kernel
+  const bool planned = p.own.k || (p.pre.k && p.parts == 1);
+  const int ot = planned ? __ldcg(p.plan + 3) : 0;
+  int np = planned ? __ldcg(p.plan) : 0;
+  if (n_pre < 0 || n_pre > p.pre.cache_len || n_own < 0 || n_own > p.own.cache_len) {
+    if (threadIdx.x == 0) atomicOr(&g_device_error, static_cast<unsigned>(ERR_ARG));
+    return;
+  }
   if (p.parts == 2) {  // the tcgen05 kernel's splits: the tiles dealt evenly, two partials each
     const int tiles = static_cast<int>((n_pre + 127) / 128), per = tiles_of_split(tiles, p.max_np);
     np = 2 * ((tiles + per - 1) / per);

@@ -767,11 +767,13 @@ int launch_prefix_attn(const rb_prefix_attn_args* a, int num_sms, int flags, cud
   p.out = a->out;
   p.ldq = a->ldq;
   p.ldo = a->ldo;
+  // k is null where there is no row to read, len where there is no cache: a cache without slots still has its lengths checked
   auto side = [](const rb_kv_cache* s, const int64_t* len) {
-    return Side{static_cast<const uint8_t*>(s->k), static_cast<const uint8_t*>(s->v), s->k_par, s->v_par, len, s->cache_len};
+    const bool rows = s->cache_len > 0;
+    return Side{rows ? static_cast<const uint8_t*>(s->k) : nullptr, static_cast<const uint8_t*>(s->v), s->k_par, s->v_par, len, s->cache_len};
   };
-  if (a->prefix && a->prefix->cache_len) p.pre = side(a->prefix, a->prefix_len);
-  if (a->own && a->own->cache_len) p.own = side(a->own, a->own_len);
+  if (a->prefix) p.pre = side(a->prefix, a->prefix_len);
+  if (a->own) p.own = side(a->own, a->own_len);
   p.n_seqs = static_cast<int>(a->n_seqs);
   p.n_q = a->n_q_heads;
   p.n_kv = c->n_kv_heads;

@@ -361,3 +361,47 @@ def test_refusals():
     wide = torch.zeros(2, 34, 64, dtype=torch.float16, device=DEV)
     with pytest.raises(RuntimeError):      # seventeen query heads a key-value head
         PrefixAttention(wide, torch.empty_like(wide), **ok)
+
+
+@pytest.mark.parametrize("kernel", ["mma", "tc"])
+@pytest.mark.parametrize("fmt", ["plain", "int8", "int4"])
+@pytest.mark.parametrize("pre_slots,own_slots", [(0, None), (None, 0), (0, 0), (0, 40), (300, 0)])
+def test_caches_without_a_slot(pre_slots, own_slots, fmt, kernel):
+    """Caches of no slots alone, together and beside one with rows, over a workspace that holds anything: zeros where there
+    is nothing to attend to, and a length above zero is one outside its cache."""
+    B, nkv, hd = 3, 2, 64
+    q = rows((B, 4, hd), torch.float16, 41)
+    out = torch.full((B, 4, hd), 7.0, dtype=torch.float16, device=DEV)
+    kw, vals = {}, {}
+    for nm, n, slots in (("prefix", 1, pre_slots), ("own", B, own_slots)):
+        if slots is None:
+            continue
+        full = KVCache(n, nkv, max(slots, 1), hd, fmt)
+        if slots:
+            k, v = rows((n, slots, nkv, hd), torch.float16, 42), rows((n, slots, nkv, hd), torch.float16, 43)
+            full.write(k.to(DEV), v.to(DEV), torch.zeros(n, dtype=torch.int64, device=DEV))
+            vals[nm] = tuple(ref.values(x, fmt).transpose(1, 2) for x in (k, v))
+        else:
+            full = KVCache.wrap(*(t if t is None else t[:, :, :0].contiguous() for t in (full.k, full.v, full.k_par, full.v_par)), dtype=full.dtype)
+        kw[nm], kw[nm + "_len"] = full, torch.full((n,), slots, dtype=torch.int64, device=DEV)
+    attn = PrefixAttention(q.to(DEV), out, kernel=kernel, **kw)
+    attn.ws.fill_(1)
+    attn()
+    assert rb.device_error() == 0
+    if vals:
+        pre = tuple(x[0] for x in vals["prefix"]) if "prefix" in vals else None
+        want, bound = ref.attention(q, pre, vals.get("own"), [own_slots] * B, hd ** -0.5, 2.0 ** -11)
+        assert ((out.cpu().double() - want).abs() <= want.abs() * 2.0 ** -11 * (1 + 2 ** -7) + bound * (1 + 2.0 ** -11) + 2.0 ** -25).all()
+    else:
+        assert not out.any()
+    if pre_slots == 0:
+        kw["prefix_len"].fill_(1)
+        out.fill_(7)
+        attn()
+        assert rb.device_error() == rb._lib.DEVERR_ARG and (out == 7).all()
+        kw["prefix_len"].zero_()
+    if own_slots == 0:
+        kw["own_len"][1] = 1
+        out.fill_(7)
+        attn()
+        assert rb.device_error() == rb._lib.DEVERR_ARG and (out[1] == 7).all() and not (out[0] == 7).any() and not (out[2] == 7).any()

@@ -35,6 +35,7 @@ constexpr int kThreads = kWarps * 32;
 constexpr bool wide_steps(int fmt, int hd) { return fmt != RB_KV_PLAIN && hd == 128; }
 constexpr int ctas_per_sm(int fmt, int hd) { return wide_steps(fmt, hd) ? 2 : 3; }
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLeastFactor = 1.17549435e-38f;  // of a row's scores: the smallest normal number, so that a masked slot's -inf stays -inf
 constexpr float kSlack = 8.f;     // a row's reference is raised when a score exceeds it by this (log2)
 constexpr float kLowestE = -90.f; // exponent range of the value scales folded into the reference
 constexpr float kHighestE = 90.f;
@@ -408,7 +409,7 @@ __device__ __forceinline__ void run_item(const Params& p, const Item it, const i
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
-    float f = fmaxf(fabsf(p.scale) * kLog2e, 1e-30f);
+    float f = fabsf(p.scale) * kLog2e;
     float sum = 0.f;
     if (!F::kPlain && p.bf16) {
       // fp16 queries for the codes' product: scaled by a power of two so that the row's largest is in [1, 2) - exact
@@ -448,7 +449,7 @@ __device__ __forceinline__ void run_item(const Params& p, const Item it, const i
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
     }
-    fr[x] = f;
+    fr[x] = fmaxf(f, kLeastFactor);
     qs[x] = sum;
   }
   store_par();

@@ -621,7 +621,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attn_tc_kernel(const __gri
 #pragma unroll
       for (int i = 0; i < F::kHd / 8; ++i) q[i] = on ? ldg_cg_128(src + i) : make_uint4(0u, 0u, 0u, 0u);
       const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
-      float f = fmaxf(fabsf(p.scale) * pfx::kLog2e, 1e-30f), sum = 0.f, down = 1.f;
+      float f = fabsf(p.scale) * pfx::kLog2e, sum = 0.f, down = 1.f;
       if constexpr (!F::kPlain) {
         uint32_t top = 0u;
 #pragma unroll
@@ -652,7 +652,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attn_tc_kernel(const __gri
         }
         sts128(s0 + piece_at(lane_row, i), w[0], w[1], w[2], w[3]);
       }
-      rowf[lane_row] = f;
+      rowf[lane_row] = fmaxf(f, pfx::kLeastFactor);
       qsum[lane_row] = flip ? -sum : sum;
       fence_proxy_async_smem();
     }

@@ -405,3 +405,18 @@ def test_caches_without_a_slot(pre_slots, own_slots, fmt, kernel):
         out.fill_(7)
         attn()
         assert rb.device_error() == rb._lib.DEVERR_ARG and (out[1] == 7).all() and not (out[0] == 7).any() and not (out[2] == 7).any()
+
+
+@pytest.mark.parametrize("kernel", ["mma", "tc"])
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("fmt", ["plain", "int8", "int4"])
+@pytest.mark.parametrize("scale", [0.0, 1e-20, -1e-30])
+def test_no_scale_and_no_query(fmt, dtype, kernel, scale):
+    """A scale of zero, or next to it, over query rows of zeros: every visible slot weighs the same."""
+    s = Setup(5, 8, 2, 64, 300, [3, 0, 1, 70, 2], fmt, dtype, seed=31)
+    s.q[:, ::2] = 0
+    s.attn._keep[0].copy_(s.q)
+    s.scale = scale
+    PrefixAttention(s.attn._keep[0], s.out, prefix=s.pre, prefix_len=s.prefix_len, own=s.own, own_len=s.own_len, scale=scale,
+                    kernel=kernel)()
+    s.check()

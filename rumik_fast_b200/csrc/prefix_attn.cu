@@ -8,8 +8,16 @@
 //
 // The query rows of one key-value head, r = b rep + j over the whole batch, share its keys: they are the M side of the
 // two products. One pass over the slots keeps, per row, a reference R (log2 units), l = sum 2^(t - R) and
-// O = sum 2^(t - R) v in fp32 (t: the score times log2 e). R is only raised when a score exceeds it by more than 2^8,
-// so the accumulators are rarely rescaled; any R gives the same O / l.
+// O = sum 2^(t - R) v in fp32 (t: the score times log2 e). Any R gives the same O / l. It is chosen for the 16-bit factor
+// of the second product, 2^(t - R) s: R is the largest t + e so far, e the exponent of the slot's value scale (0 for 16-bit
+// rows), less kRoom, and is only raised when a slot exceeds it by kSlack more, so the accumulators are rarely rescaled. So
+// what counts is a slot's weight times its values: one of large values and no weight takes no accuracy from the others,
+// nor does one of much weight and no values (a reference from the scores and the largest scale by themselves would).
+//
+// 16 bits hold, beside the caches' own rounding: the factors 2^(t - R) s, rounded to fp16 (2^-11 of themselves, 2^-31 of the
+// row's largest where they are subnormal; 4-bit rows add the remainder as a second term), or for bf16 rows to bf16 (2^-8:
+// products on the tensor cores take both operands in one type); and bf16 queries over codes, as fp16 under a power of
+// two of their row. l sums the factors before they are rounded, in fp32 like the scores and O.
 //
 // Work is cut along the slots so that every SM streams a share of the caches: CTAs take (key-value head, 16 wm rows,
 // split of the prefix) or (sequence, key-value head, split of its own rows) items and leave an fp32 partial
@@ -36,9 +44,11 @@ constexpr bool wide_steps(int fmt, int hd) { return fmt != RB_KV_PLAIN && hd == 
 constexpr int ctas_per_sm(int fmt, int hd) { return wide_steps(fmt, hd) ? 2 : 3; }
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLeastFactor = 1.17549435e-38f;  // of a row's scores: the smallest normal number, so that a masked slot's -inf stays -inf
-constexpr float kSlack = 8.f;     // a row's reference is raised when a score exceeds it by this (log2)
-constexpr float kLowestE = -90.f; // exponent range of the value scales folded into the reference
-constexpr float kHighestE = 90.f;
+// t + e of a row's slots stays below R + kRoom + kSlack, so that 2^(t - R) s < 2^15 and fits fp16; the largest is at least
+// 2^kRoom, which keeps factors down to 2^-20 of it normal numbers.
+constexpr float kRoom = 6.f, kSlack = 8.f;
+constexpr int kLeastE = -80;      // of e: 2^(t - R) is at most 2^94, and sums of 2^27 of them are finite
+constexpr int kBelowM = 60;       // e is at least the exponent of a 4-bit row's m less this: 2^(t - R) m is finite, too
 
 struct Side {
   const uint8_t* k;
@@ -70,6 +80,19 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// v 2^d for d <= 0, also where 2^d is below fp32's range: references lie as far apart as value scales do, and the sums under
+// the lower one as far above one.
+__device__ __forceinline__ float lowered(float v, float d) {
+  const float h = ex2(0.5f * d);
+  return v * h * h;
+}
+
+// A value row's e, from its scale and (4-bit rows, else 0) the middle of its range. A NaN scale shows by itself.
+__device__ __forceinline__ float value_exponent(float s, float m) {
+  const int es = static_cast<int>(__float_as_uint(s) >> 23), em = static_cast<int>((__float_as_uint(m) >> 23) & 255u) - kBelowM;
+  return s == s ? static_cast<float>(max(max(es, em) - 127, kLeastE)) : static_cast<float>(kLeastE);
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
@@ -146,7 +169,8 @@ struct Fmt {
   static constexpr int kCtas = ctas_per_sm(kFmt, kHd);
   static constexpr int kTile = wide_steps(kFmt, kHd) ? 128 : 64;  // slots of a stage
   static constexpr int kSide = kTile * kRow;       // bytes of a stage's keys (or values)
-  static constexpr int kPar = kPlain ? 0 : kTile * 4 * (kFmt == RB_KV_INT4 ? 4 : 2);  // fp32 s (and m) of keys, values
+  static constexpr int kE = kFmt == RB_KV_INT4 ? 4 : 2;  // a stage's parameters in fp32, kTile each: s of keys, of values, (m of keys, of values,) e of values
+  static constexpr int kPar = kPlain ? 0 : kTile * 4 * (kE + 1);
   static constexpr int kStage = 2 * kSide + kPar;
 
   // 16-byte chunk `ch` of row `r` in the key (value) tile; conflict-free for the loads below
@@ -378,9 +402,12 @@ __device__ __forceinline__ void run_item(const Params& p, const Item it, const i
         const int x = i * kThreads + tid;
         const float sc = __uint_as_float(par[i] << 16);
         dst[x] = sc;
-        if constexpr (F::kFmt == RB_KV_INT4)  // codes enter as c - 8: m + 8 s stands for the middle of the row's range
-          dst[2 * F::kTile + x] =
-              fmaf(8.f, sc, p.bf16 ? __uint_as_float(par[i] & 0xffff0000u) : __half2float(__ushort_as_half(static_cast<unsigned short>(par[i] >> 16))));
+        float mid = 0.f;
+        if constexpr (F::kFmt == RB_KV_INT4) {  // codes enter as c - 8: m + 8 s stands for the middle of the row's range
+          mid = fmaf(8.f, sc, p.bf16 ? __uint_as_float(par[i] & 0xffff0000u) : __half2float(__ushort_as_half(static_cast<unsigned short>(par[i] >> 16))));
+          dst[2 * F::kTile + x] = mid;
+        }
+        if (x >= F::kTile) dst[(F::kE - 1) * F::kTile + x] = value_exponent(sc, mid);
       }
     }
   };
@@ -466,7 +493,6 @@ __device__ __forceinline__ void run_item(const Params& p, const Item it, const i
   }
 
   float o[F::kNv][4], l[2], w[2], ref[2];
-  float ve = F::kPlain ? 0.f : kLowestE;  // exponent of the value scales seen, part of every row's reference
 #pragma unroll
   for (int u = 0; u < F::kNv; ++u)
 #pragma unroll
@@ -536,39 +562,32 @@ __device__ __forceinline__ void run_item(const Params& p, const Item it, const i
             if (b0 + 8 * n + 2 * c + (e & 1) >= left) s[n][e] = -INFINITY;
       }
 #pragma unroll
-      for (int n = 0; n < T::kNt; ++n)
+      for (int n = 0; n < T::kNt; ++n) {
+        float2 ev = make_float2(0.f, 0.f);
+        if constexpr (!F::kPlain) ev = lds64f(pt + (F::kE * F::kTile + b0 + 8 * n + 2 * c) * 4);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
-      bool raise = top[0] * fr[0] > ref[0] + kSlack || top[1] * fr[1] > ref[1] + kSlack;
-      float ven = ve;
-      if constexpr (!F::kPlain) {
-        // the block's largest value scale (NaN left out: it shows by itself): its exponent goes into the reference,
-        // so that the 16-bit p s stay within fp16's range whatever the size of the values
-        const float vs = __uint_as_float(lds32(pt + (F::kTile + b0 + (lane & (T::kBlock - 1))) * 4));
-        const uint32_t hi = __reduce_max_sync(0xffffffffu, vs == vs ? __float_as_uint(vs) : 0u);
-        ven = fmaxf(ve, fminf(fmaxf(static_cast<float>(static_cast<int>(hi >> 23) - 127), kLowestE), kHighestE));
-        raise |= ven > ve;
+        for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], F::kPlain ? s[n][e] : fmaf(s[n][e], fr[e >> 1], (e & 1) ? ev.y : ev.x));
       }
-      if (__any_sync(0xffffffffu, raise)) {
+      if constexpr (F::kPlain) top[0] *= fr[0], top[1] *= fr[1];
+      if (__any_sync(0xffffffffu, top[0] > ref[0] + (kRoom + kSlack) || top[1] > ref[1] + (kRoom + kSlack))) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           float v = top[x];
           v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
           v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
-          const float nr = fmaxf(ref[x], v * fr[x]);
-          const float f = ref[x] == -INFINITY ? 0.f : ex2((ref[x] - nr) + (ve - ven));
+          const float nr = fmaxf(ref[x], v - kRoom);
+          const float d = ref[x] == -INFINITY ? -INFINITY : ref[x] - nr, f = ex2(d);
           ref[x] = nr;
-          l[x] *= f;
-          if constexpr (F::kFmt == RB_KV_INT4) w[x] *= f;
+          l[x] = lowered(l[x], d);
+          if constexpr (F::kFmt == RB_KV_INT4) w[x] = lowered(w[x], d);
 #pragma unroll
           for (int u = 0; u < F::kNv; ++u) o[u][2 * x] *= f, o[u][2 * x + 1] *= f;
         }
-        ve = ven;
       }
       // ---- probabilities ----
       float base[2];
 #pragma unroll
-      for (int x = 0; x < 2; ++x) base[x] = ref[x] == -INFINITY ? 0.f : -(ref[x] + ve);
+      for (int x = 0; x < 2; ++x) base[x] = ref[x] == -INFINITY ? 0.f : -ref[x];
 #pragma unroll
       for (int n = 0; n < T::kNt; ++n) {
         const int col = b0 + 8 * n + 2 * c;
@@ -624,7 +643,7 @@ __device__ __forceinline__ void run_item(const Params& p, const Item it, const i
     }
     if (c == 0)
       rl[warp * 16 + x * 8 + g] =
-          make_float2(ref[x] == -INFINITY && l[x] == 0.f ? -INFINITY : (ref[x] == -INFINITY ? 0.f : ref[x] + ve), l[x]);
+          make_float2(ref[x] == -INFINITY && l[x] == 0.f ? -INFINITY : (ref[x] == -INFINITY ? 0.f : ref[x]), l[x]);
   }
   __syncthreads();
   {
@@ -634,13 +653,15 @@ __device__ __forceinline__ void run_item(const Params& p, const Item it, const i
       float hi = -INFINITY;
       for (int k = wm; k < kWarps; k += wm_n) hi = fmaxf(hi, rl[k * 16 + x * 8 + g].x);
       const float mine = rl[warp * 16 + x * 8 + g].x;
-      f[x] = mine == -INFINITY ? 0.f : ex2(mine - hi);
+      // 4-bit rows: half of the way, to be taken twice, as in lowered(); without p m in them, the sums of a warp whose factor
+      // is below fp32's range are nothing beside the others'
+      f[x] = mine == -INFINITY ? 0.f : ex2((F::kFmt == RB_KV_INT4 ? 0.5f : 1.f) * (mine - hi));
     }
     uint8_t* dst = smem + warp * T::kMergeRow;
 #pragma unroll
     for (int u = 0; u < F::kNv; ++u)
       *reinterpret_cast<float4*>(dst + (u * 33 + lane) * 16) =
-          F::kFmt == RB_KV_INT4 ? make_float4((o[u][0] + w[0]) * f[0], (o[u][1] + w[0]) * f[0], (o[u][2] + w[1]) * f[1], (o[u][3] + w[1]) * f[1])
+          F::kFmt == RB_KV_INT4 ? make_float4((o[u][0] + w[0]) * f[0] * f[0], (o[u][1] + w[0]) * f[0] * f[0], (o[u][2] + w[1]) * f[1] * f[1], (o[u][3] + w[1]) * f[1] * f[1])
                                 : make_float4(o[u][0] * f[0], o[u][1] * f[0], o[u][2] * f[1], o[u][3] * f[1]);
   }
   __syncthreads();
@@ -668,7 +689,7 @@ __device__ __forceinline__ void run_item(const Params& p, const Item it, const i
     for (int k = r >> 4; k < kWarps; k += wm_n) hi = fmaxf(hi, rl[k * 16 + (r & 15)].x);
     for (int k = r >> 4; k < kWarps; k += wm_n) {
       const float2 v = rl[k * 16 + (r & 15)];
-      sum += v.x == -INFINITY ? 0.f : v.y * ex2(v.x - hi);
+      sum += v.x == -INFINITY ? 0.f : lowered(v.y, v.x - hi);
     }
     it.rl[r] = make_float2(hi, sum);
   }
@@ -855,18 +876,19 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_merge(const __grid_const
     float top = hi;
 #pragma unroll
     for (int k = 0; k < 8; ++k) top = fmaxf(top, v[k].x);
-    const float down = hi == -INFINITY ? 0.f : ex2(hi - top);
-    hi = top;
-    l *= down;
+    if (hi != -INFINITY) {  // not the first eight: l and acc hold something
+      l = lowered(l, hi - top);
 #pragma unroll
-    for (int e = 0; e < kE; ++e) acc[e] *= down;
+      for (int e = 0; e < kE; ++e) acc[e] = lowered(acc[e], hi - top);
+    }
+    hi = top;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       if (v[k].x == -INFINITY) continue;  // nothing there: its sums may not have been written
-      const float f = ex2(v[k].x - hi);
-      l = fmaf(v[k].y, f, l);
+      const float h = ex2(0.5f * (v[k].x - hi));
+      l = fmaf(v[k].y * h, h, l);
 #pragma unroll
-      for (int e = 0; e < kE; ++e) acc[e] = fmaf(x[k][e], f, acc[e]);
+      for (int e = 0; e < kE; ++e) acc[e] = fmaf(x[k][e] * h, h, acc[e]);
     }
   }
 #pragma unroll
@@ -880,8 +902,8 @@ __global__ void __launch_bounds__(kThreads) prefix_attn_merge(const __grid_const
     static_assert(kWarps == 4, "the warps' references");
 #pragma unroll
     for (int k = 0; k < kWarps; ++k) {
-      const float f = sr[k] == -INFINITY ? 0.f : ex2(sr[k] - top);
-      x = fmaf(so[k][d], f, x), y = fmaf(so[k][d + 1], f, y), lt = fmaf(sl[k], f, lt);
+      const float h = sr[k] == -INFINITY ? 0.f : ex2(0.5f * (sr[k] - top));
+      x = fmaf(so[k][d] * h, h, x), y = fmaf(so[k][d + 1] * h, h, y), lt = fmaf(sl[k] * h, h, lt);
     }
     const bool none = n_pre + n_own == 0;
     x = none ? 0.f : x / lt;

@@ -58,10 +58,10 @@ struct Fmt {
   // fp32 s and m of a tile's keys (values), in the order in which the fragments need them: slot 8 u + 2 c + e at
   // c kParC + 2 u + e, so that a lane reads its columns in sixteen-byte pieces and the four c fall on different banks
   static constexpr int kParC = kTile / 4 + 4, kParN = 4 * kParC;
-  static constexpr int kPar = kPlain ? 0 : kParN * 4 * 2;
+  static constexpr int kPar = kPlain ? 0 : kParN * 4 * 2, kVPar = kPlain ? 0 : kParN * 4 * 3;  // of the values e, too
   static constexpr int kOffK = kTileBytes, kOffV = kOffK + kKRing * kTileBytes, kOffPar = kOffV + kVRing * kTileBytes;
   static constexpr int kOffVPar = kOffPar + kKParRing * kPar;
-  static constexpr int kOffRow = kOffVPar + kVRing * kPar;  // factor and sum of the rows' queries
+  static constexpr int kOffRow = kOffVPar + kVRing * kVPar;  // factor and sum of the rows' queries
   static constexpr int kOffBar = kOffRow + kTile * 8;
   static constexpr int kBars = 2 * kKRing + 2 * kVRing + 2 * 2;
   static constexpr int kSmem = 1024 + kOffBar + kBars * 8 + 16;
@@ -161,7 +161,7 @@ __device__ __forceinline__ void run_softmax(const Params& p, uint32_t s0, uint8_
   const uint32_t tq = tmem + (static_cast<uint32_t>(quad * 32) << 16);
   const uint32_t ts = tq + g * kTile, to = tq + (2 + g) * kTile, half = 16u << 16;  // the second half's lanes
   const bool busy = quad < rows;
-  float fr[2 * kH], qs[2 * kH], ref[2 * kH], ve = F::kPlain ? 0.f : pfx::kLowestE;  // row y of the thread: lane 16 (y / 2) + 8 (y % 2) + l0
+  float fr[2 * kH], qs[2 * kH], ref[2 * kH];  // row y of the thread: lane 16 (y / 2) + 8 (y % 2) + l0
   float l[2 * kH], w[2 * kH];
 #pragma unroll
   for (int y = 0; y < 2 * kH; ++y) {
@@ -199,29 +199,29 @@ __device__ __forceinline__ void run_softmax(const Params& p, uint32_t s0, uint8_
     mm4::tc_fence_after();
     if (busy && ok) {
       const uint32_t kpar = s0 + F::kOffPar + (t % kKParRing) * F::kPar + c * (F::kParC * 4);
-      const uint32_t vpar = s0 + F::kOffVPar + (t % kVRing) * F::kPar + c * (F::kParC * 4);
+      const uint32_t vpar = s0 + F::kOffVPar + (t % kVRing) * F::kVPar + c * (F::kParC * 4);
       // A lane's row parameters of the columns 8 u + 2 c, two u at a time, loaded kAhead steps before they are used: a load
       // from shared memory takes long while the tensor core reads its operands there.
       constexpr int kAhead = F::kFmt == RB_KV_INT4 ? 1 : 2;
-      float4 ps[kAhead], pm[F::kFmt == RB_KV_INT4 ? kAhead : 1];
+      float4 ps[kAhead], pm[F::kFmt == RB_KV_INT4 ? kAhead : 1], pe;
       auto ahead = [&](uint32_t base, int i) {
         if constexpr (!F::kPlain) {
           ps[i % kAhead] = lds128f(base + 16 * i);
           if constexpr (F::kFmt == RB_KV_INT4) pm[i % kAhead] = lds128f(base + F::kParN * 4 + 16 * i);
         }
       };
+      auto ahead_e = [&](int i) {
+        if constexpr (!F::kPlain) pe = lds128f(vpar + 2 * F::kParN * 4 + 16 * i);
+      };
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) ahead(kpar, i);
+      ahead_e(0);
       const int left = static_cast<int>(min(n - static_cast<int64_t>(t) * kTile, int64_t(kTile)));
-      float ven = ve;
-      if constexpr (!F::kPlain) {
-        // the tile's largest value scale: its exponent is part of every row's reference
-        const float4 s = lds128f(vpar + ((lane >> 3) - c) * (F::kParC * 4) + 16 * (lane & 7));
-        auto bits = [](float f) { return f == f ? __float_as_uint(f) : 0u; };  // a NaN shows by itself
-        const uint32_t hi = __reduce_max_sync(0xffffffffu, max(max(bits(s.x), bits(s.y)), max(bits(s.z), bits(s.w))));
-        ven = fmaxf(ve, fminf(fmaxf(static_cast<float>(static_cast<int>(hi >> 23) - 127), pfx::kLowestE), pfx::kHighestE));
-      }
-      // the rows' scores, scaled by the keys' scales, -inf beyond the prefix
+      // the rows' scores, scaled by the keys' scales, -inf beyond the prefix; and the largest score plus exponent of the
+      // value's scale (-inf beyond the prefix), in log2 units
+      float top[2 * kH];
+#pragma unroll
+      for (int y = 0; y < 2 * kH; ++y) top[y] = -INFINITY;
       float x[kH][64];
 #pragma unroll
       for (int h = 0; h < kH; ++h) tmem_ld_frag(ts + h * half, x[h]);
@@ -230,12 +230,14 @@ __device__ __forceinline__ void run_softmax(const Params& p, uint32_t s0, uint8_
       if constexpr (!F::kPlain) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float4 k4 = ps[i % kAhead], m4 = F::kFmt == RB_KV_INT4 ? pm[i % (F::kFmt == RB_KV_INT4 ? kAhead : 1)] : k4;
+          const float4 k4 = ps[i % kAhead], m4 = F::kFmt == RB_KV_INT4 ? pm[i % (F::kFmt == RB_KV_INT4 ? kAhead : 1)] : k4, e4 = pe;
           if (i + kAhead < 8) ahead(kpar, i + kAhead);
+          if (i < 7) ahead_e(i + 1);
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             const int u = 2 * i + q;
             const float2 ks = q ? make_float2(k4.z, k4.w) : make_float2(k4.x, k4.y), km = q ? make_float2(m4.z, m4.w) : make_float2(m4.x, m4.y);
+            const float2 ev = q ? make_float2(e4.z, e4.w) : make_float2(e4.x, e4.y);
 #pragma unroll
             for (int y = 0; y < 2 * kH; ++y) {
               float& a = x[y >> 1][4 * u + 2 * (y & 1)];
@@ -244,6 +246,8 @@ __device__ __forceinline__ void run_softmax(const Params& p, uint32_t s0, uint8_
               if constexpr (F::kFmt == RB_KV_INT8) v = mul2(v, ks);
               else v = fma2(v, ks, mul2(km, make_float2(qs[y], qs[y])));
               a = v.x, b = v.y;
+              v = fma2(v, make_float2(fr[y], fr[y]), ev);
+              top[y] = fmaxf(top[y], fmaxf(v.x, v.y));
             }
           }
         }
@@ -257,14 +261,15 @@ __device__ __forceinline__ void run_softmax(const Params& p, uint32_t s0, uint8_
           for (int i = 0; i < 64; ++i)
             if (8 * (i >> 2) + 2 * c + (i & 1) >= left) x[h][i] = -INFINITY;
       }
-      float top[2 * kH];
-      bool raise = ven > ve;
+      bool raise = false;
 #pragma unroll
       for (int y = 0; y < 2 * kH; ++y) {
-        top[y] = -INFINITY;
+        if constexpr (F::kPlain) {
 #pragma unroll
-        for (int u = 0; u < 16; ++u) top[y] = fmaxf(top[y], fmaxf(x[y >> 1][4 * u + 2 * (y & 1)], x[y >> 1][4 * u + 2 * (y & 1) + 1]));
-        raise |= top[y] * fr[y] > ref[y] + pfx::kSlack;
+          for (int u = 0; u < 16; ++u) top[y] = fmaxf(top[y], fmaxf(x[y >> 1][4 * u + 2 * (y & 1)], x[y >> 1][4 * u + 2 * (y & 1) + 1]));
+          top[y] *= fr[y];
+        }
+        raise |= top[y] > ref[y] + (pfx::kRoom + pfx::kSlack);
       }
       if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
@@ -272,11 +277,11 @@ __device__ __forceinline__ void run_softmax(const Params& p, uint32_t s0, uint8_
           float v = top[y];
           v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
           v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
-          const float nr = fmaxf(ref[y], v * fr[y]);
-          top[y] = ref[y] == -INFINITY ? 0.f : ex2((ref[y] - nr) + (ve - ven));  // the rows' factor from here on
+          const float nr = fmaxf(ref[y], v - pfx::kRoom), d = ref[y] == -INFINITY ? -INFINITY : ref[y] - nr;
+          top[y] = ex2(d);  // O's factor from here on
           ref[y] = nr;
-          l[y] *= top[y];
-          w[y] *= top[y];
+          l[y] = pfx::lowered(l[y], d);
+          w[y] = pfx::lowered(w[y], d);
         }
         if (t >= 2) {  // the group's O holds something: all of it is there, and the next PV waits for this tile's P
           ok = __all_sync(0xffffffffu, mbar_wait(pvdone, ((t >> 1) - 1) & 1, ERR_PFX_WAIT));
@@ -298,7 +303,7 @@ __device__ __forceinline__ void run_softmax(const Params& p, uint32_t s0, uint8_
       // P = 2^(t - R), over the columns that S came from
       float base[2 * kH];
 #pragma unroll
-      for (int y = 0; y < 2 * kH; ++y) base[y] = ref[y] == -INFINITY ? 0.f : -(ref[y] + ven);
+      for (int y = 0; y < 2 * kH; ++y) base[y] = ref[y] == -INFINITY ? 0.f : -ref[y];
 #pragma unroll
       for (int u0 = 0; u0 < 16; u0 += 4) {  // 32 columns: sixteen of packed pairs, and sixteen for their remainders
         uint32_t hi[kH][8], lo[F::kFmt == RB_KV_INT4 ? kH : 1][8];
@@ -338,7 +343,6 @@ __device__ __forceinline__ void run_softmax(const Params& p, uint32_t s0, uint8_
           if constexpr (F::kFmt == RB_KV_INT4) tmem_st_pairs(ts + h * half + 8 * u0 + 16, lo[h]);
         }
       }
-      ve = ven;
       tmem_wait_st();
     }
     mm4::tc_fence_before();
@@ -377,7 +381,7 @@ __device__ __forceinline__ void run_softmax(const Params& p, uint32_t s0, uint8_
     w[y] += __shfl_xor_sync(0xffffffffu, w[y], 2);
     const int r = (8 * y + l0) * 4 + quad;
     if (c == 0 && r < rows)
-      p.rl[first + r] = make_float2(!mine || (ref[y] == -INFINITY && l[y] == 0.f) ? -INFINITY : (ref[y] == -INFINITY ? 0.f : ref[y] + ve), l[y]);
+      p.rl[first + r] = make_float2(!mine || (ref[y] == -INFINITY && l[y] == 0.f) ? -INFINITY : (ref[y] == -INFINITY ? 0.f : ref[y]), l[y]);
   }
   if (mine && busy && ok) {
 #pragma unroll 2
@@ -588,12 +592,16 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attn_tc_kernel(const __gri
             }
           }
         }
-        float* pd = reinterpret_cast<float*>(smem + (keys ? F::kOffPar + (t % kKParRing) * F::kPar : F::kOffVPar + slot * F::kPar));
+        float* pd = reinterpret_cast<float*>(smem + (keys ? F::kOffPar + (t % kKParRing) * F::kPar : F::kOffVPar + slot * F::kVPar));
         const float s = __uint_as_float(par << 16);
         const int at = ((lt >> 1) & 3) * F::kParC + 2 * (lt >> 3) + (lt & 1);
+        float mid = 0.f;
         pd[at] = s;
-        if constexpr (F::kFmt == RB_KV_INT4)
-          pd[F::kParN + at] = fmaf(8.f, s, p.bf16 ? __uint_as_float(par & 0xffff0000u) : __half2float(__ushort_as_half(static_cast<unsigned short>(par >> 16))));
+        if constexpr (F::kFmt == RB_KV_INT4) {
+          mid = fmaf(8.f, s, p.bf16 ? __uint_as_float(par & 0xffff0000u) : __half2float(__ushort_as_half(static_cast<unsigned short>(par >> 16))));
+          pd[F::kParN + at] = mid;
+        }
+        if (!keys) pd[2 * F::kParN + at] = lt < n - static_cast<int64_t>(t0 + t) * kTile ? pfx::value_exponent(s, mid) : -INFINITY;
         arrive(slot);
         next_slot();
         fetch(t + kAhead, raw, par);

@@ -117,3 +117,27 @@ def reorder(t, parents, slots):
             n = int(slots[r * nb + b])
             out[r * nb + c, :, :n] = t[r * nb + b, :, :n]
     return out
+
+
+def attention_by_weight(q, rows, scale, u_p):
+    """attention() over one set of quantised rows (k, v) [nkv, S, hd] for every sequence, with an error bound that a slot
+    enters by its weight: 16-bit products p s round by u_p of themselves, and by 2^-25 where they are subnormal - 2^-31 of
+    the row's largest product, which is at least 2^6. A product stands for codes whose values, codes times s, are at most the
+    size (the largest value plus the range) of its slot's values: 2^-31 of the largest p * size.
+    fp32 scores, 2 hd 2^-24 of scale * sum |q k| for each slot; fp32 sums and the exponential, 2^-19."""
+    q = q.to(F64)
+    B, nq, hd = q.shape
+    k, v = rows
+    rep = nq // k.shape[0]
+    out, bound = torch.zeros(B, nq, hd, dtype=F64), torch.zeros(B, nq, hd, dtype=F64)
+    for h in range(nq):
+        kh, vh = k[h // rep], v[h // rep]
+        s = (q[:, h] @ kh.T) * scale
+        e_s = 2 * hd * 2.0 ** -24 * abs(scale) * (q[:, h].abs() @ kh.abs().T)
+        p = torch.exp(s - s.amax(-1, keepdim=True))
+        l = p.sum(-1, keepdim=True)
+        span = vh.abs().amax(-1) + (vh.amax(-1) - vh.amin(-1))
+        out[:, h] = (p @ vh) / l
+        bound[:, h] = (p @ vh.abs()) / l * (2 * u_p + 2.0 ** -19) + ((p * e_s) @ vh.abs() + (p * e_s).sum(-1, keepdim=True) * out[:, h].abs()) / l
+        bound[:, h] += len(kh) * 2.0 ** -31 * (p * span).amax(-1, keepdim=True) / l
+    return out, bound

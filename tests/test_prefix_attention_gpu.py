@@ -420,3 +420,78 @@ def test_no_scale_and_no_query(fmt, dtype, kernel, scale):
     PrefixAttention(s.attn._keep[0], s.out, prefix=s.pre, prefix_len=s.prefix_len, own=s.own, own_len=s.own_len, scale=scale,
                     kernel=kernel)()
     s.check()
+
+
+def slot_without_weight(B, nq, nkv, hd, S, fmt, dtype, spread, out_at, ratio, seed, size=1.0):
+    """q, k, v whose slot out_at has values 2^ratio times the others' and a score a hundred below every other one."""
+    dt = DTYPES[dtype]
+    g = torch.Generator().manual_seed(seed)
+    base = torch.randn(nkv, hd, generator=g)
+    q = base.repeat_interleave(nq // nkv, 0) + 0.1 * torch.randn(B, nq, hd, generator=g)
+    k = spread * torch.randn(1, S, nkv, hd, generator=g)
+    v = torch.randn(1, S, nkv, hd, generator=g) * size
+    k[0, out_at] = -100 * hd ** 0.5 * base / base.square().sum(-1, keepdim=True)
+    v[0, out_at] *= 2.0 ** ratio
+    return q.to(dt), k.to(dt), v.to(dt)
+
+
+def check_by_weight(out, q, k, v, fmt, dtype):
+    want, bound = ref.attention_by_weight(q, tuple(ref.values(x[0], fmt).transpose(0, 1) for x in (k, v)), q.shape[2] ** -0.5, 2.0 ** -11)
+    half = 2.0 ** -8 if dtype == "bf16" else 2.0 ** -11
+    got = out.cpu()
+    off = (got.double() - want).abs()
+    over = off - (want.abs() * half * (1 + 2 ** -7) + bound * (1 + half) + 2.0 ** -25 * (dtype == "fp16"))
+    assert torch.isfinite(got).all() and (over <= 0).all(), f"largest error {off.max():.3g}, over its bound by {over.max():.3g}"
+
+
+@pytest.mark.parametrize("kernel", ["mma", "tc"])
+@pytest.mark.parametrize("fmt", ["int8", "int4"])
+@pytest.mark.parametrize("dtype,ratio,size", [("fp16", 9, 1.0), ("fp16", 20, 2.0 ** -9), ("bf16", 16, 1.0), ("bf16", 24, 1.0), ("bf16", 100, 1.0)])
+@pytest.mark.parametrize("S,out_at", [(200, 0), (200, 150), (4000, 37), (4000, 3900)])
+def test_a_large_row_without_weight(S, out_at, dtype, ratio, size, fmt, kernel):
+    """One visible slot whose values, and so whose scale, are far larger than the others' but whose probability is next to
+    nothing: the others keep their accuracy, which is bounded by their own weights and values. (8 heads of 16 sequences:
+    few splits, so that most slots share a partial with that one.)"""
+    q, k, v = slot_without_weight(16, 64, 8, 64, S, fmt, dtype, 1.0, out_at, ratio, seed=S + out_at, size=size)
+    cache = KVCache(1, 8, S, 64, fmt, DTYPES[dtype])
+    cache.write(k.to(DEV), v.to(DEV), torch.zeros(1, dtype=torch.int64, device=DEV))
+    out = torch.empty(q.shape, dtype=q.dtype, device=DEV)
+    PrefixAttention(q.to(DEV), out, prefix=cache, prefix_len=torch.tensor([S], device=DEV), kernel=kernel)()
+    check_by_weight(out, q, k, v, fmt, dtype)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "int4"])
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+def test_a_flat_tail_beside_a_large_row_without_weight(fmt, dtype):
+    """Own rows, one split each: a slot without values holds most of the weight, thousands hold 2^-18 to 2^-20 of it each,
+    and the values of one without weight are 2^9 times larger. The tail's sum is the output."""
+    B, nkv, S, hd = 40, 8, 4000, 128
+    q, k, v = slot_without_weight(B, nkv, nkv, hd, S, fmt, dtype, 0.05, 77, 9, seed=3, size=0.25)
+    top = q.float().mean(0)
+    k[0, 1234] = (13.2 * hd ** 0.5 * top / top.square().sum(-1, keepdim=True)).to(k.dtype)
+    v[0, 1234] = 0
+    own = KVCache(B, nkv, S, hd, fmt, DTYPES[dtype])
+    own.write(k.to(DEV).expand(B, -1, -1, -1), v.to(DEV).expand(B, -1, -1, -1), torch.zeros(B, dtype=torch.int64, device=DEV))
+    out = torch.empty(q.shape, dtype=q.dtype, device=DEV)
+    PrefixAttention(q.to(DEV), out, own=own, own_len=torch.full((B,), S, device=DEV))()
+    check_by_weight(out, q, k, v, fmt, dtype)
+
+
+@pytest.mark.parametrize("kernel", ["mma", "tc"])
+@pytest.mark.parametrize("fmt", ["int8", "int4"])
+@pytest.mark.parametrize("lo,hi", [(0, 0), (-100, -60), (-100, 100), (40, 112), (112, 112)])
+def test_values_over_the_whole_range_of_bf16(lo, hi, fmt, kernel):
+    """Values from 2^lo to 2^hi, and rows of zeros among them, in ascending, descending and mixed order."""
+    S = 700
+    g = torch.Generator().manual_seed(5)
+    q, k, v = torch.randn(3, 8, 128, generator=g), torch.randn(1, S, 2, 128, generator=g) * 0.3, torch.randn(1, S, 2, 128, generator=g)
+    size = torch.linspace(lo, hi, S, dtype=torch.float64)
+    for order in (torch.arange(S), torch.arange(S).flip(0), torch.randperm(S, generator=g)):
+        w = (v.clamp(-3, 3).double() * 2.0 ** size[order][None, :, None, None])
+        w[:, ::5] = 0
+        qq, kk, vv = q.bfloat16(), k.bfloat16(), w.float().bfloat16()
+        cache = KVCache(1, 2, S, 128, fmt, torch.bfloat16)
+        cache.write(kk.to(DEV), vv.to(DEV), torch.zeros(1, dtype=torch.int64, device=DEV))
+        out = torch.empty(3, 8, 128, dtype=torch.bfloat16, device=DEV)
+        PrefixAttention(qq.to(DEV), out, prefix=cache, prefix_len=torch.tensor([S], device=DEV), kernel=kernel)()
+        check_by_weight(out, qq, kk, vv, fmt, "bf16")

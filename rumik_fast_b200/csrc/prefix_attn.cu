@@ -704,14 +704,15 @@ struct Plan {
 
 template <int kTile>
 __device__ __forceinline__ Plan make_plan(const Params& p, int grid) {
-  // every warp by itself: no barrier, and the loads of all lengths go out together
+  // every warp by itself: no barrier, and the loads of all lengths go out together. The launch before may have written the
+  // lengths while this one was resident: loads that stay behind the wait (__ldg's may not), as everywhere below
   const int lane = threadIdx.x & 31;
-  const int64_t np_raw = p.pre.k ? __ldg(p.pre.len) : 0;
+  const int64_t np_raw = p.pre.k ? __ldcg(p.pre.len) : 0;
   int sum = 0, most = 0;
   if (p.own.k) {
 #pragma unroll 2
     for (int b = lane; b < p.n_seqs; b += 32) {
-      const int64_t n = __ldg(p.own.len + b);
+      const int64_t n = __ldcg(p.own.len + b);
       if (n <= 0 || n > p.own.cache_len) continue;
       const int t = static_cast<int>((n + kTile - 1) / kTile);
       sum += min(t + 2, 1 << 20);  // an item's start and end cost about two stages
@@ -773,7 +774,7 @@ __global__ void __launch_bounds__(kThreads, F::kCtas) prefix_attn_kernel(const _
       it.kv = lane_i / p.tiles_m;
       const int rt = lane_i % p.tiles_m;
       head = it.kv;
-      it.n = *S.len;
+      it.n = __ldcg(S.len);
       it.t0 = sp * pl.pt;
       it.t1 = it.t0 + pl.pt;
       it.seq = -1;
@@ -788,7 +789,7 @@ __global__ void __launch_bounds__(kThreads, F::kCtas) prefix_attn_kernel(const _
       const int x = i - pl.prefix_items, sp = x % pl.ns;
       it.kv = (x / pl.ns) % p.n_kv;
       it.seq = x / pl.ns / p.n_kv;
-      it.n = S.len[it.seq];
+      it.n = __ldcg(S.len + it.seq);
       if (it.n < 0 || it.n > S.cache_len) {
         if (threadIdx.x == 0) atomicOr(&g_device_error, static_cast<unsigned>(ERR_ARG));
         continue;
@@ -815,7 +816,7 @@ __global__ void __launch_bounds__(kThreads, F::kCtas) prefix_attn_kernel(const _
   // an own length outside its cache with no item of its own (no split at all) is reported here
   if (cta == 0 && pl.ns == 0 && p.own.k)
     for (int b = threadIdx.x; b < p.n_seqs; b += kThreads)
-      if (p.own.len[b] < 0 || p.own.len[b] > p.own.cache_len) atomicOr(&g_device_error, static_cast<unsigned>(ERR_ARG));
+      if (const int64_t n = __ldcg(p.own.len + b); n < 0 || n > p.own.cache_len) atomicOr(&g_device_error, static_cast<unsigned>(ERR_ARG));
 }
 
 // A CTA joins the partials of one (sequence, query head): prefix splits, then own splits. Warp w takes every fourth

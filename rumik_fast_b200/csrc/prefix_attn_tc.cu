@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attn_tc_kernel(const __gri
 
   griddep_wait();
   griddep_launch_dependents();
-  const int64_t n = *p.pre.len;
+  const int64_t n = __ldcg(p.pre.len);
   const int lane_i = blockIdx.x / p.max_np, sp = blockIdx.x % p.max_np;
   const int kv = lane_i / p.tiles_m, row0 = (lane_i % p.tiles_m) * kTile;
   if (n < 0 || n > p.pre.cache_len) {

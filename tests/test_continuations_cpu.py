@@ -1,6 +1,8 @@
 """The C ABI of the caches, the prefix attention and the beams without a GPU: bad arguments come back with their status
 before any CUDA call, empty calls succeed."""
 import ctypes
+import os
+import re
 
 from rumik_fast_b200 import _lib
 
@@ -118,3 +120,15 @@ def test_beam_reorder_validation(native_lib):
         assert reorder(**kw) == _lib.ERR_SHAPE, kw
     assert reorder(p=None) == _lib.ERR_NULL and reorder(parents=None) == _lib.ERR_NULL and reorder(slots=None) == _lib.ERR_NULL
     assert reorder(p=A + 1) == _lib.ERR_ALIGN
+
+
+def test_no_read_only_loads_of_what_the_launch_before_may_write():
+    """Lengths, positions, parents and scores are written by launches that may still run when these kernels become resident
+    (programmatic dependent launch). __ldg is a load of memory that is read-only for a kernel's whole life: it need not stay
+    behind the kernel's wait, so none of these kernels uses it."""
+    csrc = os.path.join(os.path.dirname(os.path.abspath(_lib.__file__)), "csrc")
+    for name in ("kv_cache.cu", "prefix_attn.cu", "prefix_attn_tc.cu", "beams.cu"):
+        with open(os.path.join(csrc, name)) as f:
+            code = re.sub(r"//[^\n]*", "", f.read())
+        assert "griddep_wait()" in code, name
+        assert not re.search(r"__ldg\s*\(|ld\.global\.nc|__restrict__", code), name

@@ -329,11 +329,13 @@ __global__ void __launch_bounds__(kThreads, kSelectCtas) beam_select_kernel(cons
         });
   } else {
     // a finished beam: its end row with the score it has; then, and for a beam without any candidate, rows of -inf
+    // in their order (all of them where the score is not finite)
     const int end = static_cast<int>(p.end_idx);
+    const bool counts = done && !dead;
     for (int r = tid; r < nb; r += kThreads) {
-      const int rest = done ? (r - 1 >= end ? r : r - 1) : r;
-      const int at = done && r == 0 ? end : rest;
-      cand[r] = done && r == 0 && !dead ? score : -INFINITY;
+      const int rest = counts ? (r - 1 >= end ? r : r - 1) : r;
+      const int at = counts && r == 0 ? end : rest;
+      cand[r] = counts && r == 0 ? score : -INFINITY;
       idx[r] = at < p.V ? at : -1;
     }
   }

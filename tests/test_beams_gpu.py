@@ -235,3 +235,15 @@ def test_refusals():
                 ([f(4, 2, 8, 1, dt=torch.uint8)], parents, slots), ([t], parents.int(), slots), ([t], parents, slots[:3]), ([t], parents[0], slots)):
         with pytest.raises(RuntimeError):
             BeamReorder(*bad)
+
+
+@pytest.mark.parametrize("nb,end", [(2, 1), (4, 5), (6, 3), (8, 0)])
+def test_finished_beams_without_a_score(nb, end):
+    """A finished beam whose score is not finite has no candidate: its rows fill up in their order like a live one's, its
+    end row among them and not before them."""
+    for seed, bad in enumerate((-float("inf"), float("nan"), float("inf"))):
+        logits, scores, done = inputs(2, nb, 40, torch.float16, 60 + seed)
+        done[:], scores[:] = True, bad                    # nobody has one
+        check(logits, scores, done, end, BeamSelect(logits.to(DEV), scores.to(DEV), done.to(DEV), end_idx=end)())
+        scores[1, nb - 1] = -1.5                          # the last one of a request is finished with a score
+        check(logits, scores, done, end, BeamSelect(logits.to(DEV), scores.to(DEV), done.to(DEV), end_idx=end)())

@@ -2,7 +2,7 @@
 // (rb_beam_select) and the reordering of the beams' cache rows by their parents, in place (rb_beam_reorder).
 //
 // Selection, per request of nb beams:
-//   cand[b, v] = (x[b, v] - lse_b) + score_b,  lse_b = log sum_v exp(x[b, v])        (a live beam)
+//   cand[b, v] = (x[b, v] - m_b) - log sum_v exp(x[b, v] - m_b) + score_b,  m_b = max_v x[b, v]        (a live beam)
 //   cand[b, end] = score_b and nothing else                                           (a finished beam)
 // and the nb best of the nb V candidates. Within a beam the order of the candidates is the order of the logits, so no
 // normaliser is needed to find a beam's nb best rows: one pass over the logits yields each chunk's maximum, sum of
@@ -319,12 +319,14 @@ __global__ void __launch_bounds__(kThreads, kSelectCtas) beam_select_kernel(cons
     if (odd && tid == 0) atomicOr(&g_device_error, static_cast<unsigned>(ERR_ARG));
   }
   if (!done && !dead && !odd && ms.x > -INFINITY) {
-    const float lse = ms.x + logf(ms.y);  // ms.y >= 1 up to rounding: the largest logit's own term
+    // ms.y >= 1 up to rounding: the largest logit's own term. The largest logit is taken off first: rounded to a sum with
+    // it, the logarithm would lose what logits far from zero leave no bits for.
+    const float log_sum = logf(ms.y);
     const Key* src = p.keys + static_cast<int64_t>(row) * p.chunks * nb;
     cta_top(
         sh, nb, p.chunks * nb, [&](int i) { return __ldcg(src + i); },
         [&](int r, Key key) {
-          cand[r] = key ? (key_value(key) - lse) + score : -INFINITY;
+          cand[r] = key ? ((key_value(key) - ms.x) - log_sum) + score : -INFINITY;
           idx[r] = key ? static_cast<int>(key_row(key)) : -1;
         });
   } else {

@@ -247,3 +247,17 @@ def test_finished_beams_without_a_score(nb, end):
         check(logits, scores, done, end, BeamSelect(logits.to(DEV), scores.to(DEV), done.to(DEV), end_idx=end)())
         scores[1, nb - 1] = -1.5                          # the last one of a request is finished with a score
         check(logits, scores, done, end, BeamSelect(logits.to(DEV), scores.to(DEV), done.to(DEV), end_idx=end)())
+
+
+@pytest.mark.parametrize("shift", [20000.0, -20000.0, 3.0e6])
+def test_scores_of_logits_far_from_zero(shift):
+    """Logits that lie around 20,000 or 3,000,000 are exact inputs: their differences, and so the scores, are as exact as
+    those of logits around zero (the module's bound, which does not depend on the logits' size)."""
+    g = torch.Generator().manual_seed(26)
+    logits = torch.randn(2, 4, 6000, generator=g) * 4.0 + shift
+    done = torch.zeros(2, 4, dtype=torch.bool)
+    for _ in range(200):
+        scores = -2 - 5 * torch.rand(2, 4, generator=g)
+        if ref.select(logits, scores, done, 0)[4] > 2e-4:
+            break
+    check(logits, scores, done, 0, BeamSelect(logits.to(DEV), scores.to(DEV), done.to(DEV), end_idx=0)())

@@ -29,9 +29,12 @@ constexpr int kChunk = kThreads * kPer;        // 4096 rows a batch
 constexpr int kSelectCtas = 4;                 // of an SM, by registers and shared memory
 constexpr int kFew = 64;                        // threads whose keys a list takes before it is cut back to the nb best (144: 32 us, not 30)
 constexpr int kMaxBeams = 32;
-constexpr int kMaxChunks = 256;                // V <= 2^20
 constexpr int kCap = kThreads / 32 * kMaxBeams * kPer;                // keys that may pass a bound: 4096
-static_assert(kCap >= kChunk && kCap >= kFew * kPer && kCap >= kMaxBeams * (kMaxChunks * kMaxBeams / kThreads), "those of a beam's merged lists as well");
+// Keys of the lists that a beam's or a request's last CTA merges: nb of each of a beam's chunks, of which a launch has no more
+// than kMaxCtas over all rows unless each row has just one (select_per); or nb of each beam.
+constexpr int kMaxCtas = 4096;
+static_assert(kCap >= kChunk && kCap >= kFew * kPer && kMaxCtas <= kThreads * kPer && kMaxBeams * kMaxBeams <= kThreads * kPer,
+              "at most kPer keys a thread, as in a batch");
 
 struct SelectParams {
   const void* logits;
@@ -73,29 +76,25 @@ struct Shared {
   int last;
 };
 
-// A bound that at least k of the CTA's keys reach. `best` is this thread's largest key (0: none). kWide: the k-th
-// largest of all threads' own (at most k threads hold a key that reaches it); else, from the ranks within the warps (an
-// eighth of the comparisons), the larger of two such bounds: the largest over the warps of a warp's k-th (at most k
-// lanes of each warp reach it), and the smallest over the warps of a warp's ceil(k / 8)-th (8 ceil(k / 8) keys do), which
-// is the closer one on ordinary logits - about 2 k keys pass it.
-template <bool kWide>
+// A bound that at least k of the CTA's keys reach. `best` is this thread's largest key (0: none). From the ranks within the
+// warps, the larger of two such bounds: the largest over the warps of a warp's k-th (at most k lanes of each warp reach
+// it), and the smallest over the warps of a warp's ceil(k / 8)-th (8 ceil(k / 8) keys do), which is the closer one on
+// ordinary logits - about 2 k keys pass it.
 __device__ __forceinline__ Key cta_bound(Shared& sh, int k, Key best) {
-  constexpr int kN = kWide ? kThreads : 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   sh.top[threadIdx.x] = best;
   if (lane == 0) sh.bound[warp] = 1, sh.each[warp] = 0;
-  if (kWide) __syncthreads();
-  else __syncwarp();
+  __syncwarp();
   int rank = 0;
-  const ulonglong2* all = reinterpret_cast<const ulonglong2*>(sh.top + (kWide ? 0 : warp * 32));
+  const ulonglong2* all = reinterpret_cast<const ulonglong2*>(sh.top + warp * 32);
 #pragma unroll 8
-  for (int j = 0; j < kN / 2; ++j) {
+  for (int j = 0; j < 16; ++j) {
     const ulonglong2 v = all[j];
     rank += v.x > best;
     rank += v.y > best;
   }
   if (rank == k - 1 && best != 0) sh.bound[warp] = best;  // keys differ: one thread has this rank
-  if (!kWide && rank == (k + kThreads / 32 - 1) / (kThreads / 32) - 1) sh.each[warp] = best;
+  if (rank == (k + kThreads / 32 - 1) / (kThreads / 32) - 1) sh.each[warp] = best;
   __syncthreads();
   Key lim = 1, least = ~Key(0);
 #pragma unroll
@@ -103,7 +102,7 @@ __device__ __forceinline__ Key cta_bound(Shared& sh, int k, Key best) {
     lim = sh.bound[w] > lim ? sh.bound[w] : lim;
     least = sh.each[w] < least ? sh.each[w] : least;
   }
-  return !kWide && least > lim ? least : lim;
+  return least > lim ? least : lim;
 }
 
 // The k largest of the keys in sh.cand, best first, through out(rank, key); ranks without a key get 0.
@@ -123,7 +122,7 @@ __device__ __forceinline__ void cta_rank(Shared& sh, int k, Out out) {
   __syncthreads();
 }
 
-// The k largest of n keys get(0) .. get(n - 1) (0: none).
+// The k largest of n <= kPer kThreads keys get(0) .. get(n - 1) (0: none).
 template <typename Get, typename Out>
 __device__ __forceinline__ void cta_top(Shared& sh, int k, int n, Get get, Out out) {
   if (n <= kThreads) {  // a key a thread: all of them are ranked
@@ -139,7 +138,7 @@ __device__ __forceinline__ void cta_top(Shared& sh, int k, int n, Get get, Out o
       const Key v = get(i);
       best = v > best ? v : best;
     }
-    const Key lim = n <= kPer * kThreads ? cta_bound<false>(sh, k, best) : cta_bound<true>(sh, k, best);
+    const Key lim = cta_bound(sh, k, best);
     if (best >= lim) {
 #pragma unroll 1
       for (int i = threadIdx.x; i < n; i += kThreads) {
@@ -257,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, kSelectCtas) beam_select_kernel(cons
       // rows past the vocabulary hold -inf like masked ones, but no key
       auto reaches = [&] { return first < end && !(top < least); };
       if (from == begin) {
-        lim = cta_bound<false>(sh, nb, best());
+        lim = cta_bound(sh, nb, best());
         least = key_value(lim);
       }
       int many = __syncthreads_count(reaches());
@@ -271,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, kSelectCtas) beam_select_kernel(cons
         held = nb;
         many = __syncthreads_count(reaches());
         if (many > kFew) {  // rising logits, for one: this batch's own bound is closer
-          lim = max(lim, cta_bound<false>(sh, nb, best()));
+          lim = max(lim, cta_bound(sh, nb, best()));
           least = key_value(lim);
           many = __syncthreads_count(reaches());
         }
@@ -448,13 +447,22 @@ __global__ void __launch_bounds__(kReorderThreads) beam_reorder_kernel(const __g
 
 namespace {
 int64_t align16(int64_t n) { return (n + 15) / 16 * 16; }
-int64_t select_chunks(int64_t V) { return (V + bm::kChunk - 1) / bm::kChunk; }
+// Batches of kChunk logits that a CTA takes: one while the CTAs of all rows are no more than `ctas`, else the fewest that
+// make them so (all of a row's, if need be).
+int64_t select_per(int64_t rows, int64_t V, int64_t ctas) {
+  const int64_t batches = (V + bm::kChunk - 1) / bm::kChunk;
+  int64_t per = 1;
+  while (per < batches && rows * ((batches + per - 1) / per) > std::min<int64_t>(ctas, bm::kMaxCtas)) ++per;
+  return per;
+}
+int64_t select_chunks(int64_t V, int64_t per) { return (V + per * bm::kChunk - 1) / (per * bm::kChunk); }
 }  // namespace
 
 int64_t beam_select_tickets(int64_t requests, int nb) { return align16((requests * nb + requests) * 4); }
 
 int64_t beam_select_workspace(int64_t requests, int nb, int64_t V) {
-  const int64_t rows = requests * nb, ch = select_chunks(V);
+  // for the most CTAs that a launch has, however many the device holds: more of them have no fewer chunks a row
+  const int64_t rows = requests * nb, ch = select_chunks(V, select_per(rows, V, bm::kMaxCtas));
   return beam_select_tickets(requests, nb) + align16(rows * ch * 8) + align16(rows * ch * nb * 8) + 2 * align16(rows * nb * 4);
 }
 
@@ -476,12 +484,8 @@ int launch_beam_select(const rb_beam_select_args* a, int num_sms, int flags, cud
   p.min_new = a->min_new;
   p.nb = a->n_beams;
   p.V = static_cast<int>(a->n_vocab);
-  // one batch a CTA while the CTAs fit on the SMs at once, else the fewest that make them fit
-  const int64_t batches = select_chunks(a->n_vocab);
-  int64_t per = 1;
-  while (per < batches && rows * ((batches + per - 1) / per) > kSelectCtas * static_cast<int64_t>(num_sms)) ++per;
-  p.per = static_cast<int>(per);
-  p.chunks = static_cast<int>((batches + per - 1) / per);
+  p.per = static_cast<int>(select_per(rows, a->n_vocab, kSelectCtas * static_cast<int64_t>(num_sms)));  // the CTAs fit on the SMs at once
+  p.chunks = static_cast<int>(select_chunks(a->n_vocab, p.per));
   uint8_t* w = static_cast<uint8_t*>(a->ws);
   p.tickets = reinterpret_cast<unsigned int*>(w);
   w += beam_select_tickets(a->requests, a->n_beams);

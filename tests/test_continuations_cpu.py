@@ -132,3 +132,16 @@ def test_no_read_only_loads_of_what_the_launch_before_may_write():
             code = re.sub(r"//[^\n]*", "", f.read())
         assert "griddep_wait()" in code, name
         assert not re.search(r"__ldg\s*\(|ld\.global\.nc|__restrict__", code), name
+
+
+def test_beam_select_workspace_follows_the_launch(native_lib):
+    """A launch has at most some thousand CTAs, or one a row: the workspace is for that many lists, not for one every 4,096
+    logits of every row; and it grows with the vocabulary and the rows as far as the launch does."""
+    need = native_lib.rb_beam_select_workspace
+    assert need(2047, 32, 1 << 20) < 1 << 26                     # 65,504 rows of one list each
+    assert need(8, 16, 130001) >= 128 * 32 * 16 * 8              # 32 chunks a row fit the CTAs
+    for requests, beams in ((1, 1), (1, 32), (3, 5), (100, 16), (2047, 32)):
+        sizes = [need(requests, beams, v) for v in (1, 4096, 4097, 70001, 1 << 20)]
+        rows = requests * beams
+        assert all(s >= rows * (beams * 16 + 8) for s in sizes), "one list, one row of candidates and a sum for each row"
+        assert max(sizes) <= max(rows, 4096) * (beams + 1) * 8 + rows * beams * 8 + (rows + requests) * 4 + 5 * 16

@@ -681,19 +681,25 @@ namespace pfx {
 // Warps along the rows: the fewest whose 16-row tiles hold the batch's rows, at most four.
 inline int warps_m(int64_t rows) { return rows <= 16 ? 1 : (rows <= 32 ? 2 : 4); }
 
-// Which kernel streams the prefix, when the flags do not say: by its capacity, the lengths being on the device. The
-// tcgen05 kernel's start costs about what one to two thousand slots cost the warp-level one (8 heads of 128, 16 bits, 20
-// own slots, 24 rows: 1,000 slots 11 us against 13, 3,000 12 against 18, 40,000 42 against 44; 256 rows: 27 against 32, 32
-// against 40, 103 against 179). Only for up to 16 rows of 8-bit codes of 128 columns is the warp-level kernel, which
-// converts in registers what the products read, the faster one on the whole (8 heads, 8 rows: 3,000 slots 12.4 us against
-// 12.0, 10,000 17.7 against 16.8, 40,000 35.9 against 33.2; 2 heads 11.3 against 9.9, 14.7 against 14.7, 20.7 against 22.1;
-// 8 heads, 24 rows: 13.2 against 14.7, 21.6 against 21.0, 39.5 against 46.7).
+// Which kernel streams the prefix, when the flags do not say: by its capacity, the lengths being on the device. us of the
+// warp-level kernel / the tcgen05 kernel, 20 own slots a sequence:
+//   The tcgen05 kernel's start costs about what one to two thousand slots cost the other one (128 columns, 16 bits, 8 heads:
+//   24 rows 1,100 slots 12.8 / 10.9, 10,000 21.6 / 18.4; 128 rows 18.2 / 17.7, 36.8 / 29.9; 64 columns, int8, 2 heads: 16 rows
+//   1,100 slots 9.2 / 9.5, 10,000 23.0 / 12.6; 128 rows 2,100 slots 13.1 / 12.7, 10,000 17.9 / 15.7).
+//   With one tile of 16 rows over rows of up to 128 bytes the warp-level kernel, which converts in registers what the
+//   products read, keeps up as long as it has slots for all SMs: from some 98,304 of all heads together (64 columns, 4 rows of
+//   8 heads, 40,000 slots: plain 19.9 / 26.7, int8 21.3 / 27.3, int4 25.4 / 35.7; 8 rows of 2 heads, 10,000: plain 21.1 / 11.7,
+//   int8 19.2 / 12.6), and with 8-bit codes of 128 columns on the whole (8 rows: 2 heads 2,100 slots 9.7 / 11.0, 10,000 15.2 /
+//   14.0; 8 heads 11.4 / 11.8, 14.7 / 20.4). Over 2,700 sizes of 1 to 16 heads, 1 to 128 rows and 600 to 40,000 slots this
+//   choice takes 2.3 % longer than the better kernel each time would, 1.5 times as long at worst.
 inline bool use_tc(const rb_prefix_attn_args* a, int rep, int flags) {
   if (!a->prefix || (flags & RB_FLAG_KERNEL_MMA)) return false;
   if (flags & RB_FLAG_KERNEL_TC) return true;
+  const rb_kv_cache* c = a->prefix;
   const int64_t rows = a->n_seqs * rep;
-  if (a->prefix->fmt == RB_KV_INT8 && a->prefix->head_dim == 128 && rows <= 16) return false;
-  return a->prefix->cache_len >= (rows > 32 ? 1024 : 2048);
+  const bool int8 = c->fmt == RB_KV_INT8, wide = c->head_dim == 128;
+  if (rows <= 16 && !(c->fmt == RB_KV_PLAIN && wide) && ((int8 && wide) || c->n_kv_heads * c->cache_len >= 98304)) return false;
+  return c->cache_len >= (rows > 32 ? 1024 : 2048);
 }
 
 struct Layout {

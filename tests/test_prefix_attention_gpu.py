@@ -495,3 +495,24 @@ def test_values_over_the_whole_range_of_bf16(lo, hi, fmt, kernel):
         out = torch.empty(3, 8, 128, dtype=torch.bfloat16, device=DEV)
         PrefixAttention(qq.to(DEV), out, prefix=cache, prefix_len=torch.tensor([S], device=DEV), kernel=kernel)()
         check_by_weight(out, qq, kk, vv, fmt, "bf16")
+
+
+@pytest.mark.parametrize("fmt,hd,heads,rep,S,kernel", [
+    ("int8", 64, 16, 1, 20000, "mma"), ("int4", 128, 16, 2, 20000, "mma"), ("plain", 64, 16, 1, 20000, "mma"),   # few rows, all SMs busy
+    ("int8", 128, 2, 1, 3000, "mma"),
+    ("int8", 64, 2, 1, 10000, "tc"), ("int4", 128, 2, 1, 20000, "tc"), ("plain", 128, 16, 1, 20000, "tc"), ("int8", 64, 16, 8, 20000, "tc"),
+    ("plain", 128, 2, 1, 1500, "mma"), ("int8", 128, 2, 16, 1500, "tc"),
+])
+def test_choice_of_the_kernel(fmt, hd, heads, rep, S, kernel):
+    """Without a word about the kernel the one that was measured faster runs: its bits, where the two kernels' differ."""
+    B = 4
+    g = torch.Generator(device=DEV).manual_seed(7)
+    cache = KVCache(1, heads, S, hd, fmt)
+    x = torch.randn(2, 1, S, heads, hd, generator=g, device=DEV).half()
+    cache.write(x[0], x[1], torch.zeros(1, dtype=torch.int64, device=DEV))
+    q = torch.randn(B, heads * rep, hd, generator=g, device=DEV).half()
+    got = {}
+    for k in (None, "mma", "tc"):
+        got[k] = torch.empty_like(q)
+        PrefixAttention(q, got[k], prefix=cache, prefix_len=torch.tensor([S], device=DEV), kernel=k)()
+    assert not torch.equal(got["mma"], got["tc"]) and torch.equal(got[None], got[kernel])

@@ -531,8 +531,13 @@ int rb_kv_read(const rb_kv_cache* cache, void* k_out, void* v_out, int64_t start
  * slots j < own_len[b] of sequence b in `own` (n_seqs as the call's). The prefix is read once for the whole batch, not
  * once a sequence. A sequence without any slot gets zeros. Either cache may be NULL; both have one format, dtype, head
  * count and head_dim. 1 <= n_q_heads / n_kv_heads <= 16. Lengths are int64 on the device; a *prefix_len or own_len[b]
- * outside its cache stores nothing for the sequences it concerns and sets RB_DEVERR_ARG. Scores, softmax and sums are
- * fp32; a quantised row enters the products as its codes. Rows at or beyond a length may hold anything. A wait that runs out sets bit 12 (0x1000) of the device error word.
+ * outside its cache stores nothing for the sequences it concerns and sets RB_DEVERR_ARG (in a cache of no slots every
+ * length above zero does). Scores, exponentials and sums are fp32; a quantised row enters the products as its codes. In
+ * 16 bits are the probabilities as a factor of the second product: of PLAIN bf16 rows in bf16 (relative rounding 2^-8), of
+ * fp16 rows in fp16 (2^-11), of codes times the values' scale in fp16 (INT4: as the sum of two); the sum that divides is of
+ * the unrounded ones. bf16 queries enter products with codes as fp16 under a power of two of their row: elements 2^-14
+ * below the row's largest lose bits. Rows at or beyond a length may hold anything. A wait that runs out sets bit 12
+ * (0x1000) of the device error word.
  * ws: rb_prefix_attn_workspace(...) bytes, 16-byte aligned, whatever they hold. Calls that share a workspace must not
  * overlap in time.
  */

@@ -25,7 +25,7 @@
 //
 // Bound: the latency of a split's stages and of the launches (attention and merge) where the caches are small - 4 sequences
 // on 301 slots 10 us - and beyond some 16 rows the conversion of the codes to 16 bits, once a warp: 8 heads, 40,000 slots
-// of int8 33 us with 8 rows (2.5 TB/s), 67 with 48. From there on prefix_attn_tc.cu, which converts a tile once for 128
+// of int8 30 us with 8 rows (2.7 TB/s), 65 with 48. From there on prefix_attn_tc.cu, which converts a tile once for 128
 // rows, takes the prefix.
 #include "common.cuh"
 #include "tc.cuh"

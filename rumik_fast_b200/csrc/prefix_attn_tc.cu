@@ -20,7 +20,8 @@
 // Bound: 16-bit rows by HBM in the loop over the tiles (64 KB in 2,950 cycles on every SM: 6.1 TB/s), beside 10 us of start
 // and merge (32,768 slots of 8 heads with 48 rows: 46 us). 8-bit codes of up to 64 rows by the loaders, 2,100 cycles a tile of keys or values: conversion, the
 // proxy fence and the loads' latency in turn. More rows by a group's chain of QK, softmax and PV, 6,000 cycles for each of
-// two tiles under way, in any format (100,001 slots of 4 heads with 256 rows, int8: 115 us, 99 of them here, 530 TFLOP/s).
+// two tiles under way, with codes somewhat more (100,001 slots of 4 heads with 256 rows, int8: 121 us, 105 without the own
+// rows, 500 TFLOP/s; 6 of them for the largest t + e of the rows slot by slot, which the largest t and e apart would save).
 #include "common.cuh"
 #include "tc.cuh"
 #include "kernels.h"

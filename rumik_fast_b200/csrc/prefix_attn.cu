@@ -43,7 +43,8 @@ constexpr int kThreads = kWarps * 32;
 constexpr bool wide_steps(int fmt, int hd) { return fmt != RB_KV_PLAIN && hd == 128; }
 constexpr int ctas_per_sm(int fmt, int hd) { return wide_steps(fmt, hd) ? 2 : 3; }
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLeastFactor = 1.17549435e-38f;  // of a row's scores: the smallest normal number, so that a masked slot's -inf stays -inf
+// A row's factor from scores to log2 units, within the normal numbers: a masked slot's -inf stays -inf, a score of zero zero.
+__device__ __forceinline__ float factor_in_range(float f) { return fminf(fmaxf(f, 1.17549435e-38f), 3.402823466e38f); }
 // t + e of a row's slots stays below R + kRoom + kSlack, so that 2^(t - R) s < 2^15 and fits fp16; the largest is at least
 // 2^kRoom, which keeps factors down to 2^-20 of it normal numbers.
 constexpr float kRoom = 6.f, kSlack = 8.f;
@@ -476,7 +477,7 @@ __device__ __forceinline__ void run_item(const Params& p, const Item it, const i
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
     }
-    fr[x] = fmaxf(f, kLeastFactor);
+    fr[x] = factor_in_range(f);
     qs[x] = sum;
   }
   store_par();

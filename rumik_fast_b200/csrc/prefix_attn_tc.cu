@@ -661,7 +661,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attn_tc_kernel(const __gri
         }
         sts128(s0 + piece_at(lane_row, i), w[0], w[1], w[2], w[3]);
       }
-      rowf[lane_row] = fmaxf(f, pfx::kLeastFactor);
+      rowf[lane_row] = pfx::factor_in_range(f);
       qsum[lane_row] = flip ? -sum : sum;
       fence_proxy_async_smem();
     }

@@ -516,3 +516,18 @@ def test_choice_of_the_kernel(fmt, hd, heads, rep, S, kernel):
         got[k] = torch.empty_like(q)
         PrefixAttention(q, got[k], prefix=cache, prefix_len=torch.tensor([S], device=DEV), kernel=k)()
     assert not torch.equal(got["mma"], got["tc"]) and torch.equal(got[None], got[kernel])
+
+
+@pytest.mark.parametrize("kernel", ["mma", "tc"])
+@pytest.mark.parametrize("fmt", ["plain", "int8", "int4"])
+@pytest.mark.parametrize("scale", [3.3e38, -3.3e38])
+def test_largest_scale_and_no_query(fmt, kernel, scale):
+    """Scales whose product with log2 e is no fp32 number any more, over queries of zeros: scores of zero."""
+    for dtype in sorted(DTYPES):
+        s = Setup(5, 8, 2, 64, 300, [3, 0, 1, 70, 2], fmt, dtype, seed=32)
+        s.q.zero_()
+        s.attn._keep[0].zero_()
+        s.scale = scale
+        PrefixAttention(s.attn._keep[0], s.out, prefix=s.pre, prefix_len=s.prefix_len, own=s.own, own_len=s.own_len, scale=scale,
+                        kernel=kernel)()
+        s.check()

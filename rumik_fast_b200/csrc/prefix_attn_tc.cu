@@ -64,7 +64,7 @@ struct Fmt {
   static constexpr int kOffVPar = kOffPar + kKParRing * kPar;
   static constexpr int kOffRow = kOffVPar + kVRing * kVPar;  // factor and sum of the rows' queries
   static constexpr int kOffBar = kOffRow + kTile * 8;
-  static constexpr int kBars = 2 * kKRing + 2 * kVRing + 2 * 2;
+  static constexpr int kBars = 2 * kKRing + 2 * kVRing + 3 * 2;
   static constexpr int kSmem = 1024 + kOffBar + kBars * 8 + 16;
   static constexpr int kRaw = kPlain ? 1 : kTile * kRow / 16 / kLoadThreads;  // 16-byte pieces of a thread in a tile of codes
   static constexpr uint32_t kType = kBf16 ? 1u : 0u;
@@ -157,6 +157,7 @@ __device__ __forceinline__ void run_softmax(const Params& p, uint32_t s0, uint8_
   uint64_t* vempty = vfull + kVRing;
   uint64_t* sfull = vempty + kVRing + g;
   uint64_t* pvdone = sfull + 2;
+  uint64_t* ended = pvdone + 2;
   const float* rowf = reinterpret_cast<const float*>(smem + F::kOffRow);
   const int l0 = lane >> 2, c = lane & 3;
   const uint32_t tq = tmem + (static_cast<uint32_t>(quad * 32) << 16);
@@ -372,6 +373,15 @@ __device__ __forceinline__ void run_softmax(const Params& p, uint32_t s0, uint8_
   // ---- the group's partial ----
   const int mine = nt > g ? (nt - g + 1) / 2 : 0;  // tiles of this group
   if (mine && ok) ok = __all_sync(0xffffffffu, mbar_wait(pvdone, (mine - 1) & 1, ERR_PFX_WAIT));
+  if (!ok && quad == 0) {
+    // A wait ran out, whatever the limit in force: the products that this warp has issued still end before their shared and
+    // tensor memory is given back. One more commit tells when; they wait for nothing, and the bound is the longest limit.
+    if (elect_one()) mm4::umma_commit(ended);
+    __syncwarp();
+    const unsigned long long t0 = globaltimer_ns();
+    while (!mbar_try_wait(ended, 0) && globaltimer_ns() - t0 < kMaxWaitNs) {
+    }
+  }
   mm4::tc_fence_after();
   const int64_t first = (split * 2 + g) * kTile;
 #pragma unroll
@@ -416,7 +426,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attn_tc_kernel(const __gri
   uint64_t* vempty = vfull + kVRing;
   uint64_t* sfull = vempty + kVRing;  // [2] S of the group's tile is there
   uint64_t* pvdone = sfull + 2;       // [2] the group's last PV is complete
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pvdone + 2);
+  uint64_t* ended = pvdone + 2;       // [2] all that the group issued is complete: waited for where another wait ran out
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ended + 2);
 
   griddep_wait();
   griddep_launch_dependents();
@@ -444,6 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_attn_tc_kernel(const __gri
     for (int i = 0; i < 2; ++i) {
       mbar_init(sfull + i, 1);
       mbar_init(pvdone + i, 1);
+      mbar_init(ended + i, 1);
     }
     fence_mbar_init();
   }

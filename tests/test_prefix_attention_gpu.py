@@ -531,3 +531,24 @@ def test_largest_scale_and_no_query(fmt, kernel, scale):
         PrefixAttention(s.attn._keep[0], s.out, prefix=s.pre, prefix_len=s.prefix_len, own=s.own, own_len=s.own_len, scale=scale,
                         kernel=kernel)()
         s.check()
+
+
+@pytest.mark.parametrize("fmt", ["plain", "int8", "int4"])
+def test_tcgen05_kernel_with_the_shortest_wait_limit(fmt):
+    """With a limit of a microsecond, waits on products that are under way run out. The kernel ends them before it gives its
+    memory back: it reports the wait or, where none ran out, the right output, and the next call is as ever."""
+    s = Setup(40, 6, 2, 128, 9000, None, fmt, "fp16", seed=51, kernel="tc")
+    for _ in range(3):
+        rb._lib.set_wait_limit(1000)
+        try:
+            s.attn()
+            torch.cuda.synchronize()
+        finally:
+            rb._lib.set_wait_limit(0)
+        err = rb.device_error()
+        assert err in (0, rb._lib.DEVERR_PFX_WAIT)
+        if not err:
+            s.check()
+        s.attn()
+        assert rb.device_error() == 0
+        s.check()
